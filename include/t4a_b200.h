@@ -28,6 +28,7 @@
 #include <stddef.h>
 
 #include "t4a_b200/abi.h"
+#include "t4a_b200/cache.h"
 
 #ifdef __cplusplus
 extern "C" {

@@ -1,0 +1,70 @@
+// Launches of k_attend for one cache kind: the padded dim and the row warps pick the instance.
+#pragma once
+
+#include <atomic>
+
+#include "attention_mma.cuh"
+#include "runtime.h"
+
+namespace t4a {
+namespace cache {
+
+constexpr int kSms = 148;
+
+// Allows a kernel its dynamic shared memory, once a device.
+template <typename Kernel>
+int allow_shared(Kernel kernel, int bytes, std::atomic<unsigned long long>* done) {
+  int device = 0;
+  cudaError_t err = cudaGetDevice(&device);
+  const unsigned long long bit = 1ull << (device & 63);
+  if (err == cudaSuccess && device < 64 && (done->load(std::memory_order_acquire) & bit)) return T4A_OK;
+  if (err == cudaSuccess) err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err != cudaSuccess) {
+    runtime::last_error() = static_cast<int>(err);
+    cudaGetLastError();
+    return T4A_ERR_CUDA;
+  }
+  done->fetch_or(bit, std::memory_order_release);
+  return T4A_OK;
+}
+
+// With `blocks`, only says how many blocks to launch: as many as the SMs hold at once.
+template <int Kind, int Dim, int kRowWarps>
+int launch_one(const AttendArgs& a, cudaStream_t stream, int* blocks) {
+  using Shape = MmaShape<Kind, Dim>;
+  if (blocks != nullptr) {
+    *blocks = kSms * Shape::per_sm;
+    return T4A_OK;
+  }
+  static std::atomic<unsigned long long> allowed{0};
+  T4A_TRY(allow_shared(k_attend<Kind, Dim, kRowWarps>, Shape::shared, &allowed));
+  k_attend<Kind, Dim, kRowWarps><<<a.blocks, kMmaThreads, Shape::shared, stream>>>(a);
+  return runtime::check_launch();
+}
+
+template <int Kind, int Dim>
+int launch_rows_of(const AttendArgs& a, int row_warps, cudaStream_t stream, int* blocks) {
+  switch (row_warps) {
+    case 1: return launch_one<Kind, Dim, 1>(a, stream, blocks);
+    case 2: return launch_one<Kind, Dim, 2>(a, stream, blocks);
+    default: return launch_one<Kind, Dim, 4>(a, stream, blocks);
+  }
+}
+
+template <int Kind>
+int launch_mma(const AttendArgs& a, int padded, int row_warps, cudaStream_t stream, int* blocks) {
+  switch (padded) {
+    case 64: return launch_rows_of<Kind, 64>(a, row_warps, stream, blocks);
+    case 96: return launch_rows_of<Kind, 96>(a, row_warps, stream, blocks);
+    case 128: return launch_rows_of<Kind, 128>(a, row_warps, stream, blocks);
+    default: return launch_rows_of<Kind, 256>(a, row_warps, stream, blocks);
+  }
+}
+
+int launch_mma_f16(const AttendArgs& a, int padded, int row_warps, cudaStream_t stream, int* blocks);
+int launch_mma_bf16(const AttendArgs& a, int padded, int row_warps, cudaStream_t stream, int* blocks);
+int launch_mma_i8(const AttendArgs& a, int padded, int row_warps, cudaStream_t stream, int* blocks);
+int launch_mma_e4m3(const AttendArgs& a, int padded, int row_warps, cudaStream_t stream, int* blocks);
+
+}  // namespace cache
+}  // namespace t4a

@@ -1,0 +1,14 @@
+// The warp-level attention kernels of one cache kind (one file a kind, so that they build beside
+// each other).
+#include "attention_mma.cuh"
+#include "attention_launch.h"
+
+namespace t4a {
+namespace cache {
+
+int launch_mma_e4m3(const AttendArgs& a, int padded, int row_warps, cudaStream_t stream, int* blocks) {
+  return launch_mma<T4A_E4M3>(a, padded, row_warps, stream, blocks);
+}
+
+}  // namespace cache
+}  // namespace t4a

@@ -1,0 +1,232 @@
+// t4a_tree_attention: checks, the choice of the kernel, and the joining of parts.
+#include "attention_launch.h"
+
+namespace t4a {
+namespace cache {
+namespace {
+
+constexpr int kJoinThreads = 128;
+
+// One warp a query row of a head: nothing where one block had the whole unit; zeros where the
+// sequence has nothing to see; else its parts weighed by 2^(lse - max) in the blocks' order.
+__global__ void __launch_bounds__(kJoinThreads) k_join(const AttendArgs a) {
+  const int lane = threadIdx.x & 31;
+  const long long task = (static_cast<long long>(blockIdx.x) * kJoinThreads + threadIdx.x) >> 5;
+  const long long rows = static_cast<long long>(a.cache.heads) * a.rows;
+  const int b = static_cast<int>(task / rows);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (b >= a.batch) return;
+  const long long in = task - b * rows;
+  const int head = static_cast<int>(in / a.rows), row = static_cast<int>(in - static_cast<long long>(head) * a.rows);
+  const int row_tile = row / a.tile_rows, r = row - row_tile * a.tile_rows;
+  const long long tiles = sequence_tiles(a, b);
+  const int dim = a.cache.dim;
+  if (tiles == 0) {
+    const long long to = out_row(a, b, head, row);
+    for (int d = 2 * lane; d < dim; d += 64) store_out(a, to + d, 0.0f, 0.0f, true);
+    if (lane == 0) store_lse(a, b, head, row, -INFINITY);
+    return;
+  }
+  long long total, before;
+  count_tiles(a, b, &total, &before);
+  const long long quota = quota_of(a, total);
+  const long long start = before + (static_cast<long long>(head) * a.row_tiles + row_tile) * tiles;
+  const long long c0 = start / quota, c1 = (start + tiles - 1) / quota;
+  if (c0 == c1) return;
+  auto part = [&](long long c) { return (c * 2 + (c == c0 ? 1 : 0)) * a.tile_rows + r; };
+  float most = -INFINITY;
+  for (long long c = c0 + lane; c <= c1; c += 32) most = fmaxf(most, a.part_lse[part(c)]);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+  const float less = most == -INFINITY ? 0.0f : most;
+  float x[8], sum = 0.0f;  // columns 2 * lane + 64 * k and the next
+#pragma unroll
+  for (int k = 0; k < 8; ++k) x[k] = 0.0f;
+#pragma unroll 4
+  for (long long c = c0; c <= c1; ++c) {
+    const long long at = part(c);
+    const float w = exp2f(a.part_lse[at] - less);
+    sum += w;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int d = 2 * lane + 64 * k;
+      if (d >= dim) continue;
+      const float2 v = *reinterpret_cast<const float2*>(a.part_out + at * dim + d);
+      x[2 * k] += w * v.x;
+      x[2 * k + 1] += w * v.y;
+    }
+  }
+  const bool empty = sum == 0.0f;
+  const float over = empty ? 0.0f : 1.0f / sum;
+  const long long to = out_row(a, b, head, row);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int d = 2 * lane + 64 * k;
+    if (d < dim) store_out(a, to + d, x[2 * k] * over, x[2 * k + 1] * over, true);
+  }
+  if (lane == 0) store_lse(a, b, head, row, empty ? -INFINITY : less + log2f(sum));
+}
+
+struct Choice {
+  int padded, row_warps, rows;
+};
+
+// Row warps to a tile: as few as hold a head's rows, up to 4.
+Choice choose(int kind, int dim, int rows) {
+  Choice c;
+  c.padded = dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : 256;
+  c.row_warps = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  c.rows = 16 * c.row_warps;
+  (void)kind;
+  return c;
+}
+
+int dispatch(int kind, const AttendArgs& a, const Choice& c, cudaStream_t s, int* blocks) {
+  switch (kind) {
+    case T4A_F16: return launch_mma_f16(a, c.padded, c.row_warps, s, blocks);
+    case T4A_BF16: return launch_mma_bf16(a, c.padded, c.row_warps, s, blocks);
+    case T4A_I8: return launch_mma_i8(a, c.padded, c.row_warps, s, blocks);
+    default: return launch_mma_e4m3(a, c.padded, c.row_warps, s, blocks);
+  }
+}
+
+// What does not depend on buffers: shapes, the kernel's choice and its blocks.
+int plan_attention(int dtype, const t4a_kv_cache* cache, const t4a_cuda_layout* q, const t4a_cuda_layout* table,
+                   bool pointers, AttendArgs* a, Choice* choice, bool* empty) {
+  if (dtype != T4A_F16 && dtype != T4A_BF16) return T4A_ERR_UNSUPPORTED_DTYPE;
+  T4A_TRY(check_cache(cache, false, pointers, &a->cache));
+  if (!is_quantised(cache->kind) && cache->kind != dtype) return T4A_ERR_UNSUPPORTED_DTYPE;
+  T4A_TRY(plan::check_layout(q));
+  T4A_TRY(plan::check_layout(table));
+  if (q->rank != 4 || table->rank != 2) return T4A_ERR_RANK_LENGTH;
+  const long long heads = q->extents[1], nodes = q->extents[2], batch = q->extents[3];
+  if (q->extents[0] != a->cache.dim || table->extents[1] != batch) return T4A_ERR_SHAPE_MISMATCH;
+  *empty = heads == 0 || nodes == 0 || batch == 0;
+  if (*empty) return T4A_OK;
+  if (a->cache.heads == 0 || heads % a->cache.heads != 0) return T4A_ERR_SHAPE_MISMATCH;
+  if (a->cache.page_size == 0) return T4A_ERR_SHAPE_MISMATCH;
+  const long long group = heads / a->cache.heads;
+  long long rows, all;
+  if (plan::mul_overflows(nodes, group, &rows) || plan::mul_overflows(rows, batch, &all)) return T4A_ERR_OVERFLOW;
+  if (rows > (1 << 24) || batch > (1 << 24) || table->extents[0] > INT_MAX) return T4A_ERR_DOMAIN_TOO_LARGE;
+  a->q_bf16 = dtype == T4A_BF16;
+  a->batch = static_cast<int>(batch);
+  a->nodes = static_cast<int>(nodes);
+  a->group = static_cast<int>(group);
+  a->rows = static_cast<int>(rows);
+  a->table_pages = static_cast<int>(table->extents[0]);
+  *choice = choose(cache->kind, a->cache.dim, a->rows);
+  a->tile_rows = choice->rows;
+  a->row_tiles = (a->rows + choice->rows - 1) / choice->rows;
+  T4A_TRY(dispatch(cache->kind, *a, *choice, nullptr, &a->blocks));
+  return T4A_OK;
+}
+
+size_t workspace_of(const AttendArgs& a) {
+  return static_cast<size_t>(a.blocks) * 2 * a.tile_rows * (a.cache.dim + 1) * sizeof(float);
+}
+
+}  // namespace
+}  // namespace cache
+}  // namespace t4a
+
+extern "C" int t4a_tree_attention_workspace_bytes(int dtype, const t4a_kv_cache* cache,
+                                                  const t4a_cuda_layout* q_layout,
+                                                  const t4a_cuda_layout* table_layout, size_t* bytes) {
+  using namespace t4a::cache;
+  if (bytes == nullptr) return T4A_ERR_NULL_ARGUMENT;
+  AttendArgs a = {};
+  Choice choice;
+  bool empty;
+  T4A_TRY(plan_attention(dtype, cache, q_layout, table_layout, false, &a, &choice, &empty));
+  *bytes = empty ? 0 : workspace_of(a);
+  return T4A_OK;
+}
+
+extern "C" int t4a_tree_attention(void* stream, int dtype, const t4a_kv_cache* cache, void* out,
+                                  const t4a_cuda_layout* out_layout, long long out_len, float* lse,
+                                  const t4a_cuda_layout* lse_layout, long long lse_len, const void* q,
+                                  const t4a_cuda_layout* q_layout, long long q_len, const int* table,
+                                  const t4a_cuda_layout* table_layout, long long table_len, const int* context,
+                                  const int* nodes, const unsigned char* mask, const t4a_cuda_layout* mask_layout,
+                                  long long mask_len, float scale, void* workspace, size_t workspace_bytes) {
+  using namespace t4a;
+  using namespace t4a::cache;
+  AttendArgs a = {};
+  Choice choice;
+  bool empty;
+  T4A_TRY(plan_attention(dtype, cache, q_layout, table_layout, true, &a, &choice, &empty));
+  T4A_TRY(check_rows(q_layout, 4, q_len, 2));
+  T4A_TRY(check_rows(out_layout, 4, out_len, 2));
+  T4A_TRY(plan::require_destination(*out_layout));
+  for (int d = 0; d < 4; ++d)
+    if (out_layout->extents[d] != q_layout->extents[d]) return T4A_ERR_SHAPE_MISMATCH;
+  T4A_TRY(check_tensor(table_layout, 2, table_len, 4));
+  if (lse != nullptr) {
+    T4A_TRY(check_tensor(lse_layout, 3, lse_len, 4));
+    T4A_TRY(plan::require_destination(*lse_layout));
+    for (int d = 0; d < 3; ++d)
+      if (lse_layout->extents[d] != q_layout->extents[d + 1]) return T4A_ERR_SHAPE_MISMATCH;
+    if (!aligned(lse, 4)) return T4A_ERR_INVALID_STRIDE;
+    a.lse = lse + lse_layout->offset;
+    a.lse_head = lse_layout->strides[0];
+    a.lse_node = lse_layout->strides[1];
+    a.lse_batch = lse_layout->strides[2];
+  }
+  if (mask != nullptr) {
+    T4A_TRY(check_tensor(mask_layout, 3, mask_len, 1));
+    if (mask_layout->extents[0] != q_layout->extents[2] || mask_layout->extents[1] != q_layout->extents[2] ||
+        mask_layout->extents[2] != q_layout->extents[3])
+      return T4A_ERR_SHAPE_MISMATCH;
+    a.mask = mask + mask_layout->offset;
+    a.mask_seen = mask_layout->strides[0];
+    a.mask_node = mask_layout->strides[1];
+    a.mask_batch = mask_layout->strides[2];
+  }
+  if (empty) return T4A_OK;
+  if (q == nullptr || out == nullptr || context == nullptr || (table == nullptr && table_layout->extents[0] != 0))
+    return T4A_ERR_NULL_ARGUMENT;
+  if (!aligned(q, 2) || !aligned(out, 2) || !aligned(table, 4) || !aligned(context, 4) || !aligned(nodes, 4))
+    return T4A_ERR_INVALID_STRIDE;
+  if (workspace == nullptr || workspace_bytes < workspace_of(a)) return T4A_ERR_WORKSPACE;
+  if (!aligned(workspace, 16)) return T4A_ERR_WORKSPACE;
+  a.q = static_cast<const char*>(q) + q_layout->offset * 2;
+  a.q_head = q_layout->strides[1];
+  a.q_node = q_layout->strides[2];
+  a.q_batch = q_layout->strides[3];
+  a.out = static_cast<char*>(out) + out_layout->offset * 2;
+  a.out_head = out_layout->strides[1];
+  a.out_node = out_layout->strides[2];
+  a.out_batch = out_layout->strides[3];
+  a.pairs = rows_aligned(q, *q_layout, 2, 4) && rows_aligned(out, *out_layout, 2, 4);
+  a.table = table + table_layout->offset;
+  a.table_page = table_layout->strides[0];
+  a.table_batch = table_layout->strides[1];
+  a.context = context;
+  a.live_nodes = nodes;
+  a.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
+  a.part_out = static_cast<float*>(workspace);
+  a.part_lse = a.part_out + static_cast<size_t>(a.blocks) * 2 * a.tile_rows * a.cache.dim;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  T4A_TRY(dispatch(cache->kind, a, choice, s, nullptr));
+
+  const unsigned long long warps = static_cast<unsigned long long>(a.batch) * a.cache.heads * a.rows;
+  unsigned long long join_blocks;
+  T4A_TRY(plan::grid_of(warps, kJoinThreads / 32, &join_blocks));
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(static_cast<unsigned>(join_blocks));
+  config.blockDim = dim3(kJoinThreads);
+  config.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attr;
+  config.numAttrs = 1;
+  const cudaError_t err = cudaLaunchKernelEx(&config, k_join, a);
+  if (err != cudaSuccess) {
+    runtime::last_error() = static_cast<int>(err);
+    cudaGetLastError();
+    return T4A_ERR_CUDA;
+  }
+  return T4A_OK;
+}

@@ -1,0 +1,396 @@
+// Rows into and out of the paged cache (t4a_cache_write, t4a_cache_read).
+//
+// A row is dim <= 256 values, 16 to a thread: a group of 1, 2, 4, 8 or 16 neighbouring lanes
+// holds it in registers, so a quantised row is read once, its largest magnitude is a shuffle
+// tree over the group, and its codes leave as one 16-byte store a thread.
+//   write: a = max |x|, scale = a * (1/Q), code = nearest(x * (Q/a))
+//   read:  x = code * scale
+// Both are bound by memory: a written row costs dim * (source + code) + 4 bytes, and no
+// arithmetic comes near that (some 3 instructions a value against the 16 that the SMs issue in
+// the time a value's bytes take).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include "cache_plan.h"
+#include "runtime.h"
+
+namespace t4a {
+namespace cache {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kPerThread = 16;               // values of a row that a thread holds
+constexpr float kLeastRow = 7.8886091e-31f;  // 2^-100: Q / a stays finite above it
+
+// What one launch does: `rows` x heads rows of K (blockIdx.y 0) and of V (1).
+struct RowsArgs {
+  View cache;
+  unsigned char* act[2];  // key and value rows
+  long long act_head[2], act_row[2];  // strides in bytes
+  const void* slots;
+  long long slot_stride;
+  long long tasks;  // rows * heads
+  int wide_index;
+  int group_shift;  // log2 of the lanes of a row
+};
+
+__device__ __forceinline__ long long load_slot(const RowsArgs& a, long long n) {
+  return a.wide_index ? static_cast<const long long*>(a.slots)[n * a.slot_stride]
+                      : static_cast<long long>(static_cast<const int*>(a.slots)[n * a.slot_stride]);
+}
+
+// 32-byte loads and stores (sm_100's widest).
+__device__ __forceinline__ void load32(const void* p, uint32_t (&r)[8]) {
+  asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "l"(p));
+}
+
+__device__ __forceinline__ void store32(void* p, const uint32_t (&r)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
+// 16 values of type T at p as F32; `Vec`: p is 32-byte aligned.
+template <typename T, bool Vec>
+__device__ __forceinline__ void load16(const unsigned char* p, float (&x)[kPerThread]) {
+  if constexpr (Vec && sizeof(T) == 2) {
+    uint32_t r[8];
+    load32(p, r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const T* h = reinterpret_cast<const T*>(&r[i]);
+      x[2 * i] = static_cast<float>(h[0]);
+      x[2 * i + 1] = static_cast<float>(h[1]);
+    }
+  } else if constexpr (Vec) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      uint32_t r[8];
+      load32(p + 32 * half, r);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[8 * half + i] = __uint_as_float(r[i]);
+    }
+  } else {
+    const T* t = reinterpret_cast<const T*>(p);
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) x[i] = static_cast<float>(t[i]);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ T rounded(float x) {
+  if constexpr (sizeof(T) == 4) return x;
+  else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(x);
+  else return __float2bfloat16_rn(x);
+}
+
+template <typename T, bool Vec>
+__device__ __forceinline__ void store16(unsigned char* p, const float (&x)[kPerThread]) {
+  if constexpr (Vec && sizeof(T) == 2) {
+    uint32_t r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      T h[2] = {rounded<T>(x[2 * i]), rounded<T>(x[2 * i + 1])};
+      r[i] = *reinterpret_cast<const uint32_t*>(h);
+    }
+    store32(p, r);
+  } else if constexpr (Vec) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      uint32_t r[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(x[8 * half + i]);
+      store32(p + 32 * half, r);
+    }
+  } else {
+    T* t = reinterpret_cast<T*>(p);
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) t[i] = rounded<T>(x[i]);
+  }
+}
+
+// The two 8-bit codes.
+struct Int8 {
+  static constexpr float kMost = 127.0f;
+  static __device__ __forceinline__ uint32_t encode4(const float* x) {
+    uint32_t r = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = max(-127, min(127, __float2int_rn(x[i])));
+      r |= static_cast<uint32_t>(c & 0xff) << (8 * i);
+    }
+    return r;
+  }
+  static __device__ __forceinline__ void decode4(uint32_t r, float* x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = static_cast<float>(static_cast<signed char>(r >> (8 * i)));
+  }
+};
+
+struct E4m3 {
+  static constexpr float kMost = 448.0f;
+  static __device__ __forceinline__ uint32_t encode4(const float* x) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3);
+    return lo | (hi << 16);
+  }
+  static __device__ __forceinline__ void decode4(uint32_t r, float* x) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(r >> (16 * i)), __NV_E4M3);
+      const float2 f = __half22float2(__half2(h));
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
+  }
+};
+
+// Where task `task` of this block row lies: its activation row, and its slot split into page
+// and place.  Tasks run head by head within a row, as activations usually lie.
+struct Place {
+  const unsigned char* act;
+  long long page;
+  int place, head;
+  bool inside;
+};
+
+__device__ __forceinline__ Place find(const RowsArgs& a, long long task, int side) {
+  Place w;
+  long long n;
+  if (a.tasks <= 0x7fffffffll) {  // 32-bit divisions where they serve: a 64-bit one is some 100 instructions
+    const unsigned t = static_cast<unsigned>(task), q = t / static_cast<unsigned>(a.cache.heads);
+    n = q;
+    w.head = static_cast<int>(t - q * static_cast<unsigned>(a.cache.heads));
+  } else {
+    n = task / a.cache.heads;
+    w.head = static_cast<int>(task - n * a.cache.heads);
+  }
+  w.act = a.act[side] + n * a.act_row[side] + w.head * a.act_head[side];
+  const long long slot = load_slot(a, n);
+  w.inside = slot >= 0 && slot < a.cache.pages * a.cache.page_size;
+  if (slot <= 0x7fffffffll) {
+    const unsigned s = static_cast<unsigned>(slot), q = s / static_cast<unsigned>(a.cache.page_size);
+    w.page = q;
+    w.place = static_cast<int>(s - q * static_cast<unsigned>(a.cache.page_size));
+  } else {
+    w.page = slot / a.cache.page_size;
+    w.place = static_cast<int>(slot - w.page * a.cache.page_size);
+  }
+  return w;
+}
+
+template <typename T, typename Code, bool Vec>
+__global__ void __launch_bounds__(kThreads) k_write_quantised(const RowsArgs a) {
+  const int side = blockIdx.y, lane = threadIdx.x & ((1 << a.group_shift) - 1);
+  const Pages& to = side ? a.cache.v : a.cache.k;
+  const long long task = (static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x) >> a.group_shift;
+  const bool live = task < a.tasks && lane * kPerThread < a.cache.dim;
+  float x[kPerThread];
+  Place w;
+  w.inside = false;
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) x[i] = 0.0f;
+  if (live) {
+    w = find(a, task, side);
+    load16<T, Vec>(w.act + lane * kPerThread * sizeof(T), x);
+  }
+  // The largest magnitude as bits: for non-negative floats they order like integers, with
+  // infinity and then NaN on top, so that neither is lost as fmaxf would lose a NaN.
+  unsigned most = 0;
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
+  for (int d = 1; d < (1 << a.group_shift); d <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
+  if (!live || !w.inside) return;
+  const bool fine = most < 0x7f800000u;
+  const float top = __uint_as_float(most);
+  const bool kept = fine && top >= kLeastRow;
+  const float inverse = kept ? __fdiv_rn(Code::kMost, top) : 0.0f;
+  uint32_t code[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = kept ? x[4 * i + j] * inverse : 0.0f;
+    code[i] = Code::encode4(y);
+  }
+  unsigned char* row = to.base + w.page * to.page + w.place * to.place + w.head * to.head;
+  *reinterpret_cast<uint4*>(row + lane * kPerThread) = make_uint4(code[0], code[1], code[2], code[3]);
+  if (lane == 0)
+    to.scale[w.page * to.scale_page + w.place * to.scale_place + w.head * to.scale_head] =
+        kept ? top * (1.0f / Code::kMost) : fine ? 0.0f : __uint_as_float(0x7fc00000u);
+}
+
+// 16-bit rows (16-byte aligned) kept as they are, rounded from T.
+template <typename T, typename C, bool Vec>
+__global__ void __launch_bounds__(kThreads) k_write_plain(const RowsArgs a) {
+  const int side = blockIdx.y, lane = threadIdx.x & ((1 << a.group_shift) - 1);
+  const Pages& to = side ? a.cache.v : a.cache.k;
+  const long long task = (static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x) >> a.group_shift;
+  if (task >= a.tasks || lane * kPerThread >= a.cache.dim) return;
+  const Place w = find(a, task, side);
+  float x[kPerThread];
+  load16<T, Vec>(w.act + lane * kPerThread * sizeof(T), x);
+  if (!w.inside) return;
+  uint32_t r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    C h[2] = {rounded<C>(x[2 * i]), rounded<C>(x[2 * i + 1])};
+    r[i] = *reinterpret_cast<const uint32_t*>(h);
+  }
+  uint4* row = reinterpret_cast<uint4*>(to.base + w.page * to.page + w.place * to.place + w.head * to.head +
+                                        lane * kPerThread * sizeof(C));
+  row[0] = make_uint4(r[0], r[1], r[2], r[3]);
+  row[1] = make_uint4(r[4], r[5], r[6], r[7]);
+}
+
+template <typename T, typename Code, bool Vec>
+__global__ void __launch_bounds__(kThreads) k_read_quantised(const RowsArgs a) {
+  const int side = blockIdx.y, lane = threadIdx.x & ((1 << a.group_shift) - 1);
+  const Pages& from = side ? a.cache.v : a.cache.k;
+  const long long task = (static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x) >> a.group_shift;
+  if (task >= a.tasks || lane * kPerThread >= a.cache.dim) return;
+  const Place w = find(a, task, side);
+  float x[kPerThread];
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) x[i] = 0.0f;
+  if (w.inside) {
+    const uint4 code = *reinterpret_cast<const uint4*>(from.base + w.page * from.page + w.place * from.place +
+                                                       w.head * from.head + lane * kPerThread);
+    const float scale =
+        from.scale[w.page * from.scale_page + w.place * from.scale_place + w.head * from.scale_head];
+    const uint32_t r[4] = {code.x, code.y, code.z, code.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) Code::decode4(r[i], x + 4 * i);
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) x[i] *= scale;
+  }
+  store16<T, Vec>(const_cast<unsigned char*>(w.act) + lane * kPerThread * sizeof(T), x);
+}
+
+template <typename T, typename C, bool Vec>
+__global__ void __launch_bounds__(kThreads) k_read_plain(const RowsArgs a) {
+  const int side = blockIdx.y, lane = threadIdx.x & ((1 << a.group_shift) - 1);
+  const Pages& from = side ? a.cache.v : a.cache.k;
+  const long long task = (static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x) >> a.group_shift;
+  if (task >= a.tasks || lane * kPerThread >= a.cache.dim) return;
+  const Place w = find(a, task, side);
+  float x[kPerThread];
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) x[i] = 0.0f;
+  if (w.inside) {
+    const uint4* row = reinterpret_cast<const uint4*>(from.base + w.page * from.page + w.place * from.place +
+                                                      w.head * from.head + lane * kPerThread * sizeof(C));
+    const uint4 lo = row[0], hi = row[1];
+    const uint32_t r[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const C* h = reinterpret_cast<const C*>(&r[i]);
+      x[2 * i] = static_cast<float>(h[0]);
+      x[2 * i + 1] = static_cast<float>(h[1]);
+    }
+  }
+  store16<T, Vec>(const_cast<unsigned char*>(w.act) + lane * kPerThread * sizeof(T), x);
+}
+
+template <typename T, bool Vec>
+void launch_rows(const RowsArgs& a, int kind, bool write, dim3 grid, cudaStream_t s) {
+  if (write) {
+    switch (kind) {
+      case T4A_I8: k_write_quantised<T, Int8, Vec><<<grid, kThreads, 0, s>>>(a); break;
+      case T4A_E4M3: k_write_quantised<T, E4m3, Vec><<<grid, kThreads, 0, s>>>(a); break;
+      case T4A_F16: k_write_plain<T, __half, Vec><<<grid, kThreads, 0, s>>>(a); break;
+      default: k_write_plain<T, __nv_bfloat16, Vec><<<grid, kThreads, 0, s>>>(a); break;
+    }
+  } else {
+    switch (kind) {
+      case T4A_I8: k_read_quantised<T, Int8, Vec><<<grid, kThreads, 0, s>>>(a); break;
+      case T4A_E4M3: k_read_quantised<T, E4m3, Vec><<<grid, kThreads, 0, s>>>(a); break;
+      case T4A_F16: k_read_plain<T, __half, Vec><<<grid, kThreads, 0, s>>>(a); break;
+      default: k_read_plain<T, __nv_bfloat16, Vec><<<grid, kThreads, 0, s>>>(a); break;
+    }
+  }
+}
+
+int run_rows(void* stream, int dtype, int index_dtype, const t4a_kv_cache* cache, void* const act[2],
+             const t4a_cuda_layout* const layout[2], const long long len[2], const void* slots,
+             const t4a_cuda_layout* slots_layout, long long slots_len, bool write) {
+  RowsArgs a;
+  T4A_TRY(check_cache(cache, write, true, &a.cache));
+  if (!is_row_dtype(dtype)) return T4A_ERR_UNSUPPORTED_DTYPE;
+  if (index_dtype != T4A_CUDA_I32 && index_dtype != T4A_CUDA_I64) return T4A_ERR_UNSUPPORTED_DTYPE;
+  T4A_TRY(check_tensor(slots_layout, 1, slots_len, index_dtype == T4A_CUDA_I64 ? 8 : 4));
+  const int esize = element_size(dtype);
+  const long long rows = slots_layout->extents[0];
+  bool vec = true;
+  for (int side = 0; side < 2; ++side) {
+    T4A_TRY(check_rows(layout[side], 3, len[side], esize));
+    if (!write) T4A_TRY(plan::require_destination(*layout[side]));
+    if (layout[side]->extents[0] != a.cache.dim || layout[side]->extents[1] != a.cache.heads ||
+        layout[side]->extents[2] != rows)
+      return T4A_ERR_SHAPE_MISMATCH;
+    if (rows != 0 && a.cache.heads != 0 && act[side] == nullptr) return T4A_ERR_NULL_ARGUMENT;
+    if (!aligned(act[side], esize)) return T4A_ERR_INVALID_STRIDE;
+    a.act[side] = static_cast<unsigned char*>(act[side]) + layout[side]->offset * esize;
+    a.act_head[side] = layout[side]->strides[1] * esize;
+    a.act_row[side] = layout[side]->strides[2] * esize;
+    vec = vec && rows_aligned(act[side], *layout[side], esize, 32);
+  }
+  if (plan::mul_overflows(rows, a.cache.heads, &a.tasks)) return T4A_ERR_OVERFLOW;
+  if (a.tasks == 0) return T4A_OK;
+  if (slots == nullptr) return T4A_ERR_NULL_ARGUMENT;
+  a.slots = static_cast<const char*>(slots) + slots_layout->offset * (index_dtype == T4A_CUDA_I64 ? 8 : 4);
+  a.slot_stride = slots_layout->strides[0];
+  a.wide_index = index_dtype == T4A_CUDA_I64;
+  if (a.cache.page_size == 0) a.cache.page_size = 1, a.cache.pages = 0;  // no slot is inside; no division by zero
+  a.group_shift = 0;
+  while ((kPerThread << a.group_shift) < a.cache.dim) ++a.group_shift;
+  unsigned long long blocks;
+  T4A_TRY(plan::grid_of(a.tasks, kThreads >> a.group_shift, &blocks));
+  const dim3 grid(static_cast<unsigned>(blocks), 2);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case T4A_CUDA_F32:
+      vec ? launch_rows<float, true>(a, cache->kind, write, grid, s)
+          : launch_rows<float, false>(a, cache->kind, write, grid, s);
+      break;
+    case T4A_F16:
+      vec ? launch_rows<__half, true>(a, cache->kind, write, grid, s)
+          : launch_rows<__half, false>(a, cache->kind, write, grid, s);
+      break;
+    default:
+      vec ? launch_rows<__nv_bfloat16, true>(a, cache->kind, write, grid, s)
+          : launch_rows<__nv_bfloat16, false>(a, cache->kind, write, grid, s);
+      break;
+  }
+  return runtime::check_launch();
+}
+
+}  // namespace
+}  // namespace cache
+}  // namespace t4a
+
+extern "C" int t4a_cache_write(void* stream, int dtype, int index_dtype, const t4a_kv_cache* cache, const void* key,
+                               const t4a_cuda_layout* key_layout, long long key_len, const void* value,
+                               const t4a_cuda_layout* value_layout, long long value_len, const void* slots,
+                               const t4a_cuda_layout* slots_layout, long long slots_len) {
+  void* const act[2] = {const_cast<void*>(key), const_cast<void*>(value)};
+  const t4a_cuda_layout* const layout[2] = {key_layout, value_layout};
+  const long long len[2] = {key_len, value_len};
+  return t4a::cache::run_rows(stream, dtype, index_dtype, cache, act, layout, len, slots, slots_layout, slots_len,
+                              true);
+}
+
+extern "C" int t4a_cache_read(void* stream, int dtype, int index_dtype, const t4a_kv_cache* cache, void* key,
+                              const t4a_cuda_layout* key_layout, long long key_len, void* value,
+                              const t4a_cuda_layout* value_layout, long long value_len, const void* slots,
+                              const t4a_cuda_layout* slots_layout, long long slots_len) {
+  void* const act[2] = {key, value};
+  const t4a_cuda_layout* const layout[2] = {key_layout, value_layout};
+  const long long len[2] = {key_len, value_len};
+  return t4a::cache::run_rows(stream, dtype, index_dtype, cache, act, layout, len, slots, slots_layout, slots_len,
+                              false);
+}

@@ -1,0 +1,622 @@
+// Verification of a tree of drafted tokens against the target's logits (t4a_verify_drafts).
+//
+// One cluster of 1, 2, 4 or 8 blocks walks one sequence's tree.  Only the rows of nodes that are
+// taken are read: a tree of 32 nodes has some 4 on its path, so reading ahead all rows at once
+// would read 8 times as much.  At a node
+//   r = e / Z,  e_x = exp(l_x - m),  m = max l,  Z = sum e
+// is spread over the blocks' shared memory, each thread keeping the same vectors of the row in
+// every pass, so that no pass waits for another thread's values.  The blocks exchange one record
+// (maximum, sum, argmax key) per reduction through distributed shared memory; all of them then
+// take the same decisions from the same numbers.
+//   Without a draft the children's tokens are left out of the row's own sum, and
+//   mass = Z_rest + (children not yet turned down): sums of positive terms only, where Z - e_x
+//   would cancel when a likely token is turned down.  So a node costs one exchange, whatever the
+//   number of its children.
+//   With a draft each child turned down costs one pass, r <- max(r - q, 0), and an exchange.  The
+//   next child's r is a scalar recursion from the masses, which every block does for itself.
+// Bound by latency: a node is a dependent load of its row (64 KB a block at 128k F32), two block
+// reductions and a cluster barrier; sequences run beside each other.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "cache_plan.h"
+#include "runtime.h"
+
+namespace t4a {
+namespace cache {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMostCluster = 8;
+constexpr int kMostNodes = 1024;
+constexpr int kMostSlice = 49152;  // values of a row that a block keeps, F32
+
+struct VerifyArgs {
+  const void* logits;
+  long long logits_node, logits_batch;  // strides in elements
+  const float* draft;
+  long long draft_node, draft_batch;
+  const float* race;
+  long long race_stride, race_batch;
+  const int* tokens;
+  const int* parents;
+  const float* uniforms;
+  int* count;
+  int* path;
+  int* said;
+  float* logs;
+  long long vocab;
+  int nodes, greedy, slots;  // slots: vectors of a row that a block keeps
+  float inverse_temperature;
+};
+
+struct Record {
+  float m, s;
+  unsigned long long key;
+};
+
+// Floats in their order as unsigned integers.
+__device__ __forceinline__ unsigned ordered(float x) {
+  const unsigned b = __float_as_uint(x);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+// Lowest index first among equal values.
+__device__ __forceinline__ unsigned long long make_key(unsigned value, long long index) {
+  return (static_cast<unsigned long long>(value) << 32) | (0xffffffffu - static_cast<unsigned>(index));
+}
+
+__device__ __forceinline__ long long key_index(unsigned long long key) {
+  return 0xffffffffu - static_cast<unsigned>(key);
+}
+
+__device__ __forceinline__ unsigned cluster_rank() {
+  unsigned r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+
+__device__ __forceinline__ unsigned cluster_blocks() {
+  unsigned r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+struct Shared {
+  Record exchange[2][kMostCluster];
+  float warp_m[kWarps];
+  float warp_s[kWarps];
+  unsigned long long warp_key[kWarps];
+  int children, child[kMostNodes], token[kMostNodes], parent[kMostNodes];
+  float child_x[kMostNodes];
+  float mass[kMostNodes];  // without a draft: of what the children from here on hold; else the passes' sums
+  int elder[kMostNodes];   // the first child with the same token
+  int mark[kMostNodes];    // of a child that is its own elder: the count of resets when it was turned down, plus 1
+  int decided;             // thread 0's decision, for the block
+  float total;
+  int reset_at;
+};
+
+template <typename T>
+class Walk {
+ public:
+  static constexpr int kVec = 16 / sizeof(T);
+
+  __device__ Walk(const VerifyArgs& args, Shared& shared, float* kept)
+      : a(args), sh(shared), x(kept), rank(cluster_rank()), blocks(cluster_blocks()), b(blockIdx.x / cluster_blocks()) {}
+
+  __device__ void run() {
+    const int tid = threadIdx.x;
+    for (int i = tid; i < a.nodes; i += kThreads) {
+      sh.token[i] = a.tokens[static_cast<long long>(b) * a.nodes + i];
+      sh.parent[i] = a.parents[static_cast<long long>(b) * a.nodes + i];
+    }
+    __syncthreads();
+    if (blocks > 1) cluster_barrier();  // every block runs before its shared memory is written from another
+    int at = 0, taken = 0;
+    while (true) {
+      find_children(at);
+      load_row(at);
+      const Record all = sum_row();
+      // -infinity for a row without any finite logit: it then has no probability anywhere.
+      int next;
+      float total;
+      if (a.greedy) {
+        total = all.s;
+        next = -1;
+        for (int c = 0; c < sh.children && next < 0; ++c)
+          if (sh.token[sh.child[c]] == key_index(all.key)) next = c;
+      } else if (a.draft == nullptr) {
+        next = choose_plain(all, &total);
+      } else {
+        total = all.s;
+        next = choose_against_draft(at, all);
+      }
+      if (next < 0) {
+        finish(at, taken, all, total);
+        return;
+      }
+      if (rank == 0 && tid == 0) {
+        const long long o = static_cast<long long>(b) * a.nodes + taken;
+        a.path[o] = sh.child[next];
+        a.said[o] = sh.token[sh.child[next]];
+        if (a.logs) a.logs[o] = log_of(sh.child_x[next], all.m, total);
+      }
+      at = sh.child[next];
+      ++taken;
+      __syncthreads();  // the child list is rewritten
+    }
+  }
+
+ private:
+  const VerifyArgs& a;
+  Shared& sh;
+  float* x;  // [kVec][slots]: element e of vector j at e * slots + j, so that lanes touch neighbours
+  const unsigned rank, blocks;
+  const int b;
+  int turn = 0;      // exchanges so far
+  const T* row = nullptr;
+  int skew = 0;      // the row's first element within its 16-byte vector
+  long long first = 0, vectors = 0;  // this block's vectors of the row
+  float local_m = 0.0f;  // this block's maximum
+
+  __device__ float fix(float v) const { return v == v ? v * (a.greedy ? 1.0f : a.inverse_temperature) : -INFINITY; }
+
+  // exp(v - m), with the whole mass on infinite entries where there are some.
+  static __device__ __forceinline__ float weight(float v, float m) {
+    return v == m ? (m == -INFINITY ? 0.0f : 1.0f) : expf(v - m);
+  }
+
+  static __device__ __forceinline__ float log_of(float v, float m, float total) {
+    return v == -INFINITY ? -INFINITY : (v == m ? 0.0f : v - m) - logf(total);
+  }
+
+  __device__ void find_children(int at) {
+    const int lane = threadIdx.x & 31;
+    if (threadIdx.x < 32) {
+      int n = 0;
+      for (int i0 = at + 1; i0 < a.nodes; i0 += 32) {
+        const int i = i0 + lane;
+        const bool mine = i < a.nodes && sh.parent[i] == at;
+        const unsigned votes = __ballot_sync(0xffffffffu, mine);
+        if (mine) sh.child[n + __popc(votes & ((1u << lane) - 1))] = i;
+        n += __popc(votes);
+      }
+      if (lane == 0) sh.children = n;
+    }
+    __syncthreads();
+  }
+
+  __device__ bool in_vocab(int token) const { return token >= 0 && token < a.vocab; }
+
+  // The node's row into `x`, its scaled values; the block's maximum and, when greedy, its argmax.
+  __device__ void load_row(int at) {
+    const int tid = threadIdx.x;
+    row = static_cast<const T*>(a.logits) + static_cast<long long>(b) * a.logits_batch +
+          static_cast<long long>(at) * a.logits_node;
+    skew = static_cast<int>((reinterpret_cast<uintptr_t>(row) / sizeof(T)) % kVec);
+    const long long all = (a.vocab + skew + kVec - 1) / kVec;
+    first = static_cast<long long>(rank) * a.slots;
+    vectors = max(0ll, min(static_cast<long long>(a.slots), all - first));
+    for (int c = tid; c < sh.children; c += kThreads) {
+      const int token = sh.token[sh.child[c]];
+      sh.child_x[c] = in_vocab(token) ? fix(static_cast<float>(row[token])) : -INFINITY;
+    }
+    float m = -INFINITY;
+    long long best = 0;
+    bool any = false;
+    constexpr int kBatch = 4;
+    for (long long j0 = tid; j0 < vectors; j0 += kBatch * kThreads) {
+      uint4 raw[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const long long j = j0 + u * kThreads, i = (first + j) * kVec - skew;
+        if (j >= vectors) continue;
+        if (i >= 0 && i + kVec <= a.vocab) {
+          raw[u] = __ldcs(reinterpret_cast<const uint4*>(row + i));
+        } else {  // the row's ragged ends
+          T* r = reinterpret_cast<T*>(&raw[u]);
+#pragma unroll
+          for (int e = 0; e < kVec; ++e)
+            r[e] = i + e >= 0 && i + e < a.vocab ? row[i + e] : static_cast<T>(-INFINITY);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const long long j = j0 + u * kThreads, i = (first + j) * kVec - skew;
+        if (j >= vectors) continue;
+        const T* r = reinterpret_cast<const T*>(&raw[u]);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          const float v = fix(static_cast<float>(r[e]));
+          x[e * a.slots + j] = v;
+          if (i + e >= 0 && i + e < a.vocab && (v > m || !any)) {
+            m = v;
+            best = i + e;
+            any = true;
+          }
+        }
+      }
+    }
+    // Indices rise along a thread's walk, so `best` is its lowest.
+    unsigned long long key = any ? make_key(ordered(m), best) : 0;
+    block_reduce(&m, nullptr, &key);
+    local_m = m;
+    greedy_key = key;
+  }
+
+  unsigned long long greedy_key = 0;
+
+  // The sum of the row's weights over the cluster.  Without a draft (and unless greedy) the
+  // children's tokens are left out: `x` then holds -infinity at them.  With a draft `x` holds the
+  // weights themselves.
+  __device__ Record sum_row() {
+    const int tid = threadIdx.x;
+    const bool apart = !a.greedy && a.draft == nullptr, keep = !a.greedy && a.draft != nullptr;
+    if (apart) {
+      for (int c = tid; c < sh.children; c += kThreads) {
+        const int token = sh.token[sh.child[c]];
+        if (!in_vocab(token)) continue;
+        const long long v = (token + static_cast<long long>(skew)) / kVec - first;
+        if (v >= 0 && v < vectors) x[(token + skew) % kVec * a.slots + v] = -INFINITY;
+      }
+      __syncthreads();
+    }
+    float s = 0.0f;
+    for (long long j = tid; j < vectors; j += kThreads)
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        const float w = weight(x[e * a.slots + j], local_m);
+        s += w;
+        if (keep) x[e * a.slots + j] = w;
+      }
+    block_reduce(nullptr, &s, nullptr);
+    Record mine;
+    mine.m = local_m;
+    mine.s = s;
+    mine.key = greedy_key;
+    return exchange(mine);
+  }
+
+  // Block-wide maximum, sum and largest key, in a fixed order; every thread gets them.
+  __device__ void block_reduce(float* m, float* s, unsigned long long* key) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+      if (m) *m = fmaxf(*m, __shfl_xor_sync(0xffffffffu, *m, d));
+      if (s) *s += __shfl_xor_sync(0xffffffffu, *s, d);
+      if (key) *key = max(*key, __shfl_xor_sync(0xffffffffu, *key, d));
+    }
+    __syncthreads();
+    if (lane == 0) {
+      if (m) sh.warp_m[warp] = *m;
+      if (s) sh.warp_s[warp] = *s;
+      if (key) sh.warp_key[warp] = *key;
+    }
+    __syncthreads();
+    if (m) *m = sh.warp_m[0];
+    if (s) *s = sh.warp_s[0];
+    if (key) *key = sh.warp_key[0];
+    for (int w = 1; w < kWarps; ++w) {
+      if (m) *m = fmaxf(*m, sh.warp_m[w]);
+      if (s) *s += sh.warp_s[w];
+      if (key) *key = max(*key, sh.warp_key[w]);
+    }
+  }
+
+  // All blocks' records into every block, then their combination in rank order.  Two buffers in
+  // turn: a block writes into one again only after a barrier that every block reached after its
+  // reads of it.
+  __device__ Record exchange(const Record& mine) {
+    const int buffer = turn++ & 1;
+    if (blocks == 1) return mine;
+    if (threadIdx.x < blocks) {
+      const unsigned local = static_cast<unsigned>(__cvta_generic_to_shared(&sh.exchange[buffer][rank]));
+      unsigned remote;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(threadIdx.x));
+      asm volatile("st.shared::cluster.v2.f32 [%0], {%1,%2};" ::"r"(remote), "f"(mine.m), "f"(mine.s) : "memory");
+      asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(remote + 8), "l"(mine.key) : "memory");
+    }
+    __syncwarp();
+    cluster_barrier();
+    Record all = sh.exchange[buffer][0];
+    for (unsigned r = 1; r < blocks; ++r) all.m = fmaxf(all.m, sh.exchange[buffer][r].m);
+    all.s = 0.0f;
+    for (unsigned r = 0; r < blocks; ++r) {
+      const Record& o = sh.exchange[buffer][r];
+      all.s += o.s * weight(o.m, all.m);
+      all.key = max(all.key, o.key);
+    }
+    return all;
+  }
+
+  // The first child taken, -1 without one; *total is the row's whole sum.
+  __device__ int choose_plain(const Record& all, float* total) {
+    const int n = sh.children;
+    for (int c = threadIdx.x; c < n; c += kThreads) {
+      int first_one = c;
+      for (int k = 0; k < c && first_one == c; ++k)
+        if (sh.token[sh.child[k]] == sh.token[sh.child[c]]) first_one = k;
+      sh.elder[c] = first_one;
+      sh.mark[c] = 0;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      float behind = 0.0f;  // what the children from i on hold, a token once
+      for (int i = n - 1; i >= 0; --i) {
+        sh.mass[i] = behind;
+        if (sh.elder[i] == i) behind += weight(sh.child_x[i], all.m);
+      }
+      const float whole = all.s + behind;
+      float mass = whole;
+      int from = 0, resets = 0, found = -1;
+      for (int i = 0; i < n && whole > 0.0f; ++i) {
+        const int e = sh.elder[i];
+        const float r = sh.mark[e] == resets + 1 ? 0.0f : weight(sh.child_x[i], all.m);
+        if (a.uniforms[static_cast<long long>(b) * a.nodes + sh.child[i]] * mass < r) {
+          found = i;
+          break;
+        }
+        sh.mark[e] = resets + 1;
+        if (resets == 0) {
+          mass = all.s + sh.mass[i];
+        } else {
+          mass = all.s;
+          for (int k = 0; k < n; ++k)
+            if (sh.elder[k] == k && sh.mark[k] != resets + 1) mass += weight(sh.child_x[k], all.m);
+        }
+        if (!(mass > 0.0f)) {  // nothing is left: the node's own softmax again
+          mass = whole;
+          from = i + 1;
+          ++resets;
+        }
+      }
+      sh.decided = found;
+      sh.total = whole;
+      sh.reset_at = from;
+    }
+    __syncthreads();
+    *total = sh.total;
+    return sh.decided;
+  }
+
+  __device__ int choose_against_draft(int at, const Record& all) {
+    const float* q = a.draft + static_cast<long long>(b) * a.draft_batch + static_cast<long long>(at) * a.draft_node;
+    factor = weight(local_m, all.m) / all.s;
+    int masses = 0;  // passes since the node's softmax
+    for (int c = 0; c < sh.children; ++c) {
+      const int token = sh.token[sh.child[c]];
+      const float qx = in_vocab(token) ? q[token] : 0.0f;
+      float r = weight(sh.child_x[c], all.m) / all.s;
+      for (int i = 0; i < masses; ++i) r = fmaxf(r - qx, 0.0f) / sh.mass[i];
+      if (in_vocab(token) && a.uniforms[static_cast<long long>(b) * a.nodes + sh.child[c]] * qx < r) return c;
+      Record mine;
+      mine.m = 0.0f;
+      mine.s = subtract(q);
+      mine.key = 0;
+      const float mass = exchange(mine).s;
+      if (mass > 0.0f) {
+        factor = 1.0f / mass;
+        if (threadIdx.x == 0) sh.mass[masses] = mass;
+        ++masses;
+        __syncthreads();
+      } else {
+        masses = 0;
+        for (long long j = threadIdx.x; j < vectors; j += kThreads)
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) {
+            const long long i = (first + j) * kVec - skew + e;
+            x[e * a.slots + j] = i >= 0 && i < a.vocab ? weight(fix(static_cast<float>(row[i])), local_m) : 0.0f;
+          }
+        factor = weight(local_m, all.m) / all.s;
+      }
+    }
+    return -1;
+  }
+
+  float factor = 1.0f;  // x * factor is r
+
+  // 16 bytes of F32 at once where they lie so.
+  static __device__ __forceinline__ void load_f32(const float* p, bool whole, long long i, long long n, float (&v)[kVec],
+                                                  long long stride = 1) {
+    if (whole && stride == 1 && (reinterpret_cast<uintptr_t>(p + i) & 15) == 0) {
+#pragma unroll
+      for (int h = 0; h < kVec; h += 4) {
+        const float4 f = __ldcs(reinterpret_cast<const float4*>(p + i + h));
+        v[h] = f.x;
+        v[h + 1] = f.y;
+        v[h + 2] = f.z;
+        v[h + 3] = f.w;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) v[e] = i + e >= 0 && i + e < n ? p[(i + e) * stride] : 0.0f;
+    }
+  }
+
+  // x <- max(x * factor - q, 0); the block's sum of it.
+  __device__ float subtract(const float* q) {
+    float s = 0.0f;
+    for (long long j = threadIdx.x; j < vectors; j += kThreads) {
+      const long long i = (first + j) * kVec - skew;
+      float v[kVec];
+      load_f32(q, i >= 0 && i + kVec <= a.vocab, i, a.vocab, v);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        const float r = fmaxf(x[e * a.slots + j] * factor - v[e], 0.0f);
+        x[e * a.slots + j] = r;
+        s += r;
+      }
+    }
+    block_reduce(nullptr, &s, nullptr);
+    return s;
+  }
+
+  // The last token, its log-probability, and the places that nothing was written to.
+  __device__ void finish(int at, int taken, const Record& all, float total) {
+    const int tid = threadIdx.x;
+    long long last;
+    if (a.greedy) {
+      last = key_index(all.key);
+    } else {
+      const float* race = a.race + static_cast<long long>(b) * a.race_batch;
+      unsigned long long key = rank == 0 && tid == 0 ? make_key(0, 0) : 0;
+      for (long long j = tid; j < vectors; j += kThreads) {
+        const long long i = (first + j) * kVec - skew;
+        float v[kVec];
+        load_f32(race, i >= 0 && i + kVec <= a.vocab, i, a.vocab, v, a.race_stride);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          const float r = a.draft ? x[e * a.slots + j] * factor : weight(x[e * a.slots + j], all.m);
+          const float score = r * v[e];
+          if (score > 0.0f) key = max(key, make_key(__float_as_uint(score), i + e));
+        }
+      }
+      if (a.draft == nullptr && rank == 0 && tid == 0) {
+        // Children turned down before the node's softmax was taken again are back in it.
+        for (int c = 0; c < sh.reset_at; ++c) {
+          const int token = sh.token[sh.child[c]];
+          bool back = in_vocab(token);
+          for (int k = sh.reset_at; k < sh.children && back; ++k) back = sh.token[sh.child[k]] != token;
+          if (!back) continue;
+          const float score = weight(sh.child_x[c], all.m) * race[token * a.race_stride];
+          if (score > 0.0f) key = max(key, make_key(__float_as_uint(score), token));
+        }
+      }
+      block_reduce(nullptr, nullptr, &key);
+      Record mine;
+      mine.m = mine.s = 0.0f;
+      mine.key = key;
+      last = key_index(exchange(mine).key);
+    }
+    if (rank != 0) return;
+    const long long o = static_cast<long long>(b) * a.nodes;
+    for (int i = tid; i < a.nodes; i += kThreads) {
+      if (i >= taken) a.path[o + i] = -1;
+      if (i > taken) a.said[o + i] = -1;
+      if (i > taken && a.logs) a.logs[o + i] = 0.0f;
+    }
+    if (tid == 0) {
+      a.count[b] = taken;
+      a.said[o + taken] = static_cast<int>(last);
+      if (a.logs) a.logs[o + taken] = log_of(fix(static_cast<float>(row[last])), all.m, total);
+    }
+  }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) k_verify(const VerifyArgs a) {
+  extern __shared__ __align__(16) unsigned char raw[];
+  __shared__ Shared sh;
+  Walk<T> walk(a, sh, reinterpret_cast<float*>(raw));
+  walk.run();
+}
+
+template <typename T>
+int launch_verify(const VerifyArgs& a, int batch, int blocks, cudaStream_t stream) {
+  const size_t smem = static_cast<size_t>(a.slots) * Walk<T>::kVec * 4;
+  const cudaError_t set = cudaFuncSetAttribute(k_verify<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               kMostSlice * 4);
+  if (set != cudaSuccess) {
+    runtime::last_error() = static_cast<int>(set);
+    return T4A_ERR_CUDA;
+  }
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(static_cast<unsigned>(batch) * blocks);
+  config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = blocks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  config.attrs = attr;
+  config.numAttrs = 1;
+  const cudaError_t err = cudaLaunchKernelEx(&config, k_verify<T>, a);
+  if (err != cudaSuccess) {
+    runtime::last_error() = static_cast<int>(err);
+    cudaGetLastError();
+    return T4A_ERR_CUDA;
+  }
+  return T4A_OK;
+}
+
+}  // namespace
+}  // namespace cache
+}  // namespace t4a
+
+extern "C" int t4a_verify_drafts(void* stream, int dtype, const void* logits, const t4a_cuda_layout* logits_layout,
+                                 long long logits_len, const int* tokens, const int* parents, const float* uniforms,
+                                 const float* draft, const t4a_cuda_layout* draft_layout, long long draft_len,
+                                 const float* race, const t4a_cuda_layout* race_layout, long long race_len,
+                                 float temperature, int* count, int* path, int* said, float* logs) {
+  using namespace t4a;
+  using namespace t4a::cache;
+  if (!is_row_dtype(dtype)) return T4A_ERR_UNSUPPORTED_DTYPE;
+  const int esize = element_size(dtype);
+  T4A_TRY(check_rows(logits_layout, 3, logits_len, esize));
+  const long long vocab = logits_layout->extents[0], nodes = logits_layout->extents[1],
+                  batch = logits_layout->extents[2];
+  if (batch == 0) return T4A_OK;
+  if (vocab == 0 || nodes == 0) return T4A_ERR_SHAPE_MISMATCH;  // every sequence says a token
+  if (!(temperature >= 0.0f) || temperature > 3.0e38f || (temperature > 0.0f && temperature < 1e-30f))
+    return T4A_ERR_UNSUPPORTED_OP;
+  VerifyArgs a = {};
+  a.greedy = temperature == 0.0f;
+  if (nodes > kMostNodes) return T4A_ERR_DOMAIN_TOO_LARGE;
+  if (logits == nullptr || tokens == nullptr || parents == nullptr || count == nullptr || path == nullptr ||
+      said == nullptr)
+    return T4A_ERR_NULL_ARGUMENT;
+  if (!aligned(logits, esize)) return T4A_ERR_INVALID_STRIDE;
+  if (!a.greedy) {
+    if (uniforms == nullptr || race == nullptr) return T4A_ERR_NULL_ARGUMENT;
+    T4A_TRY(check_tensor(race_layout, 2, race_len, 4));
+    if (race_layout->extents[0] != vocab || race_layout->extents[1] != batch) return T4A_ERR_SHAPE_MISMATCH;
+    a.race = race + race_layout->offset;
+    a.race_stride = race_layout->strides[0];
+    a.race_batch = race_layout->strides[1];
+    if (draft != nullptr) {
+      T4A_TRY(check_rows(draft_layout, 3, draft_len, 4));
+      for (int d = 0; d < 3; ++d)
+        if (draft_layout->extents[d] != logits_layout->extents[d]) return T4A_ERR_SHAPE_MISMATCH;
+      a.draft = draft + draft_layout->offset;
+      a.draft_node = draft_layout->strides[1];
+      a.draft_batch = draft_layout->strides[2];
+    }
+  }
+  a.logits = static_cast<const char*>(logits) + logits_layout->offset * esize;
+  a.logits_node = logits_layout->strides[1];
+  a.logits_batch = logits_layout->strides[2];
+  a.tokens = tokens;
+  a.parents = parents;
+  a.uniforms = uniforms;
+  a.count = count;
+  a.path = path;
+  a.said = said;
+  a.logs = logs;
+  a.vocab = vocab;
+  a.nodes = static_cast<int>(nodes);
+  a.inverse_temperature = a.greedy ? 1.0f : static_cast<float>(1.0 / static_cast<double>(temperature));
+  // Blocks of a cluster: a slice of at least 4096 values each, so that a block's load outweighs
+  // its barriers, and as many as it takes for a slice to fit a block's shared memory.
+  const int vec = 16 / esize;
+  int blocks = 1;
+  while (blocks < kMostCluster && vocab >= blocks * 2 * 4096ll) blocks *= 2;
+  const long long vectors = (vocab + 2 * vec - 2) / vec;  // at the worst skew
+  const long long slots = (vectors + blocks - 1) / blocks;
+  if (slots * vec > kMostSlice || vocab > 0x7fffffffll) return T4A_ERR_DOMAIN_TOO_LARGE;
+  if (batch * blocks > 0x7fffffffll) return T4A_ERR_LAUNCH_LIMIT;
+  a.slots = static_cast<int>(slots);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case T4A_CUDA_F32: return launch_verify<float>(a, static_cast<int>(batch), blocks, s);
+    case T4A_F16: return launch_verify<__half>(a, static_cast<int>(batch), blocks, s);
+    default: return launch_verify<__nv_bfloat16>(a, static_cast<int>(batch), blocks, s);
+  }
+}

@@ -9,7 +9,8 @@ is no CPU or PyTorch fallback, and a missing library raises at import of `lib()`
 import ctypes
 import os
 
-from . import abi
+from . import abi, cache
+from .cache import cache_read, cache_write, tree_attention, tree_attention_workspace_bytes, verify_drafts
 from .abi import (F32, F64, I32, I64, BOOL, C32, C64, SUM, PROD, SUM_SQUARES, MAX, MIN, UNIT, PLANE,
                   Layout, layout, numpy_layout)
 
@@ -154,7 +155,7 @@ def _declare(l):
     _declare_more(l)
 
 
-_EXTRA_DECLS = []
+_EXTRA_DECLS = [cache.declare]
 
 
 def _declare_more(l):

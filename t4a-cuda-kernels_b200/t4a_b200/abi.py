@@ -13,6 +13,9 @@ F32, F64, I32, I64, BOOL, C32, C64 = range(7)
 DTYPE_SIZE = {F32: 4, F64: 8, I32: 4, I64: 8, BOOL: 1, C32: 8, C64: 16}
 DTYPE_NAME = {F32: "F32", F64: "F64", I32: "I32", I64: "I64", BOOL: "Bool", C32: "C32", C64: "C64"}
 
+# Element types of the paged-cache operators only (include/t4a_b200/cache.h).
+F16, BF16, I8, E4M3 = 32, 33, 34, 35
+
 SUM, PROD, SUM_SQUARES, MAX, MIN = range(5)
 OP_NAME = {SUM: "Sum", PROD: "Prod", SUM_SQUARES: "SumSquares", MAX: "Max", MIN: "Min"}
 UNIT, PLANE = 0, 1
@@ -94,6 +97,16 @@ class TransposeConfig(ctypes.Structure):
                 ("padding", ctypes.c_int), ("vector_width", ctypes.c_int)]
 
 
+class KVCache(ctypes.Structure):
+    """t4a_kv_cache: a paged cache's tensors and their layouts."""
+    _fields_ = [("kind", ctypes.c_int), ("reserved", ctypes.c_int),
+                ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+                ("k_layout", Layout), ("v_layout", Layout), ("k_scale_layout", Layout), ("v_scale_layout", Layout),
+                ("k_len", ctypes.c_longlong), ("v_len", ctypes.c_longlong),
+                ("k_scale_len", ctypes.c_longlong), ("v_scale_len", ctypes.c_longlong)]
+
+
 assert ctypes.sizeof(Layout) == 144 and Layout.offset.offset == 8 and Layout.strides.offset == 80
 assert ctypes.sizeof(AxisValues) == 72
 assert ctypes.sizeof(GatherPlan) == 280 and GatherPlan.window_dims.offset == 24
@@ -101,6 +114,7 @@ assert ctypes.sizeof(ScatterPlan) == 216 and ScatterPlan.window_dims.offset == 2
 assert ctypes.sizeof(GatherPlanAny) == 56 and GatherPlanAny.slice_sizes.offset == 48
 assert ctypes.sizeof(ScatterPlanAny) == 48 and ScatterPlanAny.scatter_dims.offset == 40
 assert ctypes.sizeof(TransposeConfig) == 16
+assert ctypes.sizeof(KVCache) == 648 and KVCache.k_layout.offset == 40
 
 
 def layout(extents, strides=None, offset=0):
