@@ -38,7 +38,8 @@ struct AttendArgs {
   float scale_log2;  // scale * log2(e)
   int batch, nodes, group, rows;  // rows = nodes * group
   int row_tiles, tile_rows;
-  int table_pages;
+  int places;       // table pages * page_size, or the most that 32 bits allow
+  int tile_pages, tile_places;  // kTile / page_size and kTile % page_size
   int q_bf16;      // q and out are BF16, else F16
   int pairs;       // q and out rows start on 4-byte boundaries
   float* part_out;  // [blocks][2][tile_rows][dim]
@@ -46,86 +47,83 @@ struct AttendArgs {
   int blocks;
 };
 
-// Tokens that sequence b's rows can see: committed ones, and all with the drafted ones.
-__device__ __forceinline__ void sequence_tokens(const AttendArgs& a, int b, long long* context, int* live,
-                                                long long* length) {
-  const long long places = static_cast<long long>(a.table_pages) * a.cache.page_size;
-  const long long c = max(0, a.context[b]);
-  const int n = a.live_nodes ? min(max(0, a.live_nodes[b]), a.nodes) : a.nodes;
-  *context = min(c, places);
+// Tokens that sequence b's rows can see: committed ones, and all with the drafted ones.  Places
+// are below 2^31 - 2^8, so that 32-bit arithmetic holds a tile past the end.
+__device__ __forceinline__ void sequence_tokens(const AttendArgs& a, int b, int* context, int* live, int* length) {
+  const int c = max(0, a.context[b]), n = a.live_nodes ? min(max(0, a.live_nodes[b]), a.nodes) : a.nodes;
+  *context = min(c, a.places);
   *live = n;
-  *length = min(c + n, places);
+  *length = static_cast<int>(min(static_cast<long long>(c) + n, static_cast<long long>(a.places)));
 }
 
-__device__ __forceinline__ long long sequence_tiles(const AttendArgs& a, int b) {
-  long long context, length;
-  int live;
+__device__ __forceinline__ int sequence_tiles(const AttendArgs& a, int b) {
+  int context, live, length;
   sequence_tokens(a, b, &context, &live, &length);
   return live == 0 ? 0 : (length + kTile - 1) / kTile;  // no live row: nothing to attend
-}
-
-// Tiles of all units, and of those of the sequences before `upto`.  Called by whole warps.
-__device__ __forceinline__ void count_tiles(const AttendArgs& a, int upto, long long* total, long long* before) {
-  const int lane = threadIdx.x & 31;
-  const long long units = static_cast<long long>(a.cache.heads) * a.row_tiles;
-  long long t = 0, p = 0;
-  for (int b = lane; b < a.batch; b += 32) {
-    const long long n = sequence_tiles(a, b) * units;
-    t += n;
-    if (b < upto) p += n;
-  }
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) {
-    t += __shfl_xor_sync(0xffffffffu, t, d);
-    p += __shfl_xor_sync(0xffffffffu, p, d);
-  }
-  *total = t;
-  *before = p;
-}
-
-__device__ __forceinline__ long long quota_of(const AttendArgs& a, long long total) {
-  return max(1ll, (total + a.blocks - 1) / a.blocks);
 }
 
 // A block's place on the line of tiles.
 struct Cursor {
   int b, head, row_tile;
-  long long tile, tiles;  // within the unit
-  long long left;         // of the block's stretch
+  int tile, tiles;  // within the unit
+  int left;         // of the block's stretch
 };
 
-// The start of block `block`'s stretch (left 0 where it has none).  Called by whole warps; all
-// lanes get the same.
+// Tiles of all units, and of those of the sequences before `upto`.  Called by whole warps; all
+// lanes get the same.  The planner keeps the number of tiles below 2^31.
+struct Line {
+  int total, before;
+};
+
+__device__ __forceinline__ Line read_line(const AttendArgs& a, int upto) {
+  const int lane = threadIdx.x & 31, units = a.cache.heads * a.row_tiles;
+  Line n = {};
+  for (int b0 = 0; b0 < a.batch; b0 += 32) {
+    const int b = b0 + lane, mine = b < a.batch ? sequence_tiles(a, b) * units : 0;
+    n.total += __reduce_add_sync(0xffffffffu, mine);
+    n.before += __reduce_add_sync(0xffffffffu, b < upto ? mine : 0);
+  }
+  return n;
+}
+
+__device__ __forceinline__ int quota_of(const AttendArgs& a, int total) {
+  return max(1, (total + a.blocks - 1) / a.blocks);
+}
+
+// The start of block `block`'s stretch (left 0 where it has none).
 __device__ __forceinline__ Cursor find_start(const AttendArgs& a, int block) {
-  const int lane = threadIdx.x & 31;
-  const long long units = static_cast<long long>(a.cache.heads) * a.row_tiles;
-  long long total, unused;
-  count_tiles(a, 0, &total, &unused);
-  const long long quota = quota_of(a, total), start = quota * block;
+  const int lane = threadIdx.x & 31, units = a.cache.heads * a.row_tiles;
   Cursor c = {};
-  c.left = max(0ll, min(quota, total - start));
-  if (c.left == 0) return c;
-  long long before = 0;
+  int total = 0, kept = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 32) {
     const int b = b0 + lane;
-    const long long mine = b < a.batch ? sequence_tiles(a, b) * units : 0;
-    long long sum = mine;  // inclusive prefix
+    kept = b < a.batch ? sequence_tiles(a, b) * units : 0;
+    total += __reduce_add_sync(0xffffffffu, kept);
+  }
+  const int quota = quota_of(a, total);
+  const long long far = static_cast<long long>(quota) * block;
+  if (far >= total) return c;
+  const int start = static_cast<int>(far);
+  c.left = min(quota, total - start);
+  int before = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 32) {
+    const int b = b0 + lane;
+    const int mine = a.batch <= 32 ? kept : b < a.batch ? sequence_tiles(a, b) * units : 0;
+    int sum = mine;  // inclusive prefix
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const long long o = __shfl_up_sync(0xffffffffu, sum, d);
+      const int o = __shfl_up_sync(0xffffffffu, sum, d);
       if (lane >= d) sum += o;
     }
     const unsigned past = __ballot_sync(0xffffffffu, before + sum > start);
     if (past) {
       const int at = __ffs(past) - 1;
-      const long long tiles = __shfl_sync(0xffffffffu, mine, at) / units;
-      const long long in = start - before - __shfl_sync(0xffffffffu, sum - mine, at);
+      c.tiles = __shfl_sync(0xffffffffu, mine, at) / units;
+      const int in = start - before - __shfl_sync(0xffffffffu, sum - mine, at), unit = in / c.tiles;
       c.b = b0 + at;
-      c.tiles = tiles;
-      const long long unit = in / tiles;
-      c.tile = in - unit * tiles;
-      c.head = static_cast<int>(unit / a.row_tiles);
-      c.row_tile = static_cast<int>(unit - static_cast<long long>(c.head) * a.row_tiles);
+      c.tile = in - unit * c.tiles;
+      c.head = unit / a.row_tiles;
+      c.row_tile = unit - c.head * a.row_tiles;
       return c;
     }
     before += __shfl_sync(0xffffffffu, sum, 31);

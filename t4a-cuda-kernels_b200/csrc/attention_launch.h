@@ -1,4 +1,4 @@
-// Launches of k_attend for one cache kind: the padded dim and the row warps pick the instance.
+// Launches of k_attend for one cache kind: the padded dim and the row tiles pick the instance.
 #pragma once
 
 #include <atomic>
@@ -29,42 +29,44 @@ int allow_shared(Kernel kernel, int bytes, std::atomic<unsigned long long>* done
 }
 
 // With `blocks`, only says how many blocks to launch: as many as the SMs hold at once.
-template <int Kind, int Dim, int kRowWarps>
+template <int Kind, int Dim, int kRowTiles>
 int launch_one(const AttendArgs& a, cudaStream_t stream, int* blocks) {
-  using Shape = MmaShape<Kind, Dim>;
+  using Shape = MmaShape<Kind, Dim, kRowTiles>;
   if (blocks != nullptr) {
     *blocks = kSms * Shape::per_sm;
     return T4A_OK;
   }
   static std::atomic<unsigned long long> allowed{0};
-  T4A_TRY(allow_shared(k_attend<Kind, Dim, kRowWarps>, Shape::shared, &allowed));
-  k_attend<Kind, Dim, kRowWarps><<<a.blocks, kMmaThreads, Shape::shared, stream>>>(a);
+  T4A_TRY(allow_shared(k_attend<Kind, Dim, kRowTiles>, Shape::shared, &allowed));
+  k_attend<Kind, Dim, kRowTiles><<<a.blocks, kMmaThreads, Shape::shared, stream>>>(a);
   return runtime::check_launch();
 }
 
 template <int Kind, int Dim>
-int launch_rows_of(const AttendArgs& a, int row_warps, cudaStream_t stream, int* blocks) {
-  switch (row_warps) {
+int launch_rows_of(const AttendArgs& a, int row_tiles, cudaStream_t stream, int* blocks) {
+  switch (row_tiles) {
     case 1: return launch_one<Kind, Dim, 1>(a, stream, blocks);
     case 2: return launch_one<Kind, Dim, 2>(a, stream, blocks);
-    default: return launch_one<Kind, Dim, 4>(a, stream, blocks);
+    default:
+      if constexpr (Dim <= 128) return launch_one<Kind, Dim, 4>(a, stream, blocks);
+      else return T4A_ERR_UNSUPPORTED_OP;
   }
 }
 
 template <int Kind>
-int launch_mma(const AttendArgs& a, int padded, int row_warps, cudaStream_t stream, int* blocks) {
+int launch_mma(const AttendArgs& a, int padded, int row_tiles, cudaStream_t stream, int* blocks) {
   switch (padded) {
-    case 64: return launch_rows_of<Kind, 64>(a, row_warps, stream, blocks);
-    case 96: return launch_rows_of<Kind, 96>(a, row_warps, stream, blocks);
-    case 128: return launch_rows_of<Kind, 128>(a, row_warps, stream, blocks);
-    default: return launch_rows_of<Kind, 256>(a, row_warps, stream, blocks);
+    case 64: return launch_rows_of<Kind, 64>(a, row_tiles, stream, blocks);
+    case 96: return launch_rows_of<Kind, 96>(a, row_tiles, stream, blocks);
+    case 128: return launch_rows_of<Kind, 128>(a, row_tiles, stream, blocks);
+    default: return launch_rows_of<Kind, 256>(a, row_tiles, stream, blocks);
   }
 }
 
-int launch_mma_f16(const AttendArgs& a, int padded, int row_warps, cudaStream_t stream, int* blocks);
-int launch_mma_bf16(const AttendArgs& a, int padded, int row_warps, cudaStream_t stream, int* blocks);
-int launch_mma_i8(const AttendArgs& a, int padded, int row_warps, cudaStream_t stream, int* blocks);
-int launch_mma_e4m3(const AttendArgs& a, int padded, int row_warps, cudaStream_t stream, int* blocks);
+int launch_mma_f16(const AttendArgs& a, int padded, int row_tiles, cudaStream_t stream, int* blocks);
+int launch_mma_bf16(const AttendArgs& a, int padded, int row_tiles, cudaStream_t stream, int* blocks);
+int launch_mma_i8(const AttendArgs& a, int padded, int row_tiles, cudaStream_t stream, int* blocks);
+int launch_mma_e4m3(const AttendArgs& a, int padded, int row_tiles, cudaStream_t stream, int* blocks);
 
 }  // namespace cache
 }  // namespace t4a

@@ -1,16 +1,19 @@
 // Attention over the paged cache with warp-level products (mma.sync m16n8k16): the kernel for few
 // query rows a cache head, where the cache's bytes bound the call.
 //
-// A block of 4 warps takes 16 * kRowWarps query rows; kRowWarps warps share a cache row and
-// 4 / kRowWarps warps share the tokens of a tile of 64.  Cache rows come by cp.async, 16 bytes a
-// lane, into a ring of stages whose row pitch is an odd number of 16-byte units, so that ldmatrix
-// meets no bank twice.  With one row warp a warp loads just the tokens that it works on, and no
-// block barrier is needed.
-//   S = Q K^T, 16 rows x 16 tokens at a time; running maximum m and sum l for each row;
-//   O = O * 2^(m_old - m) + 2^(S - m) V
-// m moves only where a new maximum exceeds it by 2^8, so the 64 multiplications of O are rare, and
-// weights carry a further 2^7: they reach from 2^15 down, so that F16 keeps all bits of those that
-// are 2^-21 of the largest.  The quotient O / l depends on neither.
+// Products are transposed: 16 tokens (or 16 columns of V) are the wide side of a product and 8
+// query rows the narrow one, so that 8 rows, a decoding step's group, waste nothing:
+//   S^T = K Q^T    [16 tokens x 8 rows]
+//   O^T = V^T P^T  [16 columns x 8 rows], P^T from S^T by an 8x8 transpose of registers (movmatrix)
+// and each code that a warp unpacks serves all kRowTiles * 8 rows.  A running maximum m and sum l
+// for each row;  O = O * 2^(m_old - m) + 2^(S - m) V.  m moves only where a new maximum exceeds it
+// by 2^8, so the multiplications of O are rare, and weights carry a further 2^7: they reach from
+// 2^15 down, so that F16 keeps all bits of those that are 2^-21 of the largest.  O / l depends on
+// neither.
+//
+// Each of a block's 4 warps takes 16 of a tile's 64 tokens, and copies just these (cp.async, 16
+// bytes a lane) into its part of a ring of stages; no warp waits for another within a unit.  The
+// row pitch is an odd number of 16-byte units, so that ldmatrix meets no bank twice.
 //
 // Quantised rows stay codes in shared memory and become F16 in registers, exactly.  K's scale
 // multiplies the score.  V's scale is an addend of the exponent, S + log2(scale): the weight that
@@ -19,10 +22,9 @@
 // make) count in the softmax alone: they have a maximum and a sum of their own, joined at the end.
 // Q is F16 too, times a power of two that brings the row's largest magnitude into [1, 2).
 // ldmatrix moves pairs of codes, so a thread's codes are not where 16-bit values would be:
-//   K: a thread's 4 neighbouring codes serve as k = 2c, 2c+1, 2c+8, 2c+9, and Q's fragments take
-//      the same order;
+//   K: a thread's 4 neighbouring codes serve as k = 2c, 2c+1, 2c+8, 2c+9, and Q has the same order;
 //   V (transposed): a register holds codes d, d+1 of tokens t, t+1; byte permutes make the pairs
-//      (t, t+1) of d and of d+1, the columns of two n-tiles.
+//      (t, t+1) of d and of d+1, rows g and g + 8 of a product.
 #pragma once
 
 #include <cuda_fp8.h>
@@ -44,19 +46,27 @@ struct KindOf {
   static constexpr int bytes = quantised ? 1 : 2;
 };
 
-template <int Kind, int Dim>
+template <int Kind, int Dim, int kRowTiles>
 struct MmaShape {
   static constexpr int bytes = KindOf<Kind>::bytes;
+  static constexpr int rows = 8 * kRowTiles;
   static constexpr int pitch = Dim * bytes + 16;  // an odd number of 16-byte units
   static constexpr int chunks = Dim * bytes / 16;
   static constexpr int stage = kTile * pitch * 2 + (KindOf<Kind>::quantised ? kTile * 8 : 0) + 16;
   static constexpr int stages = 3;
-  static constexpr int merge = kTile * Dim * 4 + kTile * 16;
-  static constexpr int shared = stages * stage > merge ? stages * stage : merge;
-  // Blocks that an SM holds: by shared memory (each block costs 1 KB more than it asks for), and at
-  // most 3, which leaves a thread 168 registers.
+  static constexpr int q_pitch = Dim * 2 + 16;
+  static constexpr int q_bytes = rows * q_pitch + rows * 4;
+  static constexpr int out_pitch = Dim + 4;  // floats: the lanes of a store meet 32 banks
+  static constexpr int merge = 4 * rows * (out_pitch * 4 + 16);
+  static constexpr int ring = stages * stage > merge ? stages * stage : merge;
+  static constexpr int shared = ring + q_bytes;
+  // Blocks that an SM holds: by shared memory (each block costs 1 KB more than it asks for) and by
+  // the registers that O takes.
   static constexpr int fit = 233472 / (shared + 1024);
-  static constexpr int per_sm = fit < 3 ? fit : 3;
+  static constexpr int by_registers = kRowTiles == 4 || Dim * kRowTiles >= 512 ? 2 : Dim * kRowTiles >= 192 ? 3 : 4;
+  static constexpr int per_sm = fit < by_registers ? fit : by_registers;
+  // Q's fragments stay in registers where they are few.
+  static constexpr bool hold_q = kRowTiles * Dim <= 256;
 };
 
 __device__ __forceinline__ unsigned shared_at(const void* p) {
@@ -178,429 +188,461 @@ __device__ __forceinline__ bool odd_values(uint32_t r) {
   else return (r & 0x7c00u) == 0x7c00u || (r & 0x7c000000u) == 0x7c000000u;
 }
 
-// Two neighbouring q values, zeros outside the rows.
-__device__ __forceinline__ void load_q2(const AttendArgs& a, long long at, float* x, float* y) {
-  if (a.q_bf16) {
-    const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(a.q) + at;
-    if (a.pairs) {
-      const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p));
-      *x = f.x;
-      *y = f.y;
-    } else {
-      *x = __bfloat162float(p[0]);
-      *y = __bfloat162float(p[1]);
+// 8x8 16-bit values across the warp, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+
+__device__ __forceinline__ float load_q(const AttendArgs& a, long long at) {
+  return a.q_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(a.q)[at])
+                  : __half2float(static_cast<const __half*>(a.q)[at]);
+}
+
+// The unit's query rows into shared memory [rows][Dim], 16 bits, in the order of K's fragments,
+// and what turns a row's products into base-2 scores.  A warp takes a row.
+template <int Kind, int Dim, int kRowTiles>
+__device__ __forceinline__ void stage_q(const AttendArgs& a, int b, int head, int first_row, unsigned char* q_rows,
+                                        float* factors) {
+  using Shape = MmaShape<Kind, Dim, kRowTiles>;
+  constexpr int kEach = Dim / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int r = warp; r < Shape::rows; r += kMmaThreads / 32) {
+    const int row = first_row + r;
+    float x[kEach];
+    float most = 0.0f;
+    const int node = row / a.group;
+    const long long base = b * a.q_batch + node * a.q_node +
+                           (static_cast<long long>(head) * a.group + (row - node * a.group)) * a.q_head;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int d = lane + 32 * i;
+      x[i] = row < a.rows && d < a.cache.dim ? load_q(a, base + d) : 0.0f;
+      most = fmaxf(most, fabsf(x[i]));
     }
-  } else {
-    const __half* p = static_cast<const __half*>(a.q) + at;
-    if (a.pairs) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(p));
-      *x = f.x;
-      *y = f.y;
-    } else {
-      *x = __half2float(p[0]);
-      *y = __half2float(p[1]);
+    float down = 1.0f, factor = a.scale_log2;
+    if constexpr (KindOf<Kind>::quantised) {
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+      int e = static_cast<int>((__float_as_uint(most) >> 23) & 0xff);  // biased exponent
+      e = most == 0.0f || e == 0xff ? 127 : min(max(e, 1), 253);
+      down = __uint_as_float(static_cast<unsigned>(254 - e) << 23);  // 2^(127 - e)
+      factor *= __uint_as_float(static_cast<unsigned>(e) << 23);
     }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int d = lane + 32 * i, in = d & 15;
+      const int slot = KindOf<Kind>::quantised ? (d & ~15) + 2 * (in >> 2) + (in & 1) + ((in & 2) << 2) : d;
+      if constexpr (KindOf<Kind>::bf16)
+        reinterpret_cast<__nv_bfloat16*>(q_rows + r * Shape::q_pitch)[slot] = __float2bfloat16_rn(x[i]);
+      else
+        reinterpret_cast<__half*>(q_rows + r * Shape::q_pitch)[slot] = __float2half_rn(x[i] * down);
+    }
+    if (lane == 0) factors[r] = factor;
   }
 }
 
-template <int Kind, int Dim, int kRowWarps>
-__global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim>::per_sm) k_attend(const AttendArgs a) {
-  using Shape = MmaShape<Kind, Dim>;
+template <int Kind, int Dim, int kRowTiles>
+__global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::per_sm) k_attend(const AttendArgs a) {
+  using Shape = MmaShape<Kind, Dim, kRowTiles>;
   constexpr bool kQuantised = KindOf<Kind>::quantised, kBf16 = KindOf<Kind>::bf16;
-  constexpr int kTokenWarps = 4 / kRowWarps, kSubs = kTile / (16 * kTokenWarps), kRows = 16 * kRowWarps;
-  constexpr int kSteps = Dim / 16, kStages = Shape::stages;
+  constexpr int kSteps = Dim / 16, kStages = Shape::stages, kRows = Shape::rows;
   extern __shared__ __align__(16) unsigned char smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int row_warp = warp % kRowWarps, token_warp = warp / kRowWarps;
-  const int g = lane >> 2, c = lane & 3;  // the thread's rows g and g + 8, and its column pair, in a fragment
+  const int g = lane >> 2, c = lane & 3;
   const int dim = a.cache.dim, used = dim * Shape::bytes / 16;
+  unsigned char* const q_rows = smem + Shape::ring;
+  float* const factors = reinterpret_cast<float*>(q_rows + kRows * Shape::q_pitch);
 
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   Cursor at = find_start(a, blockIdx.x);
 
-  auto k_row = [&](int stage, int t) { return smem + stage * Shape::stage + t * Shape::pitch; };
-  auto v_row = [&](int stage, int t) { return smem + stage * Shape::stage + (kTile + t) * Shape::pitch; };
-  auto scales = [&](int stage) {  // [2][kTile]: K's, V's
-    return reinterpret_cast<float*>(smem + stage * Shape::stage + 2 * kTile * Shape::pitch);
-  };
-  auto seen_bits = [&](int stage) {  // 16 tokens to an entry: which are there
-    return reinterpret_cast<unsigned*>(smem + stage * Shape::stage + 2 * kTile * Shape::pitch +
-                                       (kQuantised ? kTile * 8 : 0));
-  };
+  // A stage: K's rows, V's rows, K's and V's scales, and for each warp which of its tokens are there.
+  unsigned char* const my_rows = smem + 16 * warp * Shape::pitch;
+  constexpr int kV = kTile * Shape::pitch, kScales = 2 * kTile * Shape::pitch;
+  constexpr int kSeen = kScales + (kQuantised ? kTile * 8 : 0);
 
-  // The pads past dim enter products with zeros of Q, and columns that are not stored; they only
-  // have to be finite, once.
+  // The pads past dim meet zeros of Q, or make columns that are not stored; they only have to be
+  // finite, once.
   if (dim < Dim) {
-    for (int i = threadIdx.x; i < Shape::shared / 16; i += kMmaThreads)
+    for (int i = threadIdx.x; i < Shape::ring / 16; i += kMmaThreads)
       reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
   }
 
   while (at.left > 0) {
     const int b = at.b;
-    long long context, length;
-    int live;
+    int context, live, length;
     sequence_tokens(a, b, &context, &live, &length);
-    const int first_row = at.row_tile * kRows + row_warp * 16;
-    const long long tile0 = at.tile;
-    const int n = static_cast<int>(min(at.left, at.tiles - at.tile));
+    const int first_row = at.row_tile * kRows;
+    const int tile0 = at.tile, n = min(at.left, at.tiles - at.tile);
 
     // This lane's token of a tile: K's row for the lower half of the warp, V's for the upper.
     const Pages& side = lane < 16 ? a.cache.k : a.cache.v;
     const unsigned char* const head_base = side.base + at.head * side.head;
     const float* const head_scale = kQuantised ? side.scale + at.head * side.scale_head : nullptr;
-    auto find_page = [&](int i) {  // the page of the lane's token in tile i, -1 for none
-      const long long pos = (tile0 + i) * kTile + 16 * warp + (lane & 15);
-      if (i >= n || pos >= length) return -1;
-      const int page = a.table[b * a.table_batch +
-                               static_cast<long long>(static_cast<unsigned>(pos) / static_cast<unsigned>(a.cache.page_size)) *
-                                   a.table_page];
-      return page >= 0 && page < a.cache.pages ? page : -1;
+    const int* const my_table = a.table + b * a.table_batch;
+    int pos = tile0 * kTile + 16 * warp + (lane & 15);  // of the next page to look up
+    int in_table = pos / a.cache.page_size, place = pos - in_table * a.cache.page_size;
+    const int end = min(length, (tile0 + n) * kTile);
+    int page_ahead, place_ahead;  // of the next tile to copy
+    auto look_up = [&] {
+      page_ahead = -1;
+      place_ahead = place;
+      if (pos < end) page_ahead = my_table[in_table * a.table_page];
+      pos += kTile;
+      in_table += a.tile_pages;
+      place += a.tile_places;
+      if (place >= a.cache.page_size) {
+        place -= a.cache.page_size;
+        ++in_table;
+      }
     };
-    int page_ahead = find_page(0);
-    auto issue = [&](int i) {
-      const int page = page_ahead;
-      page_ahead = find_page(i + 1);
-      if (i < n) {
-        const int stage = i % kStages;
-        const unsigned pos = static_cast<unsigned>((tile0 + i) * kTile) + 16 * warp + (lane & 15);
-        const int place = static_cast<int>(pos % static_cast<unsigned>(a.cache.page_size));
-        const bool there = page >= 0;
-        long long off = 0;
-        if (there) off = page * side.page + place * side.place;
+    int to_stage = 0;
+    auto issue = [&](bool any) {
+      const int page = page_ahead, at_place = place_ahead;
+      look_up();
+      if (any) {
+        unsigned char* const stage = smem + to_stage * Shape::stage;
+        const bool there = static_cast<unsigned>(page) < static_cast<unsigned>(a.cache.pages);
         const unsigned bits = __ballot_sync(0xffffffffu, there) & 0xffffu;
-        if (lane == 0) seen_bits(stage)[warp] = bits;
+        if (lane == 0) reinterpret_cast<unsigned*>(stage + kSeen)[warp] = bits;
         if constexpr (kQuantised)
-          copy4(shared_at(scales(stage) + (lane >> 4) * kTile + 16 * warp + (lane & 15)),
-                head_scale + (there ? page * side.scale_page + place * side.scale_place : 0), there);
-        const unsigned char* const from = head_base + off;
+          copy4(shared_at(stage + kScales + ((lane >> 4) * kTile + 16 * warp + (lane & 15)) * 4),
+                head_scale + (there ? page * side.scale_page + at_place * side.scale_place : 0), there);
+        const unsigned char* const from = head_base + (there ? page * side.page + at_place * side.place : 0);
+        const unsigned to = shared_at(my_rows + to_stage * Shape::stage);
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
-          for (int u = 0; u < (16 * Shape::chunks + 31) / 32; ++u) {
+          for (int u = 0; u < 16 * Shape::chunks / 32; ++u) {
             const int k = u * 32 + lane, t = k / Shape::chunks, chunk = k - t * Shape::chunks;
             const unsigned char* row = reinterpret_cast<const unsigned char*>(
-                __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(from), (s * 16 + t) & 31));
-            if ((16 * Shape::chunks % 32 == 0 || k < 16 * Shape::chunks) && chunk < used)
-              copy16(shared_at((s ? v_row(stage, 16 * warp + t) : k_row(stage, 16 * warp + t)) + chunk * 16),
-                     row + chunk * 16, (bits >> t) & 1);
+                __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(from), s * 16 + t));
+            if (chunk < used) copy16(to + s * kV + t * Shape::pitch + chunk * 16, row + chunk * 16, (bits >> t) & 1);
           }
       }
+      to_stage = to_stage + 1 == kStages ? 0 : to_stage + 1;
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    auto sync_tile = [&] {
-      if constexpr (kRowWarps == 1) __syncwarp();
-      else __syncthreads();
-    };
 
+    look_up();
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) issue(i);
+    for (int i = 0; i < kStages - 1; ++i) issue(i < n);
 
-    // Q's fragments, and what turns a product into a base-2 score.
-    uint32_t q[kSteps][4];
-    float factor[2];
-    {
-      float most[2] = {0.0f, 0.0f};
-      float x[kQuantised ? kSteps : 1][2][4];
+    stage_q<Kind, Dim, kRowTiles>(a, b, at.head, first_row, q_rows, factors);
+    __syncthreads();
+    // Q's fragments: [n = row g][k = 2c, 2c+1] and [k = 2c+8, 2c+9] of each step.
+    uint32_t q[Shape::hold_q ? kSteps : 1][kRowTiles][2];
+    const unsigned q_at = shared_at(q_rows) + (lane & 7) * Shape::q_pitch + (lane >> 3) * 16;
+    if constexpr (Shape::hold_q) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int row = first_row + g + 8 * h;
-        const bool live_row = row < a.rows;
-        const int node = live_row ? row / a.group : 0, in_group = live_row ? row - node * a.group : 0;
-        const long long base = b * a.q_batch + node * a.q_node +
-                               (static_cast<long long>(at.head) * a.group + in_group) * a.q_head;
+      for (int j = 0; j < kRowTiles; ++j)
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-          float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          const int d0 = kQuantised ? 16 * s + 4 * c : 16 * s + 2 * c, d1 = kQuantised ? d0 + 2 : d0 + 8;
-          if (live_row && 16 * s < dim) {
-            load_q2(a, base + d0, &v[0], &v[1]);
-            load_q2(a, base + d1, &v[2], &v[3]);
-          }
-          if constexpr (kQuantised) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              most[h] = fmaxf(most[h], fabsf(v[e]));
-              x[s][h][e] = v[e];
-            }
-          } else {
-            q[s][h] = pack2<kBf16>(v[0], v[1]);
-            q[s][2 + h] = pack2<kBf16>(v[2], v[3]);
-          }
+        for (int k = 0; k < kSteps; k += 2) {
+          uint32_t r[4];
+          ldmatrix4(r, q_at + j * 8 * Shape::q_pitch + k * 32);
+          q[k][j][0] = r[0];
+          q[k][j][1] = r[1];
+          q[k + 1][j][0] = r[2];
+          q[k + 1][j][1] = r[3];
         }
-        factor[h] = a.scale_log2;
-        if constexpr (kQuantised) {
-          most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 1));
-          most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 2));
-          int e = static_cast<int>((__float_as_uint(most[h]) >> 23) & 0xff);  // biased exponent
-          e = most[h] == 0.0f || e == 0xff ? 127 : min(max(e, 1), 253);
-          const float down = __uint_as_float(static_cast<unsigned>(254 - e) << 23);  // 2^(127 - e)
-          factor[h] *= __uint_as_float(static_cast<unsigned>(e) << 23);
+    }
+    float factor[kRowTiles][2];
 #pragma unroll
-          for (int s = 0; s < kSteps; ++s) {
-            q[s][h] = pack2<false>(x[s][h][0] * down, x[s][h][1] * down);
-            q[s][2 + h] = pack2<false>(x[s][h][2] * down, x[s][h][3] * down);
-          }
+    for (int j = 0; j < kRowTiles; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) factor[j][e] = factors[8 * j + 2 * c + e];
+
+    float o[kSteps][kRowTiles][4];  // [columns g / g + 8][rows 2c, 2c + 1]
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+      for (int j = 0; j < kRowTiles; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[k][j][e] = 0.0f;
+    // Of rows 8j + 2c + e; m is the same in all lanes of a row, l a lane's own part.
+    float m[kRowTiles][2], l[kRowTiles][2];
+    float mz[kQuantised ? kRowTiles : 1][2], lz[kQuantised ? kRowTiles : 1][2];  // of V rows with a scale of 0
+#pragma unroll
+    for (int j = 0; j < kRowTiles; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        m[j][e] = -INFINITY;
+        l[j][e] = 0.0f;
+        if constexpr (kQuantised) {
+          mz[j][e] = -INFINITY;
+          lz[j][e] = 0.0f;
         }
       }
-    }
 
-    float o[2 * kSteps][4];
-#pragma unroll
-    for (int j = 0; j < 2 * kSteps; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-    float mz[2] = {-INFINITY, -INFINITY}, lz[2] = {0.0f, 0.0f};  // of V rows with a scale of 0
-
-    for (int i = 0; i < n; ++i) {
+    int from_stage = 0;
+    int pos0 = tile0 * kTile + 16 * warp;
+    for (int i = 0; i < n; ++i, pos0 += kTile) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-      sync_tile();
-      issue(i + kStages - 1);
-      const int stage = i % kStages;
-#pragma unroll 1
-      for (int sub = 0; sub < kSubs; ++sub) {
-        const int t0 = 16 * (token_warp + kTokenWarps * sub);
-        const long long pos0 = (tile0 + i) * kTile + t0;
-        const unsigned there = seen_bits(stage)[t0 >> 4];
-        if (there == 0) continue;
+      __syncwarp();
+      issue(i + kStages - 1 < n);
+      const unsigned char* const stage = smem + from_stage * Shape::stage;
+      const unsigned rows_at = shared_at(my_rows + from_stage * Shape::stage);
+      from_stage = from_stage + 1 == kStages ? 0 : from_stage + 1;
+      const unsigned there = reinterpret_cast<const unsigned*>(stage + kSeen)[warp];
+      if (there == 0) continue;
 
-        float s[2][4];
+      float s[kRowTiles][4];  // tokens g / g + 8, rows 2c, 2c + 1
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[0][e] = s[1][e] = 0.0f;
-        if constexpr (!kQuantised) {
-          // Matrices: tokens 0-7 and 8-15, each with d 0-7 and 8-15.
-          const unsigned from = shared_at(k_row(stage, t0 + (lane & 7) + ((lane >> 4) << 3)) + ((lane >> 3) & 1) * 16);
+      for (int j = 0; j < kRowTiles; ++j)
 #pragma unroll
-          for (int k = 0; k < kSteps; ++k) {
+        for (int e = 0; e < 4; ++e) s[j][e] = 0.0f;
+      // Matrices: tokens 0-7 and 8-15 of one 16-byte column, then of the next.
+      const unsigned k_at = rows_at + (lane & 15) * Shape::pitch + (lane >> 4) * 16;
+      auto times_q = [&](int k, const uint32_t(&x)[4]) {
+        if constexpr (Shape::hold_q) {
+#pragma unroll
+          for (int j = 0; j < kRowTiles; ++j) mma<kBf16>(s[j], x, q[k][j][0], q[k][j][1]);
+        } else {
+          // Two row tiles to an ldmatrix: rows 0-7 and 8-15, each k 0-7 and 8-15.
+#pragma unroll
+          for (int j = 0; j < kRowTiles; j += 2) {
             uint32_t r[4];
-            ldmatrix4(r, from + k * 32);
-            mma<kBf16>(s[0], q[k], r[0], r[1]);
-            mma<kBf16>(s[1], q[k], r[2], r[3]);
-          }
-        } else {
-          // Matrices of 8 tokens x 16 codes: two 16-code steps of tokens 0-7, then of tokens 8-15.
-          const unsigned from = shared_at(k_row(stage, t0 + (lane & 7) + ((lane >> 4) << 3)) + ((lane >> 3) & 1) * 16);
-#pragma unroll
-          for (int k = 0; k < kSteps; k += 2) {
-            uint32_t r[4], lo, hi;
-            ldmatrix4(r, from + k * 16);
-            neighbours<Kind>(r[0], &lo, &hi);
-            mma<false>(s[0], q[k], lo, hi);
-            neighbours<Kind>(r[2], &lo, &hi);
-            mma<false>(s[1], q[k], lo, hi);
-            neighbours<Kind>(r[1], &lo, &hi);
-            mma<false>(s[0], q[k + 1], lo, hi);
-            neighbours<Kind>(r[3], &lo, &hi);
-            mma<false>(s[1], q[k + 1], lo, hi);
+            ldmatrix4(r, shared_at(q_rows) + (8 * j + (lane & 7) + ((lane >> 4) << 3)) * Shape::q_pitch +
+                             ((lane >> 3) & 1) * 16 + k * 32);
+            mma<kBf16>(s[j], x, r[0], r[1]);
+            mma<kBf16>(s[j + 1], x, r[2], r[3]);
           }
         }
-
-        // Base-2 scores; s[j][2h + e] is row g + 8h, token 8j + 2c + e.
-        float per_scale[2][2];
-        bool nothing = false;  // a scale of 0 among the thread's tokens
-        if constexpr (kQuantised) {
+      };
+      if constexpr (!kQuantised) {
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int t = t0 + 8 * j + 2 * c + e;
-              const float ks = scales(stage)[t], vs = scales(stage)[kTile + t];
-              const bool zero = vs < kLeastScale;
-              const float lv = zero ? 0.0f : __log2f(vs);
-              // A NaN has made the score a NaN where the row is seen, and must not touch l elsewhere.
-              per_scale[j][e] = zero ? -1.0f : vs == vs ? exp2_fast(-lv) : 1.0f;
-              nothing = nothing || zero;
-#pragma unroll
-              for (int h = 0; h < 2; ++h) s[j][2 * h + e] = fmaf(s[j][2 * h + e] * ks, factor[h], lv);
-            }
-          nothing = __any_sync(0xffffffffu, nothing);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[j][e] *= factor[e >> 1];
+        for (int k = 0; k < kSteps; ++k) {
+          uint32_t r[4];
+          ldmatrix4(r, k_at + k * 32);
+          times_q(k, r);
         }
-        const bool partly = there != 0xffffu || pos0 + 16 > context;
-        if (partly) {
+      } else {
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int t = 8 * j + 2 * c + (e & 1);
-              const long long drafted = pos0 + t - context;
-              bool sees = (there >> t) & 1;
-              if (sees && drafted >= 0) {
-                const int node = (first_row + g + 8 * (e >> 1)) / a.group;
-                sees = node < live && node_sees(a, b, node, static_cast<int>(drafted));
-              }
-              if (!sees) s[j][e] = -INFINITY;
-            }
+        for (int k = 0; k < kSteps; k += 2) {
+          uint32_t r[4], x[4];
+          ldmatrix4(r, k_at + k * 16);
+          neighbours<Kind>(r[0], &x[0], &x[2]);
+          neighbours<Kind>(r[1], &x[1], &x[3]);
+          times_q(k, x);
+          neighbours<Kind>(r[2], &x[0], &x[2]);
+          neighbours<Kind>(r[3], &x[1], &x[3]);
+          times_q(k + 1, x);
         }
+      }
 
-        if (kQuantised && nothing) {
+      // Base-2 scores; s[j][2h + e] is token g + 8h, row 8j + 2c + e.
+      float per_scale[2];
+      bool nothing = false;  // a scale of 0 among the thread's tokens
+      if constexpr (kQuantised) {
+        const float* const scales = reinterpret_cast<const float*>(stage + kScales) + 16 * warp + g;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < 2; ++h) {
+          const float ks = scales[8 * h], vs = scales[kTile + 8 * h];
+          const bool zero = vs < kLeastScale;
+          const float lv = zero ? 0.0f : __log2f(vs);
+          // A NaN has made the score a NaN where the row is seen, and must not touch l elsewhere.
+          per_scale[h] = zero ? -1.0f : vs == vs ? exp2_fast(-lv) : 1.0f;
+          nothing = nothing || zero;
+#pragma unroll
+          for (int j = 0; j < kRowTiles; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) s[j][2 * h + e] = fmaf(s[j][2 * h + e] * ks, factor[j][e], lv);
+        }
+        nothing = __any_sync(0xffffffffu, nothing);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kRowTiles; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[j][e] *= factor[j][e & 1];
+      }
+      // Whether row 8j + 2c + e sees token t of the 16.
+      auto sees = [&](int t, int j, int e) {
+        if (!((there >> t) & 1)) return false;
+        const int drafted = pos0 + t - context;
+        if (drafted < 0) return true;
+        const int node = (first_row + 8 * j + 2 * c + e) / a.group;
+        return node < live && node_sees(a, b, node, drafted);
+      };
+      const bool partly = there != 0xffffu || pos0 + 16 > context;
+      if (partly) {
+#pragma unroll
+        for (int j = 0; j < kRowTiles; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!sees(g + 8 * (e >> 1), j, e & 1)) s[j][e] = -INFINITY;
+      }
+
+      if (kQuantised && nothing) {
+#pragma unroll
+        for (int j = 0; j < (kQuantised ? kRowTiles : 0); ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
             float high = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (per_scale[e >> 1][e & 1] < 0.0f) high = fmaxf(high, s[e >> 1][2 * h + (e & 1)]);
-            high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 1));
-            high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 2));
-            const float to = fmaxf(mz[h], high), less = to == -INFINITY ? 0.0f : to;
-            lz[h] *= exp2_fast(mz[h] - less);
-            mz[h] = to;
+            for (int h = 0; h < 2; ++h)
+              if (per_scale[h] < 0.0f) high = fmaxf(high, s[j][2 * h + e]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (per_scale[e >> 1][e & 1] < 0.0f) {
-                float& x = s[e >> 1][2 * h + (e & 1)];
-                lz[h] += exp2_fast(x - less);
-                x = -INFINITY;
+            for (int d = 4; d < 32; d <<= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, d));
+            const float to = fmaxf(mz[j][e], high), less = to == -INFINITY ? 0.0f : to;
+            lz[j][e] *= exp2_fast(mz[j][e] - less);
+            mz[j][e] = to;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (per_scale[h] < 0.0f) {
+                lz[j][e] += exp2_fast(s[j][2 * h + e] - less);
+                s[j][2 * h + e] = -INFINITY;
               }
           }
-        }
+      }
 
-        uint32_t p[4];
-        float top[2];
+      float top[kRowTiles][2];
+      bool rises = false;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          top[h] = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
-          top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-          top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+      for (int j = 0; j < kRowTiles; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float t = fmaxf(s[j][e], s[j][2 + e]);
+          rises = rises || t > m[j][e] + kSlack;
+          top[j][e] = t;
         }
-        if (__any_sync(0xffffffffu, top[0] > m[0] + kSlack || top[1] > m[1] + kSlack)) {
+      if (__any_sync(0xffffffffu, rises)) {
+#pragma unroll
+        for (int j = 0; j < kRowTiles; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) top[j][e] = fmaxf(top[j][e], __shfl_xor_sync(0xffffffffu, top[j][e], d));
+            const float to = fmaxf(m[j][e], top[j][e]);
+            const float shrink = to == -INFINITY ? 1.0f : exp2_fast(m[j][e] - to);
+            m[j][e] = to;
+            l[j][e] *= shrink;
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+              o[k][j][e] *= shrink;
+              o[k][j][2 + e] *= shrink;
+            }
+          }
+      }
+      uint32_t p[kRowTiles][2];  // [k = tokens 2c, 2c+1 / + 8][n = row g]
+#pragma unroll
+      for (int j = 0; j < kRowTiles; ++j) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float less = m[j][e] == -INFINITY ? 0.0f : m[j][e] - kLift;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float to = fmaxf(m[h], top[h]);
-            const float shrink = to == -INFINITY ? 1.0f : exp2_fast(m[h] - to);
-            m[h] = to;
-            l[h] *= shrink;
-#pragma unroll
-            for (int j = 0; j < 2 * kSteps; ++j) {
-              o[j][2 * h] *= shrink;
-              o[j][2 * h + 1] *= shrink;
-            }
+            const float w = exp2_fast(s[j][2 * h + e] - less);
+            s[j][2 * h + e] = w;
+            if constexpr (kQuantised) l[j][e] = fmaf(w, per_scale[h], l[j][e]);
+            else l[j][e] += w;
           }
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float less = m[h] == -INFINITY ? 0.0f : m[h] - kLift;
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float w0 = exp2_fast(s[j][2 * h] - less), w1 = exp2_fast(s[j][2 * h + 1] - less);
-            if constexpr (kQuantised) l[h] += w0 * per_scale[j][0] + w1 * per_scale[j][1];
-            else l[h] += w0 + w1;
-            s[j][2 * h] = w0;
-            s[j][2 * h + 1] = w1;
-            p[2 * j + h] = pack2<kBf16>(w0, w1);
-          }
-        }
+        for (int h = 0; h < 2; ++h) p[j][h] = transpose8(pack2<kBf16>(s[j][2 * h], s[j][2 * h + 1]));
+      }
 
-        // Matrices: tokens 0-7 and 8-15 of one 16-byte column, then of the next.
-        const unsigned from = shared_at(v_row(stage, t0 + (lane & 7) + (((lane >> 3) & 1) << 3)) + (lane >> 4) * 16);
+      // 16-bit matrices: d 0-7 and 8-15 of tokens 0-7, then of tokens 8-15.  Codes: tokens 0-7 and
+      // 8-15 of 16 codes, then of the next 16.
+      const unsigned v_at =
+          kQuantised ? rows_at + kV + (lane & 15) * Shape::pitch + (lane >> 4) * 16
+                     : rows_at + kV + ((lane & 7) + ((lane >> 4) << 3)) * Shape::pitch + ((lane >> 3) & 1) * 16;
+      if (Kind != T4A_I8 && partly) {
+        // An infinity or a NaN in a row that some node does not see would reach it as 0 * inf.
         bool odd = false;
-        if (partly && Kind != T4A_I8) {
-          // An infinity or a NaN in a row that some node does not see would reach it as 0 * inf.
 #pragma unroll
-          for (int k = 0; k < Dim * Shape::bytes / 32; ++k) {
-            uint32_t r[4];
-            ldmatrix4(r, from + k * 32);
+        for (int k = 0; k < Dim * Shape::bytes / 32; ++k) {
+          uint32_t r[4];
+          ldmatrix4(r, v_at + k * 32);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) odd = odd || odd_values<Kind>(r[e]);
-          }
-          odd = __any_sync(0xffffffffu, odd);
+          for (int e = 0; e < 4; ++e) odd = odd || odd_values<Kind>(r[e]);
         }
-        if (odd) {
+        if (__any_sync(0xffffffffu, odd)) {
           for (int t = 0; t < 16; ++t) {
-            const int j = t >> 3, owner = (lane & ~3) | ((t & 7) >> 1);
-            const unsigned char* row = v_row(stage, t0 + t);
+            const unsigned char* const row = my_rows + (stage - smem) + kV + t * Shape::pitch;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float w0 = __shfl_sync(0xffffffffu, j ? s[1][2 * h] : s[0][2 * h], owner);
-              const float w1 = __shfl_sync(0xffffffffu, j ? s[1][2 * h + 1] : s[0][2 * h + 1], owner);
-              const float w = t & 1 ? w1 : w0;
-              const int node = (first_row + g + 8 * h) / a.group;
-              const long long drafted = pos0 + t - context;
-              const bool sees = ((there >> t) & 1) &&
-                                (drafted < 0 || (node < live && node_sees(a, b, node, static_cast<int>(drafted))));
-              if (!sees || (kQuantised && w == 0.0f)) continue;
+            for (int j = 0; j < kRowTiles; ++j)
 #pragma unroll
-              for (int k = 0; k < kSteps; ++k) {
-                if (16 * k >= dim) break;
+              for (int e = 0; e < 2; ++e) {
+                const float w =
+                    __shfl_sync(0xffffffffu, t < 8 ? s[j][e] : s[j][2 + e], (t & 7) * 4 + c);
+                if (!sees(t, j, e) || (kQuantised && w == 0.0f)) continue;
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const int d0 = kQuantised ? 16 * k + 4 * c + 2 * e : 16 * k + 2 * c + e;
-                  const int d1 = kQuantised ? d0 + 1 : d0 + 8;
-                  o[2 * k][2 * h + e] += w * row_value<Kind>(row, d0);
-                  o[2 * k + 1][2 * h + e] += w * row_value<Kind>(row, d1);
+                for (int k = 0; k < kSteps; ++k) {
+                  if (16 * k >= dim) break;
+                  o[k][j][e] += w * row_value<Kind>(row, 16 * k + (kQuantised ? 2 * g : g));
+                  o[k][j][2 + e] += w * row_value<Kind>(row, 16 * k + (kQuantised ? 2 * g + 1 : g + 8));
                 }
               }
-            }
           }
           continue;
         }
-        if constexpr (!kQuantised) {
+      }
+      if constexpr (!kQuantised) {
 #pragma unroll
-          for (int k = 0; k < kSteps; ++k) {
-            uint32_t r[4];
-            ldmatrix4_t(r, from + k * 32);
-            mma<kBf16>(o[2 * k], p, r[0], r[1]);
-            mma<kBf16>(o[2 * k + 1], p, r[2], r[3]);
-          }
-        } else {
+        for (int k = 0; k < kSteps; ++k) {
+          uint32_t r[4];
+          ldmatrix4_t(r, v_at + k * 32);
 #pragma unroll
-          for (int k = 0; k < kSteps; k += 2) {
-            uint32_t r[4], even0, odd0, even1, odd1;
-            ldmatrix4_t(r, from + k * 16);
-            alternate<Kind>(r[0], &even0, &odd0);
-            alternate<Kind>(r[1], &even1, &odd1);
-            mma<false>(o[2 * k], p, even0, even1);
-            mma<false>(o[2 * k + 1], p, odd0, odd1);
-            alternate<Kind>(r[2], &even0, &odd0);
-            alternate<Kind>(r[3], &even1, &odd1);
-            mma<false>(o[2 * k + 2], p, even0, even1);
-            mma<false>(o[2 * k + 3], p, odd0, odd1);
-          }
+          for (int j = 0; j < kRowTiles; ++j) mma<kBf16>(o[k][j], r, p[j][0], p[j][1]);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < kSteps; k += 2) {
+          uint32_t r[4], x[4];
+          ldmatrix4_t(r, v_at + k * 16);
+          alternate<Kind>(r[0], &x[0], &x[1]);
+          alternate<Kind>(r[1], &x[2], &x[3]);
+#pragma unroll
+          for (int j = 0; j < kRowTiles; ++j) mma<false>(o[k][j], x, p[j][0], p[j][1]);
+          alternate<Kind>(r[2], &x[0], &x[1]);
+          alternate<Kind>(r[3], &x[2], &x[3]);
+#pragma unroll
+          for (int j = 0; j < kRowTiles; ++j) mma<false>(o[k + 1][j], x, p[j][0], p[j][1]);
         }
       }
     }
 
-    // The token warps' results through shared memory, which the ring no longer needs.
+    // The warps' results through shared memory, which the ring no longer needs.
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
-    float* const merged = reinterpret_cast<float*>(smem);  // [kTokenWarps][kRows][Dim]
-    float4* const stats = reinterpret_cast<float4*>(smem + kTile * Dim * 4);  // [kTokenWarps][kRows]: m, l, mz, lz
+    float* const merged = reinterpret_cast<float*>(smem);  // [4][kRows][out_pitch]
+    float4* const stats = reinterpret_cast<float4*>(smem + 4 * kRows * Shape::out_pitch * 4);  // m, l, mz, lz
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int j = 0; j < kRowTiles; ++j)
 #pragma unroll
-      for (int d = 1; d < 4; d <<= 1) {
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], d);
-        lz[h] += __shfl_xor_sync(0xffffffffu, lz[h], d);
-      }
-      const int row = token_warp * kRows + row_warp * 16 + g + 8 * h;
-      if (c == 0) stats[row] = make_float4(m[h] - kLift, l[h], mz[h], lz[h]);
-#pragma unroll
-      for (int k = 0; k < kSteps; ++k) {
-        float* to = merged + row * Dim + 16 * k;
+      for (int e = 0; e < 2; ++e) {
+        const int row = warp * kRows + 8 * j + 2 * c + e;
+        float4 st = make_float4(m[j][e] - kLift, l[j][e], -INFINITY, 0.0f);
         if constexpr (kQuantised) {
-          *reinterpret_cast<float4*>(to + 4 * c) =
-              make_float4(o[2 * k][2 * h], o[2 * k + 1][2 * h], o[2 * k][2 * h + 1], o[2 * k + 1][2 * h + 1]);
-        } else {
-          *reinterpret_cast<float2*>(to + 2 * c) = make_float2(o[2 * k][2 * h], o[2 * k][2 * h + 1]);
-          *reinterpret_cast<float2*>(to + 8 + 2 * c) = make_float2(o[2 * k + 1][2 * h], o[2 * k + 1][2 * h + 1]);
+          st.z = mz[j][e];
+          st.w = lz[j][e];
+        }
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+          st.y += __shfl_xor_sync(0xffffffffu, st.y, d);
+          if constexpr (kQuantised) st.w += __shfl_xor_sync(0xffffffffu, st.w, d);
+        }
+        if (g == 0) stats[row] = st;
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+          float* const to = merged + row * Shape::out_pitch + 16 * k;
+          to[kQuantised ? 2 * g : g] = o[k][j][e];
+          to[kQuantised ? 2 * g + 1 : g + 8] = o[k][j][2 + e];
         }
       }
-    }
     __syncthreads();
     const bool begun = tile0 == 0, whole = begun && n == at.tiles;
     const long long part = (static_cast<long long>(blockIdx.x) * 2 + (begun ? 1 : 0)) * kRows;
-    const int tile_first = at.row_tile * kRows;
     // A thread takes two columns of a row.
     for (int k = threadIdx.x; k < kRows * (Dim / 2); k += kMmaThreads) {
       const int r = k / (Dim / 2), d = 2 * (k - r * (Dim / 2));
-      if (tile_first + r >= a.rows || d >= dim) continue;
+      if (first_row + r >= a.rows || d >= dim) continue;
       float mo = -INFINITY, ml = -INFINITY;  // references of the output and of the sum
 #pragma unroll
-      for (int w = 0; w < kTokenWarps; ++w) {
+      for (int w = 0; w < 4; ++w) {
         const float4 st = stats[w * kRows + r];
         mo = fmaxf(mo, st.x);
         ml = fmaxf(ml, kQuantised ? fmaxf(st.x, st.z) : st.x);
@@ -608,17 +650,17 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim>::per_sm) k_at
       const float less_o = mo == -INFINITY ? 0.0f : mo, less_l = ml == -INFINITY ? 0.0f : ml;
       float ll = 0.0f, x = 0.0f, y = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kTokenWarps; ++w) {
+      for (int w = 0; w < 4; ++w) {
         const float4 st = stats[w * kRows + r];
         if (kQuantised && st.w != 0.0f) ll += st.w * exp2_fast(st.z - less_l);
         if (st.x == -INFINITY && st.y == 0.0f) continue;
         const float weight = exp2_fast(st.x - less_o);
-        const float2 v = *reinterpret_cast<const float2*>(merged + (w * kRows + r) * Dim + d);
+        const float2 v = *reinterpret_cast<const float2*>(merged + (w * kRows + r) * Shape::out_pitch + d);
         ll += st.y * exp2_fast(st.x - less_l);
         x += v.x * weight;
         y += v.y * weight;
       }
-      const int row = tile_first + r;
+      const int row = first_row + r;
       const bool dead = row / a.group >= live || ll == 0.0f;
       const float over = dead ? 0.0f : (mo == ml ? 1.0f : exp2_fast(less_o - less_l)) / ll;
       const float lse2 = dead ? -INFINITY : less_l + log2f(ll);

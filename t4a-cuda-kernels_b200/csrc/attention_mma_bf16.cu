@@ -6,8 +6,8 @@
 namespace t4a {
 namespace cache {
 
-int launch_mma_bf16(const AttendArgs& a, int padded, int row_warps, cudaStream_t stream, int* blocks) {
-  return launch_mma<T4A_BF16>(a, padded, row_warps, stream, blocks);
+int launch_mma_bf16(const AttendArgs& a, int padded, int row_tiles, cudaStream_t stream, int* blocks) {
+  return launch_mma<T4A_BF16>(a, padded, row_tiles, stream, blocks);
 }
 
 }  // namespace cache

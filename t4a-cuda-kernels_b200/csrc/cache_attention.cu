@@ -1,49 +1,52 @@
 // t4a_tree_attention: checks, the choice of the kernel, and the joining of parts.
+#include <initializer_list>
+
 #include "attention_launch.h"
 
 namespace t4a {
 namespace cache {
 namespace {
 
-constexpr int kJoinThreads = 128;
+constexpr int kJoinThreads = 128, kJoinWarps = kJoinThreads / 32;
 
-// One warp a query row of a head: nothing where one block had the whole unit; zeros where the
-// sequence has nothing to see; else its parts weighed by 2^(lse - max) in the blocks' order.
+// One block a query row of a head: nothing where one block of the attention had the whole unit;
+// zeros where the sequence has nothing to see; else the row's parts weighed by 2^(lse - max).  The
+// warps take every fourth part, so that a long sequence's parts (some 60 of them) come in a few
+// rounds of loads, and are added in a fixed order.  It is launched beside the attention and finds
+// its place on the line of tiles while that runs.
 __global__ void __launch_bounds__(kJoinThreads) k_join(const AttendArgs a) {
-  const int lane = threadIdx.x & 31;
-  const long long task = (static_cast<long long>(blockIdx.x) * kJoinThreads + threadIdx.x) >> 5;
-  const long long rows = static_cast<long long>(a.cache.heads) * a.rows;
-  const int b = static_cast<int>(task / rows);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (b >= a.batch) return;
-  const long long in = task - b * rows;
-  const int head = static_cast<int>(in / a.rows), row = static_cast<int>(in - static_cast<long long>(head) * a.rows);
+  __shared__ float sums[kJoinWarps][kMaxDim], weights[kJoinWarps], tops[kJoinWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, dim = a.cache.dim;
+  const unsigned rows = static_cast<unsigned>(a.cache.heads) * a.rows;
+  const int b = blockIdx.x / rows, in = blockIdx.x - b * rows, head = in / a.rows, row = in - head * a.rows;
   const int row_tile = row / a.tile_rows, r = row - row_tile * a.tile_rows;
-  const long long tiles = sequence_tiles(a, b);
-  const int dim = a.cache.dim;
+  const int tiles = sequence_tiles(a, b);
+  const Line line = read_line(a, b);
+  const int quota = quota_of(a, line.total), start = line.before + (head * a.row_tiles + row_tile) * tiles;
+  const int c0 = start / quota, c1 = tiles == 0 ? c0 : (start + tiles - 1) / quota;
+  const long long to = out_row(a, b, head, row);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (tiles == 0) {
-    const long long to = out_row(a, b, head, row);
-    for (int d = 2 * lane; d < dim; d += 64) store_out(a, to + d, 0.0f, 0.0f, true);
-    if (lane == 0) store_lse(a, b, head, row, -INFINITY);
+    for (int d = 2 * threadIdx.x; d < dim; d += 2 * kJoinThreads) store_out(a, to + d, 0.0f, 0.0f, true);
+    if (threadIdx.x == 0) store_lse(a, b, head, row, -INFINITY);
     return;
   }
-  long long total, before;
-  count_tiles(a, b, &total, &before);
-  const long long quota = quota_of(a, total);
-  const long long start = before + (static_cast<long long>(head) * a.row_tiles + row_tile) * tiles;
-  const long long c0 = start / quota, c1 = (start + tiles - 1) / quota;
   if (c0 == c1) return;
-  auto part = [&](long long c) { return (c * 2 + (c == c0 ? 1 : 0)) * a.tile_rows + r; };
+  auto part = [&](int c) { return (static_cast<long long>(c) * 2 + (c == c0 ? 1 : 0)) * a.tile_rows + r; };
   float most = -INFINITY;
-  for (long long c = c0 + lane; c <= c1; c += 32) most = fmaxf(most, a.part_lse[part(c)]);
+  for (int c = c0 + threadIdx.x; c <= c1; c += kJoinThreads) most = fmaxf(most, a.part_lse[part(c)]);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+  if (lane == 0) tops[warp] = most;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) most = fmaxf(most, tops[w]);
   const float less = most == -INFINITY ? 0.0f : most;
   float x[8], sum = 0.0f;  // columns 2 * lane + 64 * k and the next
 #pragma unroll
   for (int k = 0; k < 8; ++k) x[k] = 0.0f;
-#pragma unroll 4
-  for (long long c = c0; c <= c1; ++c) {
+#pragma unroll 8
+  for (int c = c0 + warp; c <= c1; c += kJoinWarps) {
     const long long at = part(c);
     const float w = exp2f(a.part_lse[at] - less);
     sum += w;
@@ -56,37 +59,48 @@ __global__ void __launch_bounds__(kJoinThreads) k_join(const AttendArgs a) {
       x[2 * k + 1] += w * v.y;
     }
   }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) *reinterpret_cast<float2*>(&sums[warp][2 * lane + 64 * k]) = make_float2(x[2 * k], x[2 * k + 1]);
+  if (lane == 0) weights[warp] = sum;
+  __syncthreads();
+  sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) sum += weights[w];
   const bool empty = sum == 0.0f;
   const float over = empty ? 0.0f : 1.0f / sum;
-  const long long to = out_row(a, b, head, row);
+  const int d = 2 * threadIdx.x;
+  if (d < dim) {
+    float2 v = make_float2(0.0f, 0.0f);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int d = 2 * lane + 64 * k;
-    if (d < dim) store_out(a, to + d, x[2 * k] * over, x[2 * k + 1] * over, true);
+    for (int w = 0; w < kJoinWarps; ++w) {
+      v.x += sums[w][d];
+      v.y += sums[w][d + 1];
+    }
+    store_out(a, to + d, v.x * over, v.y * over, true);
   }
-  if (lane == 0) store_lse(a, b, head, row, empty ? -INFINITY : less + log2f(sum));
+  if (threadIdx.x == 0) store_lse(a, b, head, row, empty ? -INFINITY : less + log2f(sum));
 }
 
 struct Choice {
-  int padded, row_warps, rows;
+  int padded, row_tiles, rows;
 };
 
-// Row warps to a tile: as few as hold a head's rows, up to 4.
-Choice choose(int kind, int dim, int rows) {
+// Tiles of 8 rows that a warp takes: as few as hold a head's rows, up to 4 (2 for a dim over 128,
+// whose outputs would not fit the registers).
+Choice choose(int dim, int rows) {
   Choice c;
   c.padded = dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : 256;
-  c.row_warps = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  c.rows = 16 * c.row_warps;
-  (void)kind;
+  c.row_tiles = rows <= 8 ? 1 : rows <= 16 || c.padded == 256 ? 2 : 4;
+  c.rows = 8 * c.row_tiles;
   return c;
 }
 
 int dispatch(int kind, const AttendArgs& a, const Choice& c, cudaStream_t s, int* blocks) {
   switch (kind) {
-    case T4A_F16: return launch_mma_f16(a, c.padded, c.row_warps, s, blocks);
-    case T4A_BF16: return launch_mma_bf16(a, c.padded, c.row_warps, s, blocks);
-    case T4A_I8: return launch_mma_i8(a, c.padded, c.row_warps, s, blocks);
-    default: return launch_mma_e4m3(a, c.padded, c.row_warps, s, blocks);
+    case T4A_F16: return launch_mma_f16(a, c.padded, c.row_tiles, s, blocks);
+    case T4A_BF16: return launch_mma_bf16(a, c.padded, c.row_tiles, s, blocks);
+    case T4A_I8: return launch_mma_i8(a, c.padded, c.row_tiles, s, blocks);
+    default: return launch_mma_e4m3(a, c.padded, c.row_tiles, s, blocks);
   }
 }
 
@@ -114,10 +128,21 @@ int plan_attention(int dtype, const t4a_kv_cache* cache, const t4a_cuda_layout* 
   a->nodes = static_cast<int>(nodes);
   a->group = static_cast<int>(group);
   a->rows = static_cast<int>(rows);
-  a->table_pages = static_cast<int>(table->extents[0]);
-  *choice = choose(cache->kind, a->cache.dim, a->rows);
+  const long long most_places = INT_MAX - 256;
+  const long long places = table->extents[0] > most_places / a->cache.page_size
+                               ? most_places
+                               : table->extents[0] * a->cache.page_size;
+  a->places = static_cast<int>(places);
+  a->tile_pages = kTile / a->cache.page_size;
+  a->tile_places = kTile % a->cache.page_size;
+  *choice = choose(a->cache.dim, a->rows);
   a->tile_rows = choice->rows;
   a->row_tiles = (a->rows + choice->rows - 1) / choice->rows;
+  // The line of tiles is counted in 32 bits.
+  long long tiles = (places + kTile - 1) / kTile;
+  for (long long by : {batch, static_cast<long long>(a->cache.heads), static_cast<long long>(a->row_tiles)})
+    if (plan::mul_overflows(tiles, by, &tiles)) return T4A_ERR_OVERFLOW;
+  if (tiles > INT_MAX || batch * a->cache.heads * a->rows > INT_MAX) return T4A_ERR_DOMAIN_TOO_LARGE;
   T4A_TRY(dispatch(cache->kind, *a, *choice, nullptr, &a->blocks));
   return T4A_OK;
 }
@@ -210,11 +235,8 @@ extern "C" int t4a_tree_attention(void* stream, int dtype, const t4a_kv_cache* c
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   T4A_TRY(dispatch(cache->kind, a, choice, s, nullptr));
 
-  const unsigned long long warps = static_cast<unsigned long long>(a.batch) * a.cache.heads * a.rows;
-  unsigned long long join_blocks;
-  T4A_TRY(plan::grid_of(warps, kJoinThreads / 32, &join_blocks));
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(static_cast<unsigned>(join_blocks));
+  config.gridDim = dim3(static_cast<unsigned>(a.batch) * a.cache.heads * a.rows);
   config.blockDim = dim3(kJoinThreads);
   config.stream = s;
   cudaLaunchAttribute attr[1];
