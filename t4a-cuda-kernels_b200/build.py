@@ -12,6 +12,7 @@ of csrc/ or include/, is newer than its object.
 import argparse
 import concurrent.futures
 import glob
+import importlib.util
 import os
 import subprocess
 import sys
@@ -114,6 +115,24 @@ def build_waitzero(force=False):
     return lib
 
 
+def build_binding(lib, force=False):
+    """lib/_cache_torch.so: the Python functions of binding/cache_torch.cpp over torch tensors."""
+    import sysconfig
+    spec = importlib.util.find_spec("torch")  # its headers and libraries, without importing it
+    torch_dir = os.path.dirname(spec.origin)
+    src = os.path.join(HERE, "binding", "cache_torch.cpp")
+    out = os.path.join(LIBDIR, "_cache_torch.so")
+    if force or stale(out, [src] + headers(src)):
+        cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+        includes = [os.path.join(torch_dir, "include"), os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
+                    os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
+        torch_libs = os.path.join(torch_dir, "lib")
+        run(["g++", "-std=c++17", "-O2", "-fPIC", "-shared"] + [f for i in includes for f in ("-isystem", i)] +
+            [src, "-o", out, "-L", LIBDIR, "-lt4a_b200", "-L", torch_libs, "-ltorch_python", "-ltorch_cpu", "-lc10",
+             "-lc10_cuda", "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + torch_libs])
+    return out
+
+
 def build(jobs=8, force=False):
     os.makedirs(BUILD, exist_ok=True)
     os.makedirs(LIBDIR, exist_ok=True)
@@ -129,6 +148,7 @@ def build(jobs=8, force=False):
     if force or stale(lib, objs):
         run([NVCC, "-shared"] + ARCH + ["-o", lib] + objs + ["-lcudart", "-ldl"])
     build_waitzero(force)
+    build_binding(lib, force)
     return lib
 
 

@@ -41,6 +41,7 @@ struct AttendArgs {
   int places;       // table pages * page_size, or the most that 32 bits allow
   int tile_pages, tile_places;  // kTile / page_size and kTile % page_size
   int q_bf16;      // q and out are BF16, else F16
+  int plain_copies;  // K and V have the same strides, rows fill the padded dim, and offsets / 16 fit 32 bits
   int pairs;       // q and out rows start on 4-byte boundaries
   float* part_out;  // [blocks][2][tile_rows][dim]
   float* part_lse;  // [blocks][2][tile_rows]

@@ -63,6 +63,9 @@ int launch_mma(const AttendArgs& a, int padded, int row_tiles, cudaStream_t stre
   }
 }
 
+constexpr int kTcTileRows = 128;  // rows of a unit in the tensor-memory kernel
+int launch_tc(int kind, const AttendArgs& a, int padded, cudaStream_t stream, int* blocks);
+
 int launch_mma_f16(const AttendArgs& a, int padded, int row_tiles, cudaStream_t stream, int* blocks);
 int launch_mma_bf16(const AttendArgs& a, int padded, int row_tiles, cudaStream_t stream, int* blocks);
 int launch_mma_i8(const AttendArgs& a, int padded, int row_tiles, cudaStream_t stream, int* blocks);

@@ -20,7 +20,9 @@
 // meets the codes then is relative to the largest weight * scale of its row, whatever the scales
 // are; l adds weight / scale.  Rows with a scale of 0 (or below 2^-107, which the writer does not
 // make) count in the softmax alone: they have a maximum and a sum of their own, joined at the end.
-// Q is F16 too, times a power of two that brings the row's largest magnitude into [1, 2).
+// Q is F16 too, times one power of two for the block's rows that brings their largest magnitude into
+// [2^14, 2^15): 29 binades below it are exact, and what is lost further down is 2^-38 of the
+// largest row's scores.
 // ldmatrix moves pairs of codes, so a thread's codes are not where 16-bit values would be:
 //   K: a thread's 4 neighbouring codes serve as k = 2c, 2c+1, 2c+8, 2c+9, and Q has the same order;
 //   V (transposed): a register holds codes d, d+1 of tokens t, t+1; byte permutes make the pairs
@@ -55,7 +57,7 @@ struct MmaShape {
   static constexpr int stage = kTile * pitch * 2 + (KindOf<Kind>::quantised ? kTile * 8 : 0) + 16;
   static constexpr int stages = 3;
   static constexpr int q_pitch = Dim * 2 + 16;
-  static constexpr int q_bytes = rows * q_pitch + rows * 4;
+  static constexpr int q_bytes = rows * q_pitch + 16;
   static constexpr int out_pitch = Dim + 4;  // floats: the lanes of a store meet 32 banks
   static constexpr int merge = 4 * rows * (out_pitch * 4 + 16);
   static constexpr int ring = stages * stage > merge ? stages * stage : merge;
@@ -77,6 +79,10 @@ __device__ __forceinline__ void copy16(unsigned to, const void* from, bool whole
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(whole ? 16 : 0) : "memory");
 }
 
+__device__ __forceinline__ void copy16(unsigned to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+
 __device__ __forceinline__ void copy4(unsigned to, const void* from, bool whole) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(whole ? 4 : 0) : "memory");
 }
@@ -96,12 +102,12 @@ __device__ __forceinline__ void ldmatrix4_t(uint32_t (&r)[4], unsigned at) {
 template <bool Bf16>
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (Bf16)
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -200,47 +206,49 @@ __device__ __forceinline__ float load_q(const AttendArgs& a, long long at) {
                   : __half2float(static_cast<const __half*>(a.q)[at]);
 }
 
-// The unit's query rows into shared memory [rows][Dim], 16 bits, in the order of K's fragments,
-// and what turns a row's products into base-2 scores.  A warp takes a row.
+// The unit's query rows into shared memory [rows][Dim], 16 bits, in the order of K's fragments;
+// returns what turns a product into a base-2 score.  A warp takes every fourth row.
 template <int Kind, int Dim, int kRowTiles>
-__device__ __forceinline__ void stage_q(const AttendArgs& a, int b, int head, int first_row, unsigned char* q_rows,
-                                        float* factors) {
+__device__ __forceinline__ float stage_q(const AttendArgs& a, int b, int head, int first_row, unsigned char* q_rows,
+                                         float* most_of) {
   using Shape = MmaShape<Kind, Dim, kRowTiles>;
-  constexpr int kEach = Dim / 32;
+  constexpr int kEach = Dim / 32, kMine = Shape::rows / 4;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int r = warp; r < Shape::rows; r += kMmaThreads / 32) {
-    const int row = first_row + r;
-    float x[kEach];
-    float most = 0.0f;
-    const int node = row / a.group;
+  float x[kMine][kEach], most = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int row = first_row + warp + 4 * i, node = row / a.group;
     const long long base = b * a.q_batch + node * a.q_node +
                            (static_cast<long long>(head) * a.group + (row - node * a.group)) * a.q_head;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int d = lane + 32 * i;
-      x[i] = row < a.rows && d < a.cache.dim ? load_q(a, base + d) : 0.0f;
-      most = fmaxf(most, fabsf(x[i]));
+    for (int k = 0; k < kEach; ++k) {
+      const int d = lane + 32 * k;
+      x[i][k] = row < a.rows && d < a.cache.dim ? load_q(a, base + d) : 0.0f;
+      if (fabsf(x[i][k]) < INFINITY) most = fmaxf(most, fabsf(x[i][k]));
     }
-    float down = 1.0f, factor = a.scale_log2;
-    if constexpr (KindOf<Kind>::quantised) {
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-      int e = static_cast<int>((__float_as_uint(most) >> 23) & 0xff);  // biased exponent
-      e = most == 0.0f || e == 0xff ? 127 : min(max(e, 1), 253);
-      down = __uint_as_float(static_cast<unsigned>(254 - e) << 23);  // 2^(127 - e)
-      factor *= __uint_as_float(static_cast<unsigned>(e) << 23);
-    }
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int d = lane + 32 * i, in = d & 15;
-      const int slot = KindOf<Kind>::quantised ? (d & ~15) + 2 * (in >> 2) + (in & 1) + ((in & 2) << 2) : d;
-      if constexpr (KindOf<Kind>::bf16)
-        reinterpret_cast<__nv_bfloat16*>(q_rows + r * Shape::q_pitch)[slot] = __float2bfloat16_rn(x[i]);
-      else
-        reinterpret_cast<__half*>(q_rows + r * Shape::q_pitch)[slot] = __float2half_rn(x[i] * down);
-    }
-    if (lane == 0) factors[r] = factor;
   }
+  float down = 1.0f, factor = a.scale_log2;
+  if constexpr (KindOf<Kind>::quantised) {
+    most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+    if (lane == 0) most_of[warp] = most;
+    __syncthreads();
+    most = fmaxf(fmaxf(most_of[0], most_of[1]), fmaxf(most_of[2], most_of[3]));
+    int e = static_cast<int>(__float_as_uint(most) >> 23);  // biased exponent
+    e = most == 0.0f ? 127 : max(e, 16);
+    down = __uint_as_float(static_cast<unsigned>(min(127 + 14 + 127 - e, 253)) << 23);  // 2^(14 - (e - 127))
+    factor /= down;
+  }
+#pragma unroll
+  for (int i = 0; i < kMine; ++i)
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const int d = lane + 32 * k, in = d & 15;
+      const int slot = KindOf<Kind>::quantised ? (d & ~15) + 2 * (in >> 2) + (in & 1) + ((in & 2) << 2) : d;
+      unsigned char* const q_row = q_rows + (warp + 4 * i) * Shape::q_pitch;
+      if constexpr (KindOf<Kind>::bf16) reinterpret_cast<__nv_bfloat16*>(q_row)[slot] = __float2bfloat16_rn(x[i][k]);
+      else reinterpret_cast<__half*>(q_row)[slot] = __float2half_rn(x[i][k] * down);
+    }
+  return factor;
 }
 
 template <int Kind, int Dim, int kRowTiles>
@@ -253,7 +261,7 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
   const int g = lane >> 2, c = lane & 3;
   const int dim = a.cache.dim, used = dim * Shape::bytes / 16;
   unsigned char* const q_rows = smem + Shape::ring;
-  float* const factors = reinterpret_cast<float*>(q_rows + kRows * Shape::q_pitch);
+  float* const most_of = reinterpret_cast<float*>(q_rows + kRows * Shape::q_pitch);
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   Cursor at = find_start(a, blockIdx.x);
@@ -280,7 +288,8 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
 
     // This lane's token of a tile: K's row for the lower half of the warp, V's for the upper.
     const Pages& side = lane < 16 ? a.cache.k : a.cache.v;
-    const unsigned char* const head_base = side.base + at.head * side.head;
+    const unsigned char* const k_base = a.cache.k.base + at.head * a.cache.k.head;
+    const unsigned char* const v_base = a.cache.v.base + at.head * a.cache.v.head;
     const float* const head_scale = kQuantised ? side.scale + at.head * side.scale_head : nullptr;
     const int* const my_table = a.table + b * a.table_batch;
     int pos = tile0 * kTile + 16 * warp + (lane & 15);  // of the next page to look up
@@ -311,17 +320,31 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
         if constexpr (kQuantised)
           copy4(shared_at(stage + kScales + ((lane >> 4) * kTile + 16 * warp + (lane & 15)) * 4),
                 head_scale + (there ? page * side.scale_page + at_place * side.scale_place : 0), there);
-        const unsigned char* const from = head_base + (there ? page * side.page + at_place * side.place : 0);
+        const long long off = there ? page * side.page + at_place * side.place : 0;
         const unsigned to = shared_at(my_rows + to_stage * Shape::stage);
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
+        if (a.plain_copies && bits == 0xffffu) {
+          // All tokens are there, K and V lie alike, and 16-byte units of an offset fit 32 bits.
+          const unsigned units = static_cast<unsigned>(off >> 4);
 #pragma unroll
           for (int u = 0; u < 16 * Shape::chunks / 32; ++u) {
             const int k = u * 32 + lane, t = k / Shape::chunks, chunk = k - t * Shape::chunks;
-            const unsigned char* row = reinterpret_cast<const unsigned char*>(
-                __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(from), s * 16 + t));
-            if (chunk < used) copy16(to + s * kV + t * Shape::pitch + chunk * 16, row + chunk * 16, (bits >> t) & 1);
+            const unsigned long long from =
+                static_cast<unsigned long long>(__shfl_sync(0xffffffffu, units, t) + chunk) * 16;
+            copy16(to + t * Shape::pitch + chunk * 16, k_base + from);
+            copy16(to + kV + t * Shape::pitch + chunk * 16, v_base + from);
           }
+        } else {
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+#pragma unroll 4
+            for (int u = 0; u < 16 * Shape::chunks / 32; ++u) {
+              const int k = u * 32 + lane, t = k / Shape::chunks, chunk = k - t * Shape::chunks;
+              const long long from = __shfl_sync(0xffffffffu, off, s * 16 + t);
+              if (chunk < used)
+                copy16(to + s * kV + t * Shape::pitch + chunk * 16, (s ? v_base : k_base) + from + chunk * 16,
+                       (bits >> t) & 1);
+            }
+        }
       }
       to_stage = to_stage + 1 == kStages ? 0 : to_stage + 1;
       asm volatile("cp.async.commit_group;" ::: "memory");
@@ -331,7 +354,7 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) issue(i < n);
 
-    stage_q<Kind, Dim, kRowTiles>(a, b, at.head, first_row, q_rows, factors);
+    const float factor = stage_q<Kind, Dim, kRowTiles>(a, b, at.head, first_row, q_rows, most_of);
     __syncthreads();
     // Q's fragments: [n = row g][k = 2c, 2c+1] and [k = 2c+8, 2c+9] of each step.
     uint32_t q[Shape::hold_q ? kSteps : 1][kRowTiles][2];
@@ -349,12 +372,6 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
           q[k + 1][j][1] = r[3];
         }
     }
-    float factor[kRowTiles][2];
-#pragma unroll
-    for (int j = 0; j < kRowTiles; ++j)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) factor[j][e] = factors[8 * j + 2 * c + e];
-
     float o[kSteps][kRowTiles][4];  // [columns g / g + 8][rows 2c, 2c + 1]
 #pragma unroll
     for (int k = 0; k < kSteps; ++k)
@@ -363,7 +380,7 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[k][j][e] = 0.0f;
     // Of rows 8j + 2c + e; m is the same in all lanes of a row, l a lane's own part.
-    float m[kRowTiles][2], l[kRowTiles][2];
+    float m[kRowTiles][2], l[kRowTiles][2], less[kRowTiles][2];  // less: m - kLift, 0 before any score
     float mz[kQuantised ? kRowTiles : 1][2], lz[kQuantised ? kRowTiles : 1][2];  // of V rows with a scale of 0
 #pragma unroll
     for (int j = 0; j < kRowTiles; ++j)
@@ -371,6 +388,7 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
       for (int e = 0; e < 2; ++e) {
         m[j][e] = -INFINITY;
         l[j][e] = 0.0f;
+        less[j][e] = 0.0f;
         if constexpr (kQuantised) {
           mz[j][e] = -INFINITY;
           lz[j][e] = 0.0f;
@@ -440,7 +458,7 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
         const float* const scales = reinterpret_cast<const float*>(stage + kScales) + 16 * warp + g;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float ks = scales[8 * h], vs = scales[kTile + 8 * h];
+          const float ks = scales[8 * h] * factor, vs = scales[kTile + 8 * h];
           const bool zero = vs < kLeastScale;
           const float lv = zero ? 0.0f : __log2f(vs);
           // A NaN has made the score a NaN where the row is seen, and must not touch l elsewhere.
@@ -449,14 +467,14 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
 #pragma unroll
           for (int j = 0; j < kRowTiles; ++j)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) s[j][2 * h + e] = fmaf(s[j][2 * h + e] * ks, factor[j][e], lv);
+            for (int e = 0; e < 2; ++e) s[j][2 * h + e] = fmaf(s[j][2 * h + e], ks, lv);
         }
         nothing = __any_sync(0xffffffffu, nothing);
       } else {
 #pragma unroll
         for (int j = 0; j < kRowTiles; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[j][e] *= factor[j][e & 1];
+          for (int e = 0; e < 4; ++e) s[j][e] *= factor;
       }
       // Whether row 8j + 2c + e sees token t of the 16.
       auto sees = [&](int t, int j, int e) {
@@ -486,13 +504,13 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
               if (per_scale[h] < 0.0f) high = fmaxf(high, s[j][2 * h + e]);
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, d));
-            const float to = fmaxf(mz[j][e], high), less = to == -INFINITY ? 0.0f : to;
-            lz[j][e] *= exp2_fast(mz[j][e] - less);
+            const float to = fmaxf(mz[j][e], high), base = to == -INFINITY ? 0.0f : to;
+            lz[j][e] *= exp2_fast(mz[j][e] - base);
             mz[j][e] = to;
 #pragma unroll
             for (int h = 0; h < 2; ++h)
               if (per_scale[h] < 0.0f) {
-                lz[j][e] += exp2_fast(s[j][2 * h + e] - less);
+                lz[j][e] += exp2_fast(s[j][2 * h + e] - base);
                 s[j][2 * h + e] = -INFINITY;
               }
           }
@@ -518,6 +536,7 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
             const float to = fmaxf(m[j][e], top[j][e]);
             const float shrink = to == -INFINITY ? 1.0f : exp2_fast(m[j][e] - to);
             m[j][e] = to;
+            less[j][e] = to == -INFINITY ? 0.0f : to - kLift;
             l[j][e] *= shrink;
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) {
@@ -531,10 +550,9 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
       for (int j = 0; j < kRowTiles; ++j) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float less = m[j][e] == -INFINITY ? 0.0f : m[j][e] - kLift;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float w = exp2_fast(s[j][2 * h + e] - less);
+            const float w = exp2_fast(s[j][2 * h + e] - less[j][e]);
             s[j][2 * h + e] = w;
             if constexpr (kQuantised) l[j][e] = fmaf(w, per_scale[h], l[j][e]);
             else l[j][e] += w;

@@ -1,0 +1,38 @@
+// Instances and launches of the tensor-memory attention kernel.
+#include "attention_launch.h"
+#include "attention_tc.cuh"
+
+namespace t4a {
+namespace cache {
+namespace {
+
+template <int Kind, int Dim>
+int launch_one_tc(const AttendArgs& a, cudaStream_t stream) {
+  static std::atomic<unsigned long long> allowed{0};
+  T4A_TRY(allow_shared(k_attend_tc<Kind, Dim>, TcShape<Dim>::shared, &allowed));
+  k_attend_tc<Kind, Dim><<<a.blocks, kTcThreads, TcShape<Dim>::shared, stream>>>(a);
+  return runtime::check_launch();
+}
+
+template <int Kind>
+int launch_kind_tc(const AttendArgs& a, int padded, cudaStream_t stream) {
+  return padded == 64 ? launch_one_tc<Kind, 64>(a, stream) : launch_one_tc<Kind, 128>(a, stream);
+}
+
+}  // namespace
+
+int launch_tc(int kind, const AttendArgs& a, int padded, cudaStream_t stream, int* blocks) {
+  if (blocks != nullptr) {
+    *blocks = kSms * TcShape<128>::per_sm;
+    return T4A_OK;
+  }
+  switch (kind) {
+    case T4A_F16: return launch_kind_tc<T4A_F16>(a, padded, stream);
+    case T4A_BF16: return launch_kind_tc<T4A_BF16>(a, padded, stream);
+    case T4A_I8: return launch_kind_tc<T4A_I8>(a, padded, stream);
+    default: return launch_kind_tc<T4A_E4M3>(a, padded, stream);
+  }
+}
+
+}  // namespace cache
+}  // namespace t4a

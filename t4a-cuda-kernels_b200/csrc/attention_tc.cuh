@@ -1,0 +1,738 @@
+// Attention over the paged cache on the tensor cores' own memory (tcgen05): the kernel for many
+// query rows a cache head, where products bound the call.
+//
+// A block takes 128 query rows (a unit's tile of rows), one to a lane of tensor memory, and goes
+// through the unit's tiles of 64 tokens:
+//   S = Q K^T   [128 x 64], both from shared memory, into one of two buffers of tensor memory
+//   P = 2^(S - m), by 128 threads, a row each, back into the buffer that S came from
+//   O += P V    [128 x dim], P from tensor memory, V from shared memory as it lies (d fastest)
+// so a row's maximum and sum need no exchange between threads, and P never leaves the SM's tensor
+// memory.  Roles: warps 0-3 softmax and results, warps 4-7 the cache rows, warp 8 the products' issue
+// (one thread).  S of the next tile is issued before P V of this one, and two blocks share an
+// SM (256 columns of tensor memory and some 100 KB of shared memory each), so products run while
+// exponentials are taken.  An SM takes 512 cycles for a tile's products and 512 for its 8192
+// exponentials; the two overlap.
+//
+// Shared rows of Q, K and V are 128-byte lines of 64 values, their 16-byte units XORed with the
+// line's number mod 8 (the 128-byte swizzle of the operand descriptors).  16-bit rows come there by
+// cp.async; codes come through registers, where they become F16, exactly.  Scales, weights and rows
+// with a scale of 0 are as in the kernel for few rows.
+//
+// Every wait is bounded: if one runs out all roles leave their loops, results are NaN, and tensor
+// memory is freed.
+#pragma once
+
+#include "attention_mma.cuh"
+
+namespace t4a {
+namespace cache {
+
+#ifndef T4A_STAGE_WAIT_LIMIT
+#define T4A_STAGE_WAIT_LIMIT (1u << 20)
+#endif
+
+constexpr int kTcRows = 128;
+constexpr int kTcThreads = 384;
+// Registers of a thread of each role: 80 at launch, moved between the roles.
+constexpr int kTcSoftmaxRegisters = 136, kTcLoaderRegisters = 72, kTcIssueRegisters = 32;
+static_assert(kTcSoftmaxRegisters + kTcLoaderRegisters + kTcIssueRegisters == 3 * 80, "a larger sum would wait for good");
+constexpr int kTcLoaders = 128;
+constexpr int kTcStages = 2;
+constexpr int kTcSlots = 4;  // of tiles' scales and flags: they outlive a stage by two tiles
+constexpr unsigned kTcColumns = 256;
+constexpr unsigned kTcWaitNs = 2000;
+
+// What a tile's rows carry beside their values.
+struct TcSlot {
+  float ks[kTile];  // K's scale
+  float lv[kTile];  // log2 of V's scale, -infinity for a scale of 0
+  float rv[kTile];  // 1 / V's scale
+  unsigned there[4], zero[4], odd[4];  // a loader warp's 16 tokens each
+};
+
+struct TcBarriers {
+  unsigned long long q_full, k_full[kTcStages], k_empty[kTcStages], v_full[kTcStages], v_empty[kTcStages], s_full[2],
+      p_full[2], o_done[2], slot_full[kTcSlots];
+};
+
+template <int Dim>
+struct TcShape {
+  static constexpr int blocks = Dim / 64;  // of 64 values, a line each
+  static constexpr int q_bytes = kTcRows * Dim * 2;
+  static constexpr int tile_bytes = kTile * Dim * 2;
+  static constexpr int slots_at = q_bytes + 2 * kTcStages * tile_bytes;
+  static constexpr int barriers_at = slots_at + kTcSlots * static_cast<int>(sizeof(TcSlot));
+  static constexpr int shared = barriers_at + static_cast<int>(sizeof(TcBarriers)) + 16 + 1024;  // and alignment
+  static constexpr int per_sm = 2;
+};
+
+__device__ __forceinline__ void barrier_init(unsigned long long* b, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared_at(b)), "r"(count) : "memory");
+}
+
+__device__ __forceinline__ void barrier_arrive(unsigned long long* b) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_at(b)) : "memory");
+}
+
+// False when the phase did not complete within the limit, or another role's wait ran out.
+__device__ __forceinline__ bool barrier_wait(unsigned long long* b, unsigned parity, volatile int* failed) {
+  const unsigned at = shared_at(b);
+  for (unsigned i = 0; i < T4A_STAGE_WAIT_LIMIT; ++i) {
+    unsigned ok;
+    asm volatile(
+        "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }"
+        : "=r"(ok)
+        : "r"(at), "r"(parity), "n"(kTcWaitNs)
+        : "memory");
+    if (ok) return true;
+    if (*failed) return false;
+  }
+  *failed = 1;
+  return false;
+}
+
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+__device__ __forceinline__ void tc_commit(unsigned long long* b) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(shared_at(b))
+               : "memory");
+}
+
+// 32 columns of the warp's 32 lanes.
+__device__ __forceinline__ void tc_load(uint32_t (&r)[32], unsigned at) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(at));
+}
+
+__device__ __forceinline__ void tc_store(unsigned at, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(at),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+__device__ __forceinline__ void tc_loaded() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// An operand of 128-byte lines under the 128-byte swizzle; `lines` (in bytes) leads from 8 lines to
+// the next 8, `across` from 64 values to the next 64 where they are the lines' own direction.
+__device__ __forceinline__ unsigned long long operand(unsigned at, unsigned across, unsigned lines) {
+  return static_cast<unsigned long long>((at & 0x3ffff) >> 4) | static_cast<unsigned long long>(across >> 4) << 16 |
+         static_cast<unsigned long long>(lines >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+
+__device__ __forceinline__ void tc_mma(unsigned to, unsigned long long a, unsigned long long b, unsigned form,
+                                       bool add) {
+  asm volatile(
+      "{ .reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(to),
+      "l"(a), "l"(b), "r"(form), "r"(static_cast<unsigned>(add))
+      : "memory");
+}
+
+__device__ __forceinline__ void tc_mma_from(unsigned to, unsigned a, unsigned long long b, unsigned form) {
+  asm volatile(
+      "{ .reg .pred p; setp.ne.u32 p, 1, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(to),
+      "r"(a), "l"(b), "r"(form)
+      : "memory");
+}
+
+// F32 sums of 16-bit values, M = 128; `across`: B's lines run along N.
+template <bool Bf16>
+__device__ __forceinline__ unsigned tc_form(int n, bool across) {
+  return 1u << 4 | (Bf16 ? 1u : 0u) << 7 | (Bf16 ? 1u : 0u) << 10 | (across ? 1u : 0u) << 16 |
+         static_cast<unsigned>(n >> 3) << 17 | (kTcRows >> 4) << 24;
+}
+
+template <int Kind, int Dim>
+__global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(const AttendArgs a) {
+  using Shape = TcShape<Dim>;
+  constexpr bool kQuantised = KindOf<Kind>::quantised, kBf16 = KindOf<Kind>::bf16;
+  extern __shared__ unsigned char raw[];
+  unsigned char* const smem = raw + ((1024 - (shared_at(raw) & 1023)) & 1023);
+  unsigned char* const q_lines = smem;
+  auto k_lines = [&](int stage) { return smem + Shape::q_bytes + stage * Shape::tile_bytes; };
+  auto v_lines = [&](int stage) { return smem + Shape::q_bytes + (kTcStages + stage) * Shape::tile_bytes; };
+  TcSlot* const slots = reinterpret_cast<TcSlot*>(smem + Shape::slots_at);
+  TcBarriers* const bar = reinterpret_cast<TcBarriers*>(smem + Shape::barriers_at);
+  unsigned* const tmem_at = reinterpret_cast<unsigned*>(bar + 1);
+  volatile int* const failed = reinterpret_cast<int*>(tmem_at + 1);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int dim = a.cache.dim;
+
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (threadIdx.x == 0) {
+    barrier_init(&bar->q_full, kTcRows);
+    for (int i = 0; i < kTcStages; ++i) {
+      barrier_init(&bar->k_full[i], kTcLoaders);
+      barrier_init(&bar->v_full[i], kTcLoaders);
+      barrier_init(&bar->k_empty[i], 1);
+      barrier_init(&bar->v_empty[i], 1);
+    }
+    // Two of each, in turn: a fast thread is at most one tile ahead of a slow one.
+    for (int i = 0; i < 2; ++i) {
+      barrier_init(&bar->s_full[i], 1);
+      barrier_init(&bar->p_full[i], kTcRows);
+      barrier_init(&bar->o_done[i], 1);
+    }
+    for (int i = 0; i < kTcSlots; ++i) barrier_init(&bar->slot_full[i], 4);
+    *failed = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_at(tmem_at)),
+                 "n"(kTcColumns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  // The pads past dim meet zeros of Q, or make columns that are not stored; they have to be finite.
+  if (dim < Dim)
+    for (int i = threadIdx.x; i < Shape::slots_at / 16; i += kTcThreads)
+      reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+  tc_before();
+  fence_async();
+  __syncthreads();
+  tc_after();
+  const unsigned tmem = *tmem_at, tmem_o = tmem + 128;
+
+  Cursor at = find_start(a, blockIdx.x);
+  int tiles_done = 0;  // of the block, in all its units: phases and slots go by it
+
+  if (warp >= 4 && warp < 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTcLoaderRegisters));
+    // ---- cache rows: warp w takes tokens 16 w .. 16 w + 15 of a tile ----
+    const int w = warp - 4;
+    constexpr int kChunks = Dim * KindOf<Kind>::bytes / 16;  // of a padded row
+    constexpr int kRounds = 16 * kChunks / 32;
+    const int used = dim * KindOf<Kind>::bytes / 16;
+    bool good = true;
+    while (at.left > 0 && good) {
+      const int b = at.b;
+      int context, live, length;
+      sequence_tokens(a, b, &context, &live, &length);
+      const int n = min(at.left, at.tiles - at.tile);
+      const Pages& side = lane < 16 ? a.cache.k : a.cache.v;
+      const unsigned char* const k_base = a.cache.k.base + at.head * a.cache.k.head;
+      const unsigned char* const v_base = a.cache.v.base + at.head * a.cache.v.head;
+      const int* const my_table = a.table + b * a.table_batch;
+      int pos = at.tile * kTile + 16 * w + (lane & 15);
+      int in_table = pos / a.cache.page_size, place = pos - in_table * a.cache.page_size;
+      const int end = min(length, (at.tile + n) * kTile);
+      int page_ahead, place_ahead;
+      auto look_up = [&] {
+        page_ahead = -1;
+        place_ahead = place;
+        if (pos < end) page_ahead = my_table[in_table * a.table_page];
+        pos += kTile;
+        in_table += a.tile_pages;
+        place += a.tile_places;
+        if (place >= a.cache.page_size) {
+          place -= a.cache.page_size;
+          ++in_table;
+        }
+      };
+      // The row and chunk of a lane in round u.
+      auto token_of = [&](int u) { return (u * 32 + lane) / kChunks; };
+      auto chunk_of = [&](int u) { return (u * 32 + lane) % kChunks; };
+      // Swizzled place of a 16-byte unit of 8 values of row t.
+      auto unit_at = [&](int t, int unit) {
+        return (unit >> 3) * (kTile * 128) + t * 128 + (((unit & 7) ^ (t & 7)) << 4);
+      };
+      unsigned bits = 0;
+      long long off = 0;
+      float scale = 0.0f;
+      auto step = [&] {  // the next tile's rows: where they are, and their scales
+        const int page = page_ahead, at_place = place_ahead;
+        look_up();
+        const bool there = static_cast<unsigned>(page) < static_cast<unsigned>(a.cache.pages);
+        bits = __ballot_sync(0xffffffffu, there) & 0xffffu;
+        off = there ? page * side.page + at_place * side.place : 0;
+        if constexpr (kQuantised)
+          scale = there ? side.scale[page * side.scale_page + at_place * side.scale_place + at.head * side.scale_head]
+                        : 1.0f;
+      };
+      uint4 code[kQuantised ? 2 : 1][kQuantised ? kRounds : 1];  // K's and V's
+      auto fetch = [&](int s) {
+        if constexpr (kQuantised) {
+#pragma unroll
+          for (int u = 0; u < kRounds; ++u) {
+            const int t = token_of(u), chunk = chunk_of(u);
+            const long long from = __shfl_sync(0xffffffffu, off, s * 16 + t);
+            code[s][u] = make_uint4(0, 0, 0, 0);
+            if (((bits >> t) & 1) && chunk < used)
+              code[s][u] = *reinterpret_cast<const uint4*>((s ? v_base : k_base) + from + chunk * 16);
+          }
+        }
+      };
+      // A tile's slot: what the tokens are.  E4M3 NaNs of V are noted where some node may not see them.
+      auto describe = [&](int t, unsigned the_bits, float the_scale) {
+        TcSlot& slot = slots[t % kTcSlots];
+        if (lane == 0) {
+          slot.there[w] = the_bits;
+          slot.odd[w] = 0;
+        }
+        if constexpr (kQuantised) {
+          const bool zero = the_scale < kLeastScale;
+          const unsigned zeros = __ballot_sync(0xffffffffu, zero) >> 16;
+          if (lane == 0) slot.zero[w] = zeros;
+          if (lane < 16) {
+            slot.ks[16 * w + lane] = the_scale;
+          } else {
+            const float lv = zero ? -INFINITY : __log2f(the_scale);
+            slot.lv[16 * w + lane - 16] = lv;
+            // A NaN has made the score a NaN where the row is seen, and must not touch l elsewhere.
+            slot.rv[16 * w + lane - 16] = zero ? 0.0f : the_scale == the_scale ? exp2_fast(-lv) : 1.0f;
+          }
+        }
+        __syncwarp();
+        if (lane == 0) barrier_arrive(&bar->slot_full[t % kTcSlots]);
+      };
+      // Codes to F16 lines.
+      auto unpack = [&](int s, unsigned char* lines, int t_block, bool partly) {
+        if constexpr (kQuantised) {
+#pragma unroll
+          for (int u = 0; u < kRounds; ++u) {
+            const int t = token_of(u), chunk = chunk_of(u);
+            uint32_t x[4] = {code[s][u].x, code[s][u].y, code[s][u].z, code[s][u].w}, h[8];
+            if (Kind == T4A_E4M3 && s == 1 && partly) {
+              bool odd = false;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t nan = __vcmpeq4(x[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                odd = odd || nan != 0;
+                x[e] &= ~nan;
+              }
+              if (odd) atomicOr(&slots[t_block % kTcSlots].odd[w], 1u << t);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) neighbours<Kind>(x[e], &h[2 * e], &h[2 * e + 1]);
+            // Half of the lanes store their second unit first: 8 lanes then meet 8 units.
+            const bool swap = (chunk >> 2) & 1;
+            const uint4 lo = make_uint4(h[0], h[1], h[2], h[3]), hi = make_uint4(h[4], h[5], h[6], h[7]);
+            const int t64 = 16 * w + t;
+            if (chunk < used) {
+              *reinterpret_cast<uint4*>(lines + unit_at(t64, 2 * chunk + (swap ? 1 : 0))) = swap ? hi : lo;
+              *reinterpret_cast<uint4*>(lines + unit_at(t64, 2 * chunk + (swap ? 0 : 1))) = swap ? lo : hi;
+            }
+          }
+        }
+      };
+      // 16-bit rows straight to their lines.
+      auto copy = [&](int s, unsigned char* lines, long long the_off, unsigned the_bits) {
+        if constexpr (!kQuantised) {
+          const unsigned to = shared_at(lines);
+#pragma unroll
+          for (int u = 0; u < kRounds; ++u) {
+            const int t = token_of(u), chunk = chunk_of(u);
+            const long long from = __shfl_sync(0xffffffffu, the_off, s * 16 + t);
+            if (chunk < used)
+              copy16(to + unit_at(16 * w + t, chunk), (s ? v_base : k_base) + from + chunk * 16, (the_bits >> t) & 1);
+          }
+          asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+      };
+      // Infinities and NaNs of V out of the lines of tokens that some node may not see.
+      auto clean = [&](unsigned char* lines, int t_block) {
+        if constexpr (!kQuantised) {
+#pragma unroll 1
+          for (int u = 0; u < kRounds; ++u) {
+            const int t = token_of(u), chunk = chunk_of(u);
+            if (chunk >= used) continue;
+            uint32_t* const unit = reinterpret_cast<uint32_t*>(lines + unit_at(16 * w + t, chunk));
+            bool odd = false;
+            for (int e = 0; e < 4; ++e) {
+              uint32_t x = unit[e];
+              constexpr uint32_t ones = kBf16 ? 0x7f80u : 0x7c00u;
+              if ((x & ones) == ones) x &= 0xffff0000u, odd = true;
+              if ((x & (ones << 16)) == (ones << 16)) x &= 0xffffu, odd = true;
+              unit[e] = x;
+            }
+            if (odd) atomicOr(&slots[t_block % kTcSlots].odd[w], 1u << t);
+          }
+        }
+      };
+
+      look_up();
+      step();
+      if constexpr (kQuantised) {
+        fetch(0);
+        fetch(1);
+        for (int i = 0; i < n && good; ++i) {
+          const int t = tiles_done + i, stage = t % kTcStages;
+          const unsigned turn = (t / kTcStages) & 1;
+          const bool partly = (at.tile + i + 1) * kTile > context;
+          const unsigned now_bits = bits;
+          const float now_scale = scale;
+          good = barrier_wait(&bar->k_empty[stage], turn ^ 1, failed);
+          if (!good) break;
+          describe(t, now_bits, now_scale);
+          unpack(0, k_lines(stage), t, false);
+          fence_async();
+          barrier_arrive(&bar->k_full[stage]);
+          step();
+          if (i + 1 < n) fetch(0);
+          good = barrier_wait(&bar->v_empty[stage], turn ^ 1, failed);
+          if (!good) break;
+          unpack(1, v_lines(stage), t, partly);
+          fence_async();
+          barrier_arrive(&bar->v_full[stage]);
+          if (i + 1 < n) fetch(1);
+        }
+      } else {
+        // Tile i is announced while tile i + 1 is on its way.
+        auto announce = [&](int i) {
+          const int t = tiles_done + i, stage = t % kTcStages;
+          if ((at.tile + i + 1) * kTile > context) clean(v_lines(stage), t);
+          fence_async();
+          barrier_arrive(&bar->k_full[stage]);
+          barrier_arrive(&bar->v_full[stage]);
+        };
+        for (int i = 0; i < n && good; ++i) {
+          const int t = tiles_done + i, stage = t % kTcStages;
+          const unsigned turn = (t / kTcStages) & 1;
+          const unsigned now_bits = bits;
+          const long long now_off = off;
+          good = barrier_wait(&bar->k_empty[stage], turn ^ 1, failed);
+          if (!good) break;
+          describe(t, now_bits, 0.0f);
+          copy(0, k_lines(stage), now_off, now_bits);
+          step();
+          if (i > 0) {
+            asm volatile("cp.async.wait_group 1;" ::: "memory");  // all of tile i - 1
+            announce(i - 1);
+          }
+          good = barrier_wait(&bar->v_empty[stage], turn ^ 1, failed);
+          if (!good) break;
+          copy(1, v_lines(stage), now_off, now_bits);
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (good) announce(n - 1);
+      }
+      tiles_done += n;
+      at.left -= n;
+      if (at.left > 0) next_unit(a, &at);
+    }
+  } else if (warp >= 8) {
+    // ---- products ----
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTcIssueRegisters));
+    if (warp == 8 && lane == 0) {
+      const unsigned form_s = tc_form<kBf16>(kTile, false), form_o = tc_form<kBf16>(Dim, true);
+      const unsigned q_at = shared_at(q_lines);
+      bool good = true;
+      unsigned unit = 0;
+      while (at.left > 0 && good) {
+        const int n = min(at.left, at.tiles - at.tile);
+        good = barrier_wait(&bar->q_full, unit & 1, failed);
+        for (int i = 0; i <= n && good; ++i) {
+          if (i < n) {
+            const int t = tiles_done + i, stage = t % kTcStages;
+            good = barrier_wait(&bar->k_full[stage], (t / kTcStages) & 1, failed);
+            if (!good) break;
+            tc_after();
+            const unsigned k_at = shared_at(k_lines(stage));
+#pragma unroll
+            for (int k = 0; k < Dim / 16; ++k)
+              tc_mma(tmem + (t & 1) * 64, operand(q_at + (k >> 2) * kTcRows * 128 + (k & 3) * 32, 16, 1024),
+                     operand(k_at + (k >> 2) * kTile * 128 + (k & 3) * 32, 16, 1024), form_s, k > 0);
+            tc_commit(&bar->k_empty[stage]);
+            tc_commit(&bar->s_full[t & 1]);
+          }
+          if (i > 0) {
+            const int t = tiles_done + i - 1, stage = t % kTcStages;
+            good = barrier_wait(&bar->v_full[stage], (t / kTcStages) & 1, failed) &&
+                   barrier_wait(&bar->p_full[t & 1], (t >> 1) & 1, failed);
+            if (!good) break;
+            tc_after();
+            const unsigned v_at = shared_at(v_lines(stage));
+#pragma unroll
+            for (int k = 0; k < kTile / 16; ++k)
+              tc_mma_from(tmem_o, tmem + (t & 1) * 64 + k * 8, operand(v_at + k * 2048, kTile * 128, 1024), form_o);
+            tc_commit(&bar->v_empty[stage]);
+            tc_commit(&bar->o_done[t & 1]);
+          }
+        }
+        tiles_done += n;
+        ++unit;
+        at.left -= n;
+        if (at.left > 0) next_unit(a, &at);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---- softmax: thread r has query row r of the tile ----
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTcSoftmaxRegisters));
+    const unsigned lanes = static_cast<unsigned>(warp * 32) << 16;
+    const int r = threadIdx.x;
+    bool good = true;
+    while (at.left > 0) {
+      const int b = at.b;
+      int context, live, length;
+      sequence_tokens(a, b, &context, &live, &length);
+      const int n = min(at.left, at.tiles - at.tile);
+      const int row = at.row_tile * kTcRows + r, node = row / a.group;
+      const bool here = row < a.rows && node < live, any_here = __any_sync(0xffffffffu, here);
+      float factor = a.scale_log2;
+      {
+        // The row into its lines, and zeros into its lanes of O.
+        const long long base = b * a.q_batch + node * a.q_node +
+                               (static_cast<long long>(at.head) * a.group + (row - node * a.group)) * a.q_head;
+        float down = 1.0f;
+        if constexpr (kQuantised) {
+          float most = 0.0f;
+          for (int d = 0; d < dim; ++d) {
+            const float v = here ? fabsf(load_q(a, base + d)) : 0.0f;
+            if (v < INFINITY) most = fmaxf(most, v);
+          }
+          int e = static_cast<int>(__float_as_uint(most) >> 23);  // biased exponent
+          e = most == 0.0f ? 127 : max(e, 16);
+          down = __uint_as_float(static_cast<unsigned>(min(127 + 14 + 127 - e, 253)) << 23);
+          factor /= down;
+        }
+#pragma unroll 2
+        for (int unit = 0; unit < Dim / 8; ++unit) {
+          uint32_t h[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int d = 8 * unit + 2 * e;
+            float x = 0.0f, y = 0.0f;
+            if (here && d < dim) {
+              x = load_q(a, base + d) * down;
+              y = load_q(a, base + d + 1) * down;
+            }
+            h[e] = pack2<kBf16>(x, y);
+          }
+          *reinterpret_cast<uint4*>(q_lines + (unit >> 3) * (kTcRows * 128) + r * 128 + (((unit & 7) ^ (r & 7)) << 4)) =
+              make_uint4(h[0], h[1], h[2], h[3]);
+        }
+        uint32_t zero[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) zero[e] = 0;
+#pragma unroll
+        for (int d = 0; d < Dim; d += 32) tc_store(tmem_o + lanes + d, zero);
+        tc_stored();
+        tc_before();
+        fence_async();
+        barrier_arrive(&bar->q_full);
+      }
+      float m = -INFINITY, less = -1e30f, l = 0.0f, mz = -INFINITY, lz = 0.0f;
+      for (int i = 0; i < n && good; ++i) {
+        const int t = tiles_done + i;
+        good = barrier_wait(&bar->slot_full[t % kTcSlots], (t / kTcSlots) & 1, failed) &&
+               barrier_wait(&bar->s_full[t & 1], (t >> 1) & 1, failed);
+        if (!good) break;
+        tc_after();
+        if (any_here) {
+          const TcSlot& slot = slots[t % kTcSlots];
+          const int pos0 = (at.tile + i) * kTile;
+          const unsigned s_at = tmem + (t & 1) * 64 + lanes;
+          uint32_t s0[32], s1[32];
+          tc_load(s0, s_at);
+          tc_load(s1, s_at + 32);
+          tc_loaded();
+          auto s = [&](int j) -> uint32_t& { return j < 32 ? s0[j] : s1[j - 32]; };
+          const unsigned there_lo = slot.there[0] | slot.there[1] << 16, there_hi = slot.there[2] | slot.there[3] << 16;
+          const bool partly = (there_lo & there_hi) != 0xffffffffu || pos0 + kTile > context;
+          unsigned see_lo = there_lo, see_hi = there_hi;
+          if (partly) {
+            for (int j = max(0, context - pos0); j < kTile && pos0 + j < length; ++j) {
+              const bool sees = here && node_sees(a, b, node, pos0 + j - context) && pos0 + j - context < live;
+              if (!sees) {
+                if (j < 32) see_lo &= ~(1u << j);
+                else see_hi &= ~(1u << (j - 32));
+              }
+            }
+          }
+          if constexpr (kQuantised) {
+            const unsigned zero_lo = slot.zero[0] | slot.zero[1] << 16, zero_hi = slot.zero[2] | slot.zero[3] << 16;
+            if (zero_lo | zero_hi) {
+              float high = -INFINITY;
+#pragma unroll
+              for (int j = 0; j < kTile; ++j)
+                if (((j < 32 ? zero_lo & see_lo : zero_hi & see_hi) >> (j & 31)) & 1)
+                  high = fmaxf(high, __uint_as_float(s(j)) * slot.ks[j] * factor);
+              const float to = fmaxf(mz, high), base = to == -INFINITY ? 0.0f : to;
+              lz *= exp2_fast(mz - base);
+              mz = to;
+#pragma unroll
+              for (int j = 0; j < kTile; ++j)
+                if (((j < 32 ? zero_lo & see_lo : zero_hi & see_hi) >> (j & 31)) & 1)
+                  lz += exp2_fast(__uint_as_float(s(j)) * slot.ks[j] * factor - base);
+            }
+#pragma unroll
+            for (int j = 0; j < kTile; j += 4) {
+              const float4 ks = *reinterpret_cast<const float4*>(&slot.ks[j]);
+              const float4 lv = *reinterpret_cast<const float4*>(&slot.lv[j]);
+              s(j) = __float_as_uint(fmaf(__uint_as_float(s(j)), ks.x * factor, lv.x));
+              s(j + 1) = __float_as_uint(fmaf(__uint_as_float(s(j + 1)), ks.y * factor, lv.y));
+              s(j + 2) = __float_as_uint(fmaf(__uint_as_float(s(j + 2)), ks.z * factor, lv.z));
+              s(j + 3) = __float_as_uint(fmaf(__uint_as_float(s(j + 3)), ks.w * factor, lv.w));
+            }
+            // A scale of 0 leaves -infinity, unless the product was a NaN or an infinity.
+            if (zero_lo | zero_hi) {
+#pragma unroll
+              for (int j = 0; j < kTile; ++j)
+                if (((j < 32 ? zero_lo : zero_hi) >> (j & 31)) & 1) s(j) = __float_as_uint(-INFINITY);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < kTile; ++j) s(j) = __float_as_uint(__uint_as_float(s(j)) * factor);
+          }
+          if (partly) {
+#pragma unroll
+            for (int j = 0; j < kTile; ++j)
+              if (!(((j < 32 ? see_lo : see_hi) >> (j & 31)) & 1)) s(j) = __float_as_uint(-INFINITY);
+          }
+          float top = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < kTile; ++j) top = fmaxf(top, __uint_as_float(s(j)));
+          const bool rises = here && top > less + (kSlack + kLift);
+          if (__any_sync(0xffffffffu, rises)) {
+            float shrink = 1.0f;
+            if (rises) {
+              shrink = exp2_fast(m - top);
+              m = top;
+              less = top - kLift;
+              l *= shrink;
+            }
+            if (i > 0) {
+              good = barrier_wait(&bar->o_done[(t - 1) & 1], ((t - 1) >> 1) & 1, failed);
+              tc_after();
+              uint32_t o[32];
+#pragma unroll 1
+              for (int d = 0; d < Dim; d += 32) {
+                tc_load(o, tmem_o + lanes + d);
+                tc_loaded();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink);
+                tc_store(tmem_o + lanes + d, o);
+              }
+              tc_stored();
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < kTile; j += 4) {
+            float w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = exp2_fast(__uint_as_float(s(j + e)) - less);
+            if constexpr (kQuantised) {
+              const float4 rv = *reinterpret_cast<const float4*>(&slot.rv[j]);
+              l = fmaf(w[0], rv.x, fmaf(w[1], rv.y, fmaf(w[2], rv.z, fmaf(w[3], rv.w, l))));
+            } else {
+              l += (w[0] + w[1]) + (w[2] + w[3]);
+            }
+            s(j) = __float_as_uint(w[0]);
+            s(j + 1) = __float_as_uint(w[1]);
+            s(j + 2) = __float_as_uint(w[2]);
+            s(j + 3) = __float_as_uint(w[3]);
+          }
+          if (Kind != T4A_I8 && partly) {
+            // What was cleaned out of V reaches the rows that see it.
+            good = good && barrier_wait(&bar->v_full[t % kTcStages], (t / kTcStages) & 1, failed);
+            const unsigned odd_lo = slot.odd[0] | slot.odd[1] << 16, odd_hi = slot.odd[2] | slot.odd[3] << 16;
+            if (good && (odd_lo | odd_hi)) {
+              if (i > 0) good = barrier_wait(&bar->o_done[(t - 1) & 1], ((t - 1) >> 1) & 1, failed);
+              tc_after();
+#pragma unroll 1
+              for (int d = 0; d < Dim; d += 32) {
+                uint32_t o[32];
+                tc_load(o, tmem_o + lanes + d);
+                tc_loaded();
+#pragma unroll 1
+                for (int j = 0; j < kTile; ++j) {
+                  if (!(((j < 32 ? odd_lo : odd_hi) >> (j & 31)) & 1)) continue;
+                  if (!(((j < 32 ? see_lo : see_hi) >> (j & 31)) & 1) || !here) continue;
+                  float w = 0.0f;
+#pragma unroll
+                  for (int e = 0; e < kTile; ++e) w = e == j ? __uint_as_float(s(e)) : w;
+                  const int at_pos = pos0 + j, page = a.table[b * a.table_batch + (at_pos / a.cache.page_size) * a.table_page];
+                  const unsigned char* const v_row = a.cache.v.base + at.head * a.cache.v.head + page * a.cache.v.page +
+                                                     (at_pos % a.cache.page_size) * a.cache.v.place;
+#pragma unroll
+                  for (int e = 0; e < 32; ++e) {
+                    if (d + e >= dim) continue;
+                    const float v = row_value<Kind>(v_row, d + e);
+                    if (!(fabsf(v) < INFINITY)) o[e] = __float_as_uint(__uint_as_float(o[e]) + w * v);
+                  }
+                }
+                __syncwarp();
+                tc_store(tmem_o + lanes + d, o);
+              }
+              tc_stored();
+            }
+          }
+          uint32_t p[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            p[j] = pack2<kBf16>(__uint_as_float(s(2 * j)), __uint_as_float(s(2 * j + 1)));
+          tc_store(s_at, p);
+          tc_stored();
+          tc_before();
+        }
+        barrier_arrive(&bar->p_full[t & 1]);
+      }
+      tiles_done += n;
+      if (good) good = barrier_wait(&bar->o_done[(tiles_done - 1) & 1], ((tiles_done - 1) >> 1) & 1, failed);
+      tc_after();
+      const bool begun = at.tile == 0, whole = begun && n == at.tiles;
+      if (any_here || whole) {
+        // Sums relative to the larger reference; O stays relative to its own.
+        const float mo = m == -INFINITY ? 0.0f : less;
+        const float ml = kQuantised ? fmaxf(m == -INFINITY ? -INFINITY : less, mz) : (m == -INFINITY ? -INFINITY : less);
+        const float less_l = ml == -INFINITY ? 0.0f : ml;
+        float ll = l != 0.0f ? l * exp2_fast(mo - less_l) : 0.0f;
+        if (kQuantised && lz != 0.0f) ll += lz * exp2_fast(mz - less_l);
+        const bool dead = !here || ll == 0.0f;
+        float over = dead ? 0.0f : (mo == less_l ? 1.0f : exp2_fast(mo - less_l)) / ll;
+        float lse2 = dead ? -INFINITY : less_l + log2f(ll);
+        if (!good) over = lse2 = __uint_as_float(0x7fc00000u);
+        const long long part = (static_cast<long long>(blockIdx.x) * 2 + (begun ? 1 : 0)) * kTcRows + r;
+        const long long to = row < a.rows ? out_row(a, b, at.head, row) : 0;
+#pragma unroll 1
+        for (int d = 0; d < Dim; d += 32) {
+          uint32_t o[32];
+          tc_load(o, tmem_o + lanes + d);
+          tc_loaded();
+          if (row >= a.rows) continue;
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            if (d + e >= dim) break;
+            const float x = dead && good ? 0.0f : __uint_as_float(o[e]) * over;
+            const float y = dead && good ? 0.0f : __uint_as_float(o[e + 1]) * over;
+            if (whole) store_out(a, to + d + e, x, y, true);
+            else *reinterpret_cast<float2*>(a.part_out + part * dim + d + e) = make_float2(x, y);
+          }
+        }
+        if (row < a.rows) {
+          if (whole) store_lse(a, b, at.head, row, lse2);
+          else a.part_lse[part] = lse2;
+        }
+      } else if (row < a.rows) {
+        a.part_lse[(static_cast<long long>(blockIdx.x) * 2 + (begun ? 1 : 0)) * kTcRows + r] = -INFINITY;
+        float* const to = a.part_out + ((static_cast<long long>(blockIdx.x) * 2 + (begun ? 1 : 0)) * kTcRows + r) * dim;
+        for (int d = 0; d < dim; ++d) to[d] = 0.0f;
+      }
+      tc_before();
+      at.left -= n;
+      if (at.left > 0) next_unit(a, &at);
+    }
+  }
+  __syncthreads();
+  if (warp == 8) {
+    tc_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kTcColumns) : "memory");
+  }
+}
+
+}  // namespace cache
+}  // namespace t4a

@@ -82,20 +82,27 @@ __global__ void __launch_bounds__(kJoinThreads) k_join(const AttendArgs a) {
 }
 
 struct Choice {
-  int padded, row_tiles, rows;
+  int padded, row_tiles, rows;  // row_tiles 0: the tensor-memory kernel
 };
 
-// Tiles of 8 rows that a warp takes: as few as hold a head's rows, up to 4 (2 for a dim over 128,
-// whose outputs would not fit the registers).
+// Up to 32 rows a head: warp-level products over tiles of 8 rows, as few as hold them (2 at most for
+// a dim over 128, whose outputs would not fit the registers).  More rows: 128 in tensor memory; a
+// dim over 128 does not fit there beside a second block.
 Choice choose(int dim, int rows) {
   Choice c;
   c.padded = dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : 256;
   c.row_tiles = rows <= 8 ? 1 : rows <= 16 || c.padded == 256 ? 2 : 4;
   c.rows = 8 * c.row_tiles;
+  if (rows > 32 && c.padded <= 128) {
+    c.padded = dim <= 64 ? 64 : 128;
+    c.row_tiles = 0;
+    c.rows = kTcTileRows;
+  }
   return c;
 }
 
 int dispatch(int kind, const AttendArgs& a, const Choice& c, cudaStream_t s, int* blocks) {
+  if (c.row_tiles == 0) return launch_tc(kind, a, c.padded, s, blocks);
   switch (kind) {
     case T4A_F16: return launch_mma_f16(a, c.padded, c.row_tiles, s, blocks);
     case T4A_BF16: return launch_mma_bf16(a, c.padded, c.row_tiles, s, blocks);
@@ -224,6 +231,10 @@ extern "C" int t4a_tree_attention(void* stream, int dtype, const t4a_kv_cache* c
   a.out_node = out_layout->strides[2];
   a.out_batch = out_layout->strides[3];
   a.pairs = rows_aligned(q, *q_layout, 2, 4) && rows_aligned(out, *out_layout, 2, 4);
+  const Pages &k = a.cache.k, &v = a.cache.v;
+  const long long last = (a.cache.pages - 1) * k.page + (a.cache.page_size - 1ll) * k.place + a.cache.dim * 2;
+  a.plain_copies = k.page == v.page && k.place == v.place && k.page >= 0 && k.place >= 0 &&
+                   a.cache.dim == choice.padded && last / 16 < 0xffffffffll;
   a.table = table + table_layout->offset;
   a.table_page = table_layout->strides[0];
   a.table_batch = table_layout->strides[1];
