@@ -1,11 +1,12 @@
 // What the kernels of t4a_tree_attention share: the arguments, the division of the work, and the
 // joining of parts.
 //
-// A unit is one cache head of one sequence with a tile of its query rows (row r of a head: node
-// r / group, head-in-group r % group).  Its cache rows come in tiles of kTile tokens.  All units'
-// tiles lie end to end on one line, and every block takes an equal stretch of it, so a ragged
-// batch, a single long sequence and a large batch load the SMs alike.  A unit that several
-// blocks share leaves parts (its output over the part's own softmax sum, and the base-2 log of
+// A unit is one cache head of one sequence.  Its cache rows come in tiles of kTile tokens, and all
+// units' tiles lie end to end on one line, of which every group of blocks takes an equal stretch, so
+// a ragged batch, a single long sequence and a large batch load the SMs alike.  A group has a block
+// for each tile of a head's query rows (row r of a head: node r / group, head-in-group r % group):
+// its blocks pass over the same cache rows together, and all but one find them in L2.  A unit that
+// several groups share leaves parts (its output over the part's own softmax sum, and the base-2 log of
 // that sum); k_join weighs them by 2^(lse - max) in a fixed order.  No atomics: the same inputs
 // give the same bits.
 #pragma once
@@ -42,10 +43,11 @@ struct AttendArgs {
   int tile_pages, tile_places;  // kTile / page_size and kTile % page_size
   int q_bf16;      // q and out are BF16, else F16
   int plain_copies;  // K and V have the same strides, rows fill the padded dim, and offsets / 16 fit 32 bits
+  int q_units;     // q rows start on 16-byte boundaries
   int pairs;       // q and out rows start on 4-byte boundaries
-  float* part_out;  // [blocks][2][tile_rows][dim]
-  float* part_lse;  // [blocks][2][tile_rows]
-  int blocks;
+  float* part_out;  // [groups][row_tiles][2][tile_rows][dim]
+  float* part_lse;  // [groups][row_tiles][2][tile_rows]
+  int groups;       // of row_tiles blocks each
 };
 
 // Tokens that sequence b's rows can see: committed ones, and all with the drafted ones.  Places
@@ -77,7 +79,7 @@ struct Line {
 };
 
 __device__ __forceinline__ Line read_line(const AttendArgs& a, int upto) {
-  const int lane = threadIdx.x & 31, units = a.cache.heads * a.row_tiles;
+  const int lane = threadIdx.x & 31, units = a.cache.heads;
   Line n = {};
   for (int b0 = 0; b0 < a.batch; b0 += 32) {
     const int b = b0 + lane, mine = b < a.batch ? sequence_tiles(a, b) * units : 0;
@@ -88,13 +90,14 @@ __device__ __forceinline__ Line read_line(const AttendArgs& a, int upto) {
 }
 
 __device__ __forceinline__ int quota_of(const AttendArgs& a, int total) {
-  return max(1, (total + a.blocks - 1) / a.blocks);
+  return max(1, (total + a.groups - 1) / a.groups);
 }
 
-// The start of block `block`'s stretch (left 0 where it has none).
+// The start of a block's stretch (left 0 where it has none).
 __device__ __forceinline__ Cursor find_start(const AttendArgs& a, int block) {
-  const int lane = threadIdx.x & 31, units = a.cache.heads * a.row_tiles;
+  const int lane = threadIdx.x & 31, units = a.cache.heads, group = block / a.row_tiles;
   Cursor c = {};
+  c.row_tile = block - group * a.row_tiles;
   int total = 0, kept = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 32) {
     const int b = b0 + lane;
@@ -102,7 +105,7 @@ __device__ __forceinline__ Cursor find_start(const AttendArgs& a, int block) {
     total += __reduce_add_sync(0xffffffffu, kept);
   }
   const int quota = quota_of(a, total);
-  const long long far = static_cast<long long>(quota) * block;
+  const long long far = static_cast<long long>(quota) * group;
   if (far >= total) return c;
   const int start = static_cast<int>(far);
   c.left = min(quota, total - start);
@@ -123,8 +126,7 @@ __device__ __forceinline__ Cursor find_start(const AttendArgs& a, int block) {
       const int in = start - before - __shfl_sync(0xffffffffu, sum - mine, at), unit = in / c.tiles;
       c.b = b0 + at;
       c.tile = in - unit * c.tiles;
-      c.head = unit / a.row_tiles;
-      c.row_tile = unit - c.head * a.row_tiles;
+      c.head = unit;
       return c;
     }
     before += __shfl_sync(0xffffffffu, sum, 31);
@@ -136,8 +138,6 @@ __device__ __forceinline__ Cursor find_start(const AttendArgs& a, int block) {
 // The next unit with tiles; called with left > 0, so there is one.
 __device__ __forceinline__ void next_unit(const AttendArgs& a, Cursor* c) {
   c->tile = 0;
-  if (++c->row_tile < a.row_tiles) return;
-  c->row_tile = 0;
   if (++c->head < a.cache.heads) return;
   c->head = 0;
   do ++c->b;

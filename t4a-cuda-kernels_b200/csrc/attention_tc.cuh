@@ -43,11 +43,21 @@ constexpr unsigned kTcColumns = 256;
 constexpr unsigned kTcWaitNs = 2000;
 
 // What a tile's rows carry beside their values.
-struct TcSlot {
+struct alignas(16) TcSlot {
   float ks[kTile];  // K's scale
   float lv[kTile];  // log2 of V's scale, -infinity for a scale of 0
   float rv[kTile];  // 1 / V's scale
-  unsigned there[4], zero[4], odd[4];  // a loader warp's 16 tokens each
+  // A bit a token; a loader warp writes the half word of its 16.
+  __align__(8) unsigned short there[4];
+  __align__(8) unsigned short zero[4];
+  __align__(8) unsigned odd[2];
+};
+
+static_assert(sizeof(TcSlot) % 16 == 0, "slots are read 16 bytes at a time");
+
+// Scales that change nothing, for scores that have had theirs.
+struct alignas(16) TcNeutral {
+  float ones[kTile], zeros[kTile];
 };
 
 struct TcBarriers {
@@ -61,7 +71,8 @@ struct TcShape {
   static constexpr int q_bytes = kTcRows * Dim * 2;
   static constexpr int tile_bytes = kTile * Dim * 2;
   static constexpr int slots_at = q_bytes + 2 * kTcStages * tile_bytes;
-  static constexpr int barriers_at = slots_at + kTcSlots * static_cast<int>(sizeof(TcSlot));
+  static constexpr int neutral_at = slots_at + kTcSlots * static_cast<int>(sizeof(TcSlot));
+  static constexpr int barriers_at = neutral_at + static_cast<int>(sizeof(TcNeutral));
   static constexpr int shared = barriers_at + static_cast<int>(sizeof(TcBarriers)) + 16 + 1024;  // and alignment
   static constexpr int per_sm = 2;
 };
@@ -155,6 +166,107 @@ __device__ __forceinline__ unsigned tc_form(int n, bool across) {
          static_cast<unsigned>(n >> 3) << 17 | (kTcRows >> 4) << 24;
 }
 
+__device__ __forceinline__ void tc_load1(uint32_t* r, unsigned at) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(*r) : "r"(at));
+}
+
+__device__ __forceinline__ void tc_load16(uint32_t (&r)[16], unsigned at) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(at));
+}
+
+__device__ __forceinline__ void tc_store16(unsigned at, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// Two F32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(r)
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)),
+        "l"(*reinterpret_cast<unsigned long long*>(&c)));
+  return *reinterpret_cast<float2*>(&r);
+}
+
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(r)
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+  return *reinterpret_cast<float2*>(&r);
+}
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(r)
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+  return *reinterpret_cast<float2*>(&r);
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+__device__ __forceinline__ float highest(const uint32_t (&s)[32]) {
+  float x[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    x[k] = fmaxf(__uint_as_float(s[8 * k]), __uint_as_float(s[8 * k + 1]));
+#pragma unroll
+    for (int j = 2; j < 8; j += 2) x[k] = max3(x[k], __uint_as_float(s[8 * k + j]), __uint_as_float(s[8 * k + j + 1]));
+  }
+  return fmaxf(max3(x[0], x[1], x[2]), x[3]);
+}
+
+// Products of codes to base-2 scores.
+__device__ __forceinline__ void scale_scores(uint32_t (&s)[32], const float* ks, const float* lv, float factor) {
+  const float2 f = make_float2(factor, factor);
+#pragma unroll
+  for (int j = 0; j < 32; j += 4) {
+    const float4 k = *reinterpret_cast<const float4*>(ks + j), v = *reinterpret_cast<const float4*>(lv + j);
+    const float2 lo = fma2(make_float2(__uint_as_float(s[j]), __uint_as_float(s[j + 1])),
+                           mul2(make_float2(k.x, k.y), f), make_float2(v.x, v.y));
+    const float2 hi = fma2(make_float2(__uint_as_float(s[j + 2]), __uint_as_float(s[j + 3])),
+                           mul2(make_float2(k.z, k.w), f), make_float2(v.z, v.w));
+    s[j] = __float_as_uint(lo.x);
+    s[j + 1] = __float_as_uint(lo.y);
+    s[j + 2] = __float_as_uint(hi.x);
+    s[j + 3] = __float_as_uint(hi.y);
+  }
+}
+
+// Weights 2^(s * factor - less) as pairs of 16-bit values, and their sums (over V's scale).
+template <bool Quantised, bool Bf16>
+__device__ __forceinline__ void weights(const uint32_t (&s)[32], uint32_t* p, float factor, float less, const float* rv,
+                                        float2 (&l)[2]) {
+  const float2 f = make_float2(factor, factor), minus = make_float2(-less, -less);
+#pragma unroll
+  for (int j = 0; j < 32; j += 4) {
+    float4 r;
+    if constexpr (Quantised) r = *reinterpret_cast<const float4*>(rv + j);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float2 x = make_float2(__uint_as_float(s[j + 2 * e]), __uint_as_float(s[j + 2 * e + 1]));
+      const float2 y = Quantised ? add2(x, minus) : fma2(x, f, minus);
+      const float2 w = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+      if constexpr (Quantised) l[e] = fma2(w, e ? make_float2(r.z, r.w) : make_float2(r.x, r.y), l[e]);
+      else l[e] = add2(l[e], w);
+      p[(j >> 1) + e] = pack2<Bf16>(w.x, w.y);
+    }
+  }
+}
+
 template <int Kind, int Dim>
 __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(const AttendArgs a) {
   using Shape = TcShape<Dim>;
@@ -165,6 +277,8 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
   auto k_lines = [&](int stage) { return smem + Shape::q_bytes + stage * Shape::tile_bytes; };
   auto v_lines = [&](int stage) { return smem + Shape::q_bytes + (kTcStages + stage) * Shape::tile_bytes; };
   TcSlot* const slots = reinterpret_cast<TcSlot*>(smem + Shape::slots_at);
+  float* const ones = reinterpret_cast<TcNeutral*>(smem + Shape::neutral_at)->ones;
+  float* const zeros = reinterpret_cast<TcNeutral*>(smem + Shape::neutral_at)->zeros;
   TcBarriers* const bar = reinterpret_cast<TcBarriers*>(smem + Shape::barriers_at);
   unsigned* const tmem_at = reinterpret_cast<unsigned*>(bar + 1);
   volatile int* const failed = reinterpret_cast<int*>(tmem_at + 1);
@@ -172,6 +286,10 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
   const int dim = a.cache.dim;
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (threadIdx.x < kTile) {
+    ones[threadIdx.x] = 1.0f;
+    zeros[threadIdx.x] = 0.0f;
+  }
   if (threadIdx.x == 0) {
     barrier_init(&bar->q_full, kTcRows);
     for (int i = 0; i < kTcStages; ++i) {
@@ -279,13 +397,13 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
       auto describe = [&](int t, unsigned the_bits, float the_scale) {
         TcSlot& slot = slots[t % kTcSlots];
         if (lane == 0) {
-          slot.there[w] = the_bits;
-          slot.odd[w] = 0;
+          slot.there[w] = static_cast<unsigned short>(the_bits);
+          reinterpret_cast<unsigned short*>(slot.odd)[w] = 0;
         }
         if constexpr (kQuantised) {
           const bool zero = the_scale < kLeastScale;
           const unsigned zeros = __ballot_sync(0xffffffffu, zero) >> 16;
-          if (lane == 0) slot.zero[w] = zeros;
+          if (lane == 0) slot.zero[w] = static_cast<unsigned short>(zeros);
           if (lane < 16) {
             slot.ks[16 * w + lane] = the_scale;
           } else {
@@ -313,7 +431,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
                 odd = odd || nan != 0;
                 x[e] &= ~nan;
               }
-              if (odd) atomicOr(&slots[t_block % kTcSlots].odd[w], 1u << t);
+              if (odd) atomicOr(&slots[t_block % kTcSlots].odd[w >> 1], 1u << (16 * (w & 1) + t));
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) neighbours<Kind>(x[e], &h[2 * e], &h[2 * e + 1]);
@@ -332,6 +450,18 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
       auto copy = [&](int s, unsigned char* lines, long long the_off, unsigned the_bits) {
         if constexpr (!kQuantised) {
           const unsigned to = shared_at(lines);
+          if (a.plain_copies && the_bits == 0xffffu) {
+            const unsigned units = static_cast<unsigned>(the_off >> 4);
+            const unsigned char* const base = s ? v_base : k_base;
+#pragma unroll
+            for (int u = 0; u < kRounds; ++u) {
+              const int t = token_of(u), chunk = chunk_of(u);
+              const unsigned from = __shfl_sync(0xffffffffu, units, t) + chunk;
+              copy16(to + unit_at(16 * w + t, chunk), base + static_cast<unsigned long long>(from) * 16);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            return;
+          }
 #pragma unroll
           for (int u = 0; u < kRounds; ++u) {
             const int t = token_of(u), chunk = chunk_of(u);
@@ -358,7 +488,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
               if ((x & (ones << 16)) == (ones << 16)) x &= 0xffffu, odd = true;
               unit[e] = x;
             }
-            if (odd) atomicOr(&slots[t_block % kTcSlots].odd[w], 1u << t);
+            if (odd) atomicOr(&slots[t_block % kTcSlots].odd[w >> 1], 1u << (16 * (w & 1) + t));
           }
         }
       };
@@ -482,38 +612,76 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
       const int n = min(at.left, at.tiles - at.tile);
       const int row = at.row_tile * kTcRows + r, node = row / a.group;
       const bool here = row < a.rows && node < live, any_here = __any_sync(0xffffffffu, here);
-      float factor = a.scale_log2;
+      // A negative scale is Q's sign, so that the largest product is the largest score.
+      const unsigned flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
+      float factor = fabsf(a.scale_log2);
       {
-        // The row into its lines, and zeros into its lanes of O.
-        const long long base = b * a.q_batch + node * a.q_node +
-                               (static_cast<long long>(at.head) * a.group + (row - node * a.group)) * a.q_head;
-        float down = 1.0f;
+        // The rows into their lines: units of 8 values, so that a warp reads whole rows; then zeros
+        // into the thread's lanes of O.
+        constexpr int kUnits = Dim / 8;
+        auto line_of = [&](int q_row, int unit) {
+          return reinterpret_cast<uint4*>(q_lines + (unit >> 3) * (kTcRows * 128) + q_row * 128 +
+                                          (((unit & 7) ^ (q_row & 7)) << 4));
+        };
+#pragma unroll 1
+        for (int u0 = 0; u0 < kUnits; u0 += 8) {
+          uint4 x[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            const int k = (u0 + u) * kTcRows + r, of = k / kUnits, unit = k % kUnits;
+            const int q_row = at.row_tile * kTcRows + of, q_node = q_row / a.group;
+            x[u] = make_uint4(0, 0, 0, 0);
+            if (q_row < a.rows && q_node < live && 8 * unit < dim) {
+              const unsigned short* const from =
+                  static_cast<const unsigned short*>(a.q) + b * a.q_batch + q_node * a.q_node +
+                  (static_cast<long long>(at.head) * a.group + (q_row - q_node * a.group)) * a.q_head + 8 * unit;
+              if (a.q_units) {
+                x[u] = *reinterpret_cast<const uint4*>(from);
+              } else {
+                uint32_t h[4];
+                for (int e = 0; e < 4; ++e) h[e] = from[2 * e] | static_cast<uint32_t>(from[2 * e + 1]) << 16;
+                x[u] = make_uint4(h[0], h[1], h[2], h[3]);
+              }
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            const int k = (u0 + u) * kTcRows + r;
+            x[u].x ^= flip, x[u].y ^= flip, x[u].z ^= flip, x[u].w ^= flip;
+            *line_of(k / kUnits, k % kUnits) = x[u];
+          }
+        }
         if constexpr (kQuantised) {
+          // Each thread its own row, in place: to F16 and scaled.
+          asm volatile("bar.sync 1, 128;" ::: "memory");
+          auto value = [&](uint32_t x, int e) {
+            const unsigned short h = static_cast<unsigned short>(e ? x >> 16 : x);
+            return a.q_bf16 ? __uint_as_float(static_cast<uint32_t>(h) << 16) : __half2float(__ushort_as_half(h));
+          };
           float most = 0.0f;
-          for (int d = 0; d < dim; ++d) {
-            const float v = here ? fabsf(load_q(a, base + d)) : 0.0f;
-            if (v < INFINITY) most = fmaxf(most, v);
+#pragma unroll 4
+          for (int unit = 0; unit < kUnits; ++unit) {
+            const uint4 x = *line_of(r, unit);
+            const uint32_t h[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float v = fabsf(value(h[e >> 1], e & 1));
+              if (v < INFINITY) most = fmaxf(most, v);
+            }
           }
           int e = static_cast<int>(__float_as_uint(most) >> 23);  // biased exponent
           e = most == 0.0f ? 127 : max(e, 16);
-          down = __uint_as_float(static_cast<unsigned>(min(127 + 14 + 127 - e, 253)) << 23);
+          const float down = __uint_as_float(static_cast<unsigned>(min(127 + 14 + 127 - e, 253)) << 23);
           factor /= down;
-        }
-#pragma unroll 2
-        for (int unit = 0; unit < Dim / 8; ++unit) {
-          uint32_t h[4];
+#pragma unroll 4
+          for (int unit = 0; unit < kUnits; ++unit) {
+            const uint4 x = *line_of(r, unit);
+            const uint32_t h[4] = {x.x, x.y, x.z, x.w};
+            uint32_t y[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int d = 8 * unit + 2 * e;
-            float x = 0.0f, y = 0.0f;
-            if (here && d < dim) {
-              x = load_q(a, base + d) * down;
-              y = load_q(a, base + d + 1) * down;
-            }
-            h[e] = pack2<kBf16>(x, y);
+            for (int e2 = 0; e2 < 4; ++e2) y[e2] = pack2<false>(value(h[e2], 0) * down, value(h[e2], 1) * down);
+            *line_of(r, unit) = make_uint4(y[0], y[1], y[2], y[3]);
           }
-          *reinterpret_cast<uint4*>(q_lines + (unit >> 3) * (kTcRows * 128) + r * 128 + (((unit & 7) ^ (r & 7)) << 4)) =
-              make_uint4(h[0], h[1], h[2], h[3]);
         }
         uint32_t zero[32];
 #pragma unroll
@@ -525,7 +693,8 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
         fence_async();
         barrier_arrive(&bar->q_full);
       }
-      float m = -INFINITY, less = -1e30f, l = 0.0f, mz = -INFINITY, lz = 0.0f;
+      float m = -INFINITY, less = -1e30f, mz = -INFINITY, lz = 0.0f;
+      float2 l2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
       for (int i = 0; i < n && good; ++i) {
         const int t = tiles_done + i;
         good = barrier_wait(&bar->slot_full[t % kTcSlots], (t / kTcSlots) & 1, failed) &&
@@ -536,66 +705,71 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
           const TcSlot& slot = slots[t % kTcSlots];
           const int pos0 = (at.tile + i) * kTile;
           const unsigned s_at = tmem + (t & 1) * 64 + lanes;
+          const uint2 there4 = *reinterpret_cast<const uint2*>(slot.there);
+          const unsigned there_lo = there4.x, there_hi = there4.y;
+          const bool partly = (there_lo & there_hi) != 0xffffffffu || pos0 + kTile > context;
+          const uint2 zero4 = *reinterpret_cast<const uint2*>(slot.zero);
+          const bool rare = partly || (kQuantised && (zero4.x | zero4.y) != 0);
+          float now_factor = factor;
+          const float *ks = slot.ks, *lv = slot.lv;
+          unsigned see_lo = there_lo, see_hi = there_hi;
+          if (rare) {
+            // Scores with what is not seen at -infinity, back to tensor memory for the common path;
+            // V rows with a scale of 0 into their own sum.
+            if (partly) {
+              for (int j = max(0, context - pos0); j < kTile && pos0 + j < length; ++j) {
+                const int drafted = pos0 + j - context;
+                if (!(here && drafted < live && node_sees(a, b, node, drafted))) {
+                  if (j < 32) see_lo &= ~(1u << j);
+                  else see_hi &= ~(1u << (j - 32));
+                }
+              }
+            }
+#pragma unroll 1
+            for (int half = 0; half < 2; ++half) {
+              uint32_t s[32];
+              tc_load(s, s_at + 32 * half);
+              tc_loaded();
+              const unsigned see = half ? see_hi : see_lo, zero = kQuantised ? (half ? zero4.y : zero4.x) : 0u;
+              float high = -INFINITY;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                float x = __uint_as_float(s[j]) * factor;
+                if constexpr (kQuantised) {
+                  x *= slot.ks[32 * half + j];
+                  if ((zero & see) >> j & 1) high = fmaxf(high, x);
+                  else x += slot.lv[32 * half + j];
+                }
+                s[j] = __float_as_uint((see >> j) & 1 ? x : -INFINITY);
+              }
+              if (kQuantised && zero != 0) {
+                const float to = fmaxf(mz, high), base = to == -INFINITY ? 0.0f : to;
+                lz *= exp2_fast(mz - base);
+                mz = to;
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                  if ((zero >> j) & 1) {
+                    lz += exp2_fast(__uint_as_float(s[j]) - base);
+                    s[j] = __float_as_uint(-INFINITY);
+                  }
+              }
+              tc_store(s_at + 32 * half, s);
+            }
+            tc_stored();
+            now_factor = 1.0f;
+            ks = ones;
+            lv = zeros;
+          }
           uint32_t s0[32], s1[32];
           tc_load(s0, s_at);
           tc_load(s1, s_at + 32);
           tc_loaded();
-          auto s = [&](int j) -> uint32_t& { return j < 32 ? s0[j] : s1[j - 32]; };
-          const unsigned there_lo = slot.there[0] | slot.there[1] << 16, there_hi = slot.there[2] | slot.there[3] << 16;
-          const bool partly = (there_lo & there_hi) != 0xffffffffu || pos0 + kTile > context;
-          unsigned see_lo = there_lo, see_hi = there_hi;
-          if (partly) {
-            for (int j = max(0, context - pos0); j < kTile && pos0 + j < length; ++j) {
-              const bool sees = here && node_sees(a, b, node, pos0 + j - context) && pos0 + j - context < live;
-              if (!sees) {
-                if (j < 32) see_lo &= ~(1u << j);
-                else see_hi &= ~(1u << (j - 32));
-              }
-            }
-          }
           if constexpr (kQuantised) {
-            const unsigned zero_lo = slot.zero[0] | slot.zero[1] << 16, zero_hi = slot.zero[2] | slot.zero[3] << 16;
-            if (zero_lo | zero_hi) {
-              float high = -INFINITY;
-#pragma unroll
-              for (int j = 0; j < kTile; ++j)
-                if (((j < 32 ? zero_lo & see_lo : zero_hi & see_hi) >> (j & 31)) & 1)
-                  high = fmaxf(high, __uint_as_float(s(j)) * slot.ks[j] * factor);
-              const float to = fmaxf(mz, high), base = to == -INFINITY ? 0.0f : to;
-              lz *= exp2_fast(mz - base);
-              mz = to;
-#pragma unroll
-              for (int j = 0; j < kTile; ++j)
-                if (((j < 32 ? zero_lo & see_lo : zero_hi & see_hi) >> (j & 31)) & 1)
-                  lz += exp2_fast(__uint_as_float(s(j)) * slot.ks[j] * factor - base);
-            }
-#pragma unroll
-            for (int j = 0; j < kTile; j += 4) {
-              const float4 ks = *reinterpret_cast<const float4*>(&slot.ks[j]);
-              const float4 lv = *reinterpret_cast<const float4*>(&slot.lv[j]);
-              s(j) = __float_as_uint(fmaf(__uint_as_float(s(j)), ks.x * factor, lv.x));
-              s(j + 1) = __float_as_uint(fmaf(__uint_as_float(s(j + 1)), ks.y * factor, lv.y));
-              s(j + 2) = __float_as_uint(fmaf(__uint_as_float(s(j + 2)), ks.z * factor, lv.z));
-              s(j + 3) = __float_as_uint(fmaf(__uint_as_float(s(j + 3)), ks.w * factor, lv.w));
-            }
-            // A scale of 0 leaves -infinity, unless the product was a NaN or an infinity.
-            if (zero_lo | zero_hi) {
-#pragma unroll
-              for (int j = 0; j < kTile; ++j)
-                if (((j < 32 ? zero_lo : zero_hi) >> (j & 31)) & 1) s(j) = __float_as_uint(-INFINITY);
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < kTile; ++j) s(j) = __float_as_uint(__uint_as_float(s(j)) * factor);
+            scale_scores(s0, ks, lv, now_factor);
+            scale_scores(s1, ks + 32, lv + 32, now_factor);
           }
-          if (partly) {
-#pragma unroll
-            for (int j = 0; j < kTile; ++j)
-              if (!(((j < 32 ? see_lo : see_hi) >> (j & 31)) & 1)) s(j) = __float_as_uint(-INFINITY);
-          }
-          float top = -INFINITY;
-#pragma unroll
-          for (int j = 0; j < kTile; ++j) top = fmaxf(top, __uint_as_float(s(j)));
+          float top = fmaxf(highest(s0), highest(s1));
+          if constexpr (!kQuantised) top *= now_factor;  // factors are not negative
           const bool rises = here && top > less + (kSlack + kLift);
           if (__any_sync(0xffffffffu, rises)) {
             float shrink = 1.0f;
@@ -603,84 +777,70 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
               shrink = exp2_fast(m - top);
               m = top;
               less = top - kLift;
-              l *= shrink;
+              l2[0].x *= shrink, l2[0].y *= shrink, l2[1].x *= shrink, l2[1].y *= shrink;
             }
             if (i > 0) {
               good = barrier_wait(&bar->o_done[(t - 1) & 1], ((t - 1) >> 1) & 1, failed);
               tc_after();
-              uint32_t o[32];
 #pragma unroll 1
-              for (int d = 0; d < Dim; d += 32) {
-                tc_load(o, tmem_o + lanes + d);
+              for (int d = 0; d < Dim; d += 16) {
+                uint32_t o[16];
+                tc_load16(o, tmem_o + lanes + d);
                 tc_loaded();
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink);
-                tc_store(tmem_o + lanes + d, o);
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink);
+                tc_store16(tmem_o + lanes + d, o);
               }
               tc_stored();
             }
-          }
-#pragma unroll
-          for (int j = 0; j < kTile; j += 4) {
-            float w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = exp2_fast(__uint_as_float(s(j + e)) - less);
-            if constexpr (kQuantised) {
-              const float4 rv = *reinterpret_cast<const float4*>(&slot.rv[j]);
-              l = fmaf(w[0], rv.x, fmaf(w[1], rv.y, fmaf(w[2], rv.z, fmaf(w[3], rv.w, l))));
-            } else {
-              l += (w[0] + w[1]) + (w[2] + w[3]);
-            }
-            s(j) = __float_as_uint(w[0]);
-            s(j + 1) = __float_as_uint(w[1]);
-            s(j + 2) = __float_as_uint(w[2]);
-            s(j + 3) = __float_as_uint(w[3]);
           }
           if (Kind != T4A_I8 && partly) {
             // What was cleaned out of V reaches the rows that see it.
             good = good && barrier_wait(&bar->v_full[t % kTcStages], (t / kTcStages) & 1, failed);
-            const unsigned odd_lo = slot.odd[0] | slot.odd[1] << 16, odd_hi = slot.odd[2] | slot.odd[3] << 16;
-            if (good && (odd_lo | odd_hi)) {
+            const volatile unsigned* const odd = slot.odd;
+            const uint2 odd4 = make_uint2(odd[0], odd[1]);
+            if (good && (odd4.x | odd4.y)) {
               if (i > 0) good = barrier_wait(&bar->o_done[(t - 1) & 1], ((t - 1) >> 1) & 1, failed);
               tc_after();
 #pragma unroll 1
-              for (int d = 0; d < Dim; d += 32) {
-                uint32_t o[32];
-                tc_load(o, tmem_o + lanes + d);
+              for (int j = 0; j < kTile; ++j) {
+                if (!(((j < 32 ? odd4.x : odd4.y) >> (j & 31)) & 1)) continue;
+                uint32_t score;
+                tc_load1(&score, s_at + j);
                 tc_loaded();
+                const bool sees = here && (((j < 32 ? see_lo : see_hi) >> (j & 31)) & 1);
+                const float w = exp2_fast(__uint_as_float(score) - less);
+                const int at_pos = pos0 + j, page = a.table[b * a.table_batch + (at_pos / a.cache.page_size) * a.table_page];
+                const unsigned char* const v_row = a.cache.v.base + at.head * a.cache.v.head + page * a.cache.v.page +
+                                                   (at_pos % a.cache.page_size) * a.cache.v.place;
 #pragma unroll 1
-                for (int j = 0; j < kTile; ++j) {
-                  if (!(((j < 32 ? odd_lo : odd_hi) >> (j & 31)) & 1)) continue;
-                  if (!(((j < 32 ? see_lo : see_hi) >> (j & 31)) & 1) || !here) continue;
-                  float w = 0.0f;
+                for (int d = 0; d < dim; d += 16) {
+                  uint32_t o[16];
+                  tc_load16(o, tmem_o + lanes + d);
+                  tc_loaded();
 #pragma unroll
-                  for (int e = 0; e < kTile; ++e) w = e == j ? __uint_as_float(s(e)) : w;
-                  const int at_pos = pos0 + j, page = a.table[b * a.table_batch + (at_pos / a.cache.page_size) * a.table_page];
-                  const unsigned char* const v_row = a.cache.v.base + at.head * a.cache.v.head + page * a.cache.v.page +
-                                                     (at_pos % a.cache.page_size) * a.cache.v.place;
-#pragma unroll
-                  for (int e = 0; e < 32; ++e) {
-                    if (d + e >= dim) continue;
+                  for (int e = 0; e < 16; ++e) {
                     const float v = row_value<Kind>(v_row, d + e);
-                    if (!(fabsf(v) < INFINITY)) o[e] = __float_as_uint(__uint_as_float(o[e]) + w * v);
+                    if (sees && !(fabsf(v) < INFINITY)) o[e] = __float_as_uint(__uint_as_float(o[e]) + w * v);
                   }
+                  __syncwarp();
+                  tc_store16(tmem_o + lanes + d, o);
                 }
-                __syncwarp();
-                tc_store(tmem_o + lanes + d, o);
+                tc_stored();
               }
-              tc_stored();
             }
           }
           uint32_t p[32];
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            p[j] = pack2<kBf16>(__uint_as_float(s(2 * j)), __uint_as_float(s(2 * j + 1)));
+          const float first_factor = kQuantised ? 1.0f : now_factor;
+          weights<kQuantised, kBf16>(s0, p, first_factor, less, slot.rv, l2);
+          weights<kQuantised, kBf16>(s1, p + 16, first_factor, less, slot.rv + 32, l2);
           tc_store(s_at, p);
           tc_stored();
           tc_before();
         }
         barrier_arrive(&bar->p_full[t & 1]);
       }
+      const float l = (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
       tiles_done += n;
       if (good) good = barrier_wait(&bar->o_done[(tiles_done - 1) & 1], ((tiles_done - 1) >> 1) & 1, failed);
       tc_after();

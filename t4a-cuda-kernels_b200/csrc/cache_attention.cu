@@ -22,7 +22,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_join(const AttendArgs a) {
   const int row_tile = row / a.tile_rows, r = row - row_tile * a.tile_rows;
   const int tiles = sequence_tiles(a, b);
   const Line line = read_line(a, b);
-  const int quota = quota_of(a, line.total), start = line.before + (head * a.row_tiles + row_tile) * tiles;
+  const int quota = quota_of(a, line.total), start = line.before + head * tiles;
   const int c0 = start / quota, c1 = tiles == 0 ? c0 : (start + tiles - 1) / quota;
   const long long to = out_row(a, b, head, row);
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -32,7 +32,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_join(const AttendArgs a) {
     return;
   }
   if (c0 == c1) return;
-  auto part = [&](int c) { return (static_cast<long long>(c) * 2 + (c == c0 ? 1 : 0)) * a.tile_rows + r; };
+  auto part = [&](int c) { return ((static_cast<long long>(c) * a.row_tiles + row_tile) * 2 + (c == c0 ? 1 : 0)) * a.tile_rows + r; };
   float most = -INFINITY;
   for (int c = c0 + threadIdx.x; c <= c1; c += kJoinThreads) most = fmaxf(most, a.part_lse[part(c)]);
 #pragma unroll
@@ -147,16 +147,21 @@ int plan_attention(int dtype, const t4a_kv_cache* cache, const t4a_cuda_layout* 
   a->row_tiles = (a->rows + choice->rows - 1) / choice->rows;
   // The line of tiles is counted in 32 bits.
   long long tiles = (places + kTile - 1) / kTile;
-  for (long long by : {batch, static_cast<long long>(a->cache.heads), static_cast<long long>(a->row_tiles)})
+  for (long long by : {batch, static_cast<long long>(a->cache.heads)})
     if (plan::mul_overflows(tiles, by, &tiles)) return T4A_ERR_OVERFLOW;
   if (tiles > INT_MAX || batch * a->cache.heads * a->rows > INT_MAX) return T4A_ERR_DOMAIN_TOO_LARGE;
-  T4A_TRY(dispatch(cache->kind, *a, *choice, nullptr, &a->blocks));
+  int blocks;
+  T4A_TRY(dispatch(cache->kind, *a, *choice, nullptr, &blocks));
+  a->groups = a->row_tiles < blocks ? blocks / a->row_tiles : 1;
   return T4A_OK;
 }
 
-size_t workspace_of(const AttendArgs& a) {
-  return static_cast<size_t>(a.blocks) * 2 * a.tile_rows * (a.cache.dim + 1) * sizeof(float);
+// Parts, where there is more than one group to share a unit.
+size_t part_rows(const AttendArgs& a) {
+  return a.groups > 1 ? static_cast<size_t>(a.groups) * a.row_tiles * 2 * a.tile_rows : 4;
 }
+
+size_t workspace_of(const AttendArgs& a) { return part_rows(a) * (a.cache.dim + 1) * sizeof(float); }
 
 }  // namespace
 }  // namespace cache
@@ -230,6 +235,7 @@ extern "C" int t4a_tree_attention(void* stream, int dtype, const t4a_kv_cache* c
   a.out_head = out_layout->strides[1];
   a.out_node = out_layout->strides[2];
   a.out_batch = out_layout->strides[3];
+  a.q_units = rows_aligned(q, *q_layout, 2, 16);
   a.pairs = rows_aligned(q, *q_layout, 2, 4) && rows_aligned(out, *out_layout, 2, 4);
   const Pages &k = a.cache.k, &v = a.cache.v;
   const long long last = (a.cache.pages - 1) * k.page + (a.cache.page_size - 1ll) * k.place + a.cache.dim * 2;
@@ -242,7 +248,7 @@ extern "C" int t4a_tree_attention(void* stream, int dtype, const t4a_kv_cache* c
   a.live_nodes = nodes;
   a.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
   a.part_out = static_cast<float*>(workspace);
-  a.part_lse = a.part_out + static_cast<size_t>(a.blocks) * 2 * a.tile_rows * a.cache.dim;
+  a.part_lse = a.part_out + part_rows(a) * a.cache.dim;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   T4A_TRY(dispatch(cache->kind, a, choice, s, nullptr));
 

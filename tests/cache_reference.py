@@ -31,21 +31,23 @@ def attention(q, k, v, k_scale, v_scale, table, context, sees, live, scale):
         at = table[b, place // page].long() * page + place % page
         there = (at >= 0) & (at < pages * page)
         at = at.clamp(0, max(0, pages * page - 1))
-        for i in range(n):
-            seen = there.clone()
-            seen[c:] &= sees[b, i, :length - c].bool()
-            rows = at[seen]
-            if rows.numel() == 0:
-                continue
-            for h in range(kv):
-                qq = q[b, i, h * group:(h + 1) * group].double()
-                kk, vv = kr[rows, h], vr[rows, h]
-                s = qq @ kk.T * scale
-                w = torch.softmax(s, dim=1)
-                o = slice(h * group, (h + 1) * group)
-                out[b, i, o], lse[b, i, o] = w @ vv, torch.logsumexp(s, dim=1)
-                spread[b, i, o] = w @ vv.abs()
-                size[b, i, o] = (qq.abs() @ kk.abs().T).amax(dim=1) * abs(scale)
+        if n == 0 or length == 0:
+            continue
+        seen = there.expand(n, length).clone()
+        seen[:, c:] &= sees[b, :n, :length - c].bool()
+        some = seen.any(dim=1)
+        for h in range(kv):
+            o = slice(h * group, (h + 1) * group)
+            qq, kk, vv = q[b, :n, o].double(), kr[at, h], vr[at, h]
+            # Rows that nobody sees may hold anything.
+            kk, vv = (torch.where(seen.any(dim=0)[:, None], x, 0.0) for x in (kk, vv))
+            s = torch.where(seen[:, None, :], torch.einsum("ngd,ld->ngl", qq, kk) * scale, -math.inf)
+            w = torch.where(some[:, None, None], torch.softmax(s, dim=2), 0.0)
+            out[b, :n, o] = torch.einsum("ngl,ld->ngd", w, vv)
+            lse[b, :n, o] = torch.logsumexp(s, dim=2)
+            spread[b, :n, o] = torch.einsum("ngl,ld->ngd", w, vv.abs())
+            size[b, :n, o] = torch.where(seen[:, None, :], torch.einsum("ngd,ld->ngl", qq.abs(), kk.abs()),
+                                         0.0).amax(dim=2) * abs(scale)
     return out, lse, spread, size
 
 

@@ -188,6 +188,22 @@ def test_attention(cuda, kind, dtype, batch, nodes, kv, group, dim, page, contex
 
 
 @pytest.mark.parametrize("kind,dtype", KINDS)
+@pytest.mark.parametrize("batch,nodes,kv,group,dim,page,contexts", [
+    (48, 1, 8, 4, 128, 16, [700, 3, 1100, 64]),
+    (40, 3, 8, 4, 64, 64, [500, 900, 20]),
+    (37, 5, 6, 5, 96, 24, [800, 100, 1203]),
+    (33, 9, 8, 5, 128, 16, [600, 1200, 3, 128]),
+    (30, 40, 4, 4, 96, 24, [900, 77, 2000]),
+    (24, 64, 5, 8, 64, 32, [1500, 100]),
+    (24, 7, 6, 6, 256, 16, [700, 1000]),
+])
+def test_blocks_that_take_several_tiles_and_units(cuda, kind, dtype, batch, nodes, kv, group, dim, page, contexts):
+    c = attention_case(batch, batch, nodes, kv, group, dim, page, contexts, kind, dtype)
+    poison_unused(c)
+    check_attention(c)
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
 def test_attention_without_a_mask_is_a_chain(cuda, kind, dtype):
     check_attention(attention_case(3, 2, 6, 2, 4, 128, 16, [50, 300], kind, dtype, tree=False), mask=None)
 
