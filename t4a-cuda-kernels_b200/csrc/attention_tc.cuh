@@ -36,21 +36,17 @@ constexpr int kTcThreads = 384;
 // Registers of a thread of each role: 80 at launch, moved between the roles.
 constexpr int kTcSoftmaxRegisters = 136, kTcLoaderRegisters = 72, kTcIssueRegisters = 32;
 static_assert(kTcSoftmaxRegisters + kTcLoaderRegisters + kTcIssueRegisters == 3 * 80, "a larger sum would wait for good");
-constexpr int kTcLoaders = 128;
+constexpr int kTcLoaders = 64;  // threads, of K's rows and of V's
 constexpr int kTcStages = 2;
 constexpr int kTcSlots = 4;  // of tiles' scales and flags: they outlive a stage by two tiles
 constexpr unsigned kTcColumns = 256;
-constexpr unsigned kTcWaitNs = 2000;
 
 // What a tile's rows carry beside their values.
 struct alignas(16) TcSlot {
   float ks[kTile];  // K's scale
   float lv[kTile];  // log2 of V's scale, -infinity for a scale of 0
   float rv[kTile];  // 1 / V's scale
-  // A bit a token; a loader warp writes the half word of its 16.
-  __align__(8) unsigned short there[4];
-  __align__(8) unsigned short zero[4];
-  __align__(8) unsigned odd[2];
+  unsigned there[2], zero[2], odd[2];  // a bit a token
 };
 
 static_assert(sizeof(TcSlot) % 16 == 0, "slots are read 16 bytes at a time");
@@ -91,9 +87,9 @@ __device__ __forceinline__ bool barrier_wait(unsigned long long* b, unsigned par
   for (unsigned i = 0; i < T4A_STAGE_WAIT_LIMIT; ++i) {
     unsigned ok;
     asm volatile(
-        "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }"
+        "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
         : "=r"(ok)
-        : "r"(at), "r"(parity), "n"(kTcWaitNs)
+        : "r"(at), "r"(parity)
         : "memory");
     if (ok) return true;
     if (*failed) return false;
@@ -304,7 +300,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
       barrier_init(&bar->p_full[i], kTcRows);
       barrier_init(&bar->o_done[i], 1);
     }
-    for (int i = 0; i < kTcSlots; ++i) barrier_init(&bar->slot_full[i], 4);
+    for (int i = 0; i < kTcSlots; ++i) barrier_init(&bar->slot_full[i], 2);
     *failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -329,22 +325,31 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
 
   if (warp >= 4 && warp < 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTcLoaderRegisters));
-    // ---- cache rows: warp w takes tokens 16 w .. 16 w + 15 of a tile ----
-    const int w = warp - 4;
-    constexpr int kChunks = Dim * KindOf<Kind>::bytes / 16;  // of a padded row
-    constexpr int kRounds = 16 * kChunks / 32;
+    // ---- cache rows: warps 4 and 5 K's, 6 and 7 V's, 32 of a tile's tokens each ----
+    const bool is_v = warp >= 6;
+    const int w = warp & 1;
+    constexpr int kChunks = Dim * KindOf<Kind>::bytes / 16;  // of a padded row; as many rounds of 32 lanes
     const int used = dim * KindOf<Kind>::bytes / 16;
+    const Pages& mine = is_v ? a.cache.v : a.cache.k;
+    unsigned long long* const full = is_v ? bar->v_full : bar->k_full;
+    unsigned long long* const empty = is_v ? bar->v_empty : bar->k_empty;
+    auto lines = [&](int stage) { return is_v ? v_lines(stage) : k_lines(stage); };
+    // The row and chunk of a lane in round u.
+    auto token_of = [&](int u) { return (u * 32 + lane) / kChunks; };
+    auto chunk_of = [&](int u) { return (u * 32 + lane) % kChunks; };
+    // Swizzled place of a 16-byte unit of 8 values of row t.
+    auto unit_at = [&](int t, int unit) {
+      return (unit >> 3) * (kTile * 128) + t * 128 + (((unit & 7) ^ (t & 7)) << 4);
+    };
     bool good = true;
     while (at.left > 0 && good) {
       const int b = at.b;
       int context, live, length;
       sequence_tokens(a, b, &context, &live, &length);
       const int n = min(at.left, at.tiles - at.tile);
-      const Pages& side = lane < 16 ? a.cache.k : a.cache.v;
-      const unsigned char* const k_base = a.cache.k.base + at.head * a.cache.k.head;
-      const unsigned char* const v_base = a.cache.v.base + at.head * a.cache.v.head;
+      const unsigned char* const base = mine.base + at.head * mine.head;
       const int* const my_table = a.table + b * a.table_batch;
-      int pos = at.tile * kTile + 16 * w + (lane & 15);
+      int pos = at.tile * kTile + 32 * w + lane;  // the lane's token of the next tile to look up
       int in_table = pos / a.cache.page_size, place = pos - in_table * a.cache.page_size;
       const int end = min(length, (at.tile + n) * kTile);
       int page_ahead, place_ahead;
@@ -360,199 +365,145 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
           ++in_table;
         }
       };
-      // The row and chunk of a lane in round u.
-      auto token_of = [&](int u) { return (u * 32 + lane) / kChunks; };
-      auto chunk_of = [&](int u) { return (u * 32 + lane) % kChunks; };
-      // Swizzled place of a 16-byte unit of 8 values of row t.
-      auto unit_at = [&](int t, int unit) {
-        return (unit >> 3) * (kTile * 128) + t * 128 + (((unit & 7) ^ (t & 7)) << 4);
-      };
-      unsigned bits = 0;
-      long long off = 0;
-      float scale = 0.0f;
-      auto step = [&] {  // the next tile's rows: where they are, and their scales
+      unsigned bits = 0;  // of the warp's tokens, which are there
+      long long off = 0;  // of the lane's token
+      float ks = 0.0f, vs = 0.0f;
+      auto step = [&] {  // to the next tile
         const int page = page_ahead, at_place = place_ahead;
         look_up();
         const bool there = static_cast<unsigned>(page) < static_cast<unsigned>(a.cache.pages);
-        bits = __ballot_sync(0xffffffffu, there) & 0xffffu;
-        off = there ? page * side.page + at_place * side.place : 0;
-        if constexpr (kQuantised)
-          scale = there ? side.scale[page * side.scale_page + at_place * side.scale_place + at.head * side.scale_head]
-                        : 1.0f;
+        bits = __ballot_sync(0xffffffffu, there);
+        off = there ? page * mine.page + at_place * mine.place : 0;
+        if (kQuantised && !is_v) {
+          ks = vs = 1.0f;
+          if (there) {
+            const Pages &k = a.cache.k, &v = a.cache.v;
+            ks = k.scale[page * k.scale_page + at_place * k.scale_place + at.head * k.scale_head];
+            vs = v.scale[page * v.scale_page + at_place * v.scale_place + at.head * v.scale_head];
+          }
+        }
       };
-      uint4 code[kQuantised ? 2 : 1][kQuantised ? kRounds : 1];  // K's and V's
-      auto fetch = [&](int s) {
+      uint4 code[kQuantised ? kChunks : 1];
+      auto fetch = [&] {
         if constexpr (kQuantised) {
 #pragma unroll
-          for (int u = 0; u < kRounds; ++u) {
+          for (int u = 0; u < kChunks; ++u) {
             const int t = token_of(u), chunk = chunk_of(u);
-            const long long from = __shfl_sync(0xffffffffu, off, s * 16 + t);
-            code[s][u] = make_uint4(0, 0, 0, 0);
-            if (((bits >> t) & 1) && chunk < used)
-              code[s][u] = *reinterpret_cast<const uint4*>((s ? v_base : k_base) + from + chunk * 16);
+            const long long from = __shfl_sync(0xffffffffu, off, t);
+            code[u] = make_uint4(0, 0, 0, 0);
+            if (((bits >> t) & 1) && chunk < used) code[u] = *reinterpret_cast<const uint4*>(base + from + chunk * 16);
           }
         }
       };
-      // A tile's slot: what the tokens are.  E4M3 NaNs of V are noted where some node may not see them.
-      auto describe = [&](int t, unsigned the_bits, float the_scale) {
+      // K's warps say what the tile's tokens are.
+      auto describe = [&](int t) {
         TcSlot& slot = slots[t % kTcSlots];
-        if (lane == 0) {
-          slot.there[w] = static_cast<unsigned short>(the_bits);
-          reinterpret_cast<unsigned short*>(slot.odd)[w] = 0;
-        }
+        if (lane == 0) slot.there[w] = bits;
         if constexpr (kQuantised) {
-          const bool zero = the_scale < kLeastScale;
-          const unsigned zeros = __ballot_sync(0xffffffffu, zero) >> 16;
-          if (lane == 0) slot.zero[w] = static_cast<unsigned short>(zeros);
-          if (lane < 16) {
-            slot.ks[16 * w + lane] = the_scale;
-          } else {
-            const float lv = zero ? -INFINITY : __log2f(the_scale);
-            slot.lv[16 * w + lane - 16] = lv;
-            // A NaN has made the score a NaN where the row is seen, and must not touch l elsewhere.
-            slot.rv[16 * w + lane - 16] = zero ? 0.0f : the_scale == the_scale ? exp2_fast(-lv) : 1.0f;
-          }
+          const bool zero = vs < kLeastScale;
+          const unsigned zeros_of = __ballot_sync(0xffffffffu, zero);
+          if (lane == 0) slot.zero[w] = zeros_of;
+          const float lv = zero ? -INFINITY : __log2f(vs);
+          slot.ks[32 * w + lane] = ks;
+          slot.lv[32 * w + lane] = lv;
+          // A NaN has made the score a NaN where the row is seen, and must not touch l elsewhere.
+          slot.rv[32 * w + lane] = zero ? 0.0f : vs == vs ? exp2_fast(-lv) : 1.0f;
         }
         __syncwarp();
         if (lane == 0) barrier_arrive(&bar->slot_full[t % kTcSlots]);
       };
-      // Codes to F16 lines.
-      auto unpack = [&](int s, unsigned char* lines, int t_block, bool partly) {
+      look_up();
+      step();
+      if constexpr (kQuantised) fetch();
+      for (int i = 0; i < n; ++i) {
+        const int t = tiles_done + i, stage = t % kTcStages;
+        const bool partly = (at.tile + i + 1) * kTile > context;
+        good = barrier_wait(&empty[stage], ((t / kTcStages) & 1) ^ 1, failed);
+        if (!good) break;
+        unsigned char* const to = lines(stage);
+        if (!is_v) describe(t);
+        unsigned odd = 0;  // tokens with an infinity or a NaN in V, where some node may not see them
         if constexpr (kQuantised) {
+          // Codes to F16 lines.
 #pragma unroll
-          for (int u = 0; u < kRounds; ++u) {
-            const int t = token_of(u), chunk = chunk_of(u);
-            uint32_t x[4] = {code[s][u].x, code[s][u].y, code[s][u].z, code[s][u].w}, h[8];
-            if (Kind == T4A_E4M3 && s == 1 && partly) {
-              bool odd = false;
+          for (int u = 0; u < kChunks; ++u) {
+            const int in = token_of(u), chunk = chunk_of(u), row = 32 * w + in;
+            uint32_t x[4] = {code[u].x, code[u].y, code[u].z, code[u].w}, h[8];
+            if (Kind == T4A_E4M3 && is_v && partly) {
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const uint32_t nan = __vcmpeq4(x[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-                odd = odd || nan != 0;
+                if (nan != 0) odd |= 1u << in;
                 x[e] &= ~nan;
               }
-              if (odd) atomicOr(&slots[t_block % kTcSlots].odd[w >> 1], 1u << (16 * (w & 1) + t));
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) neighbours<Kind>(x[e], &h[2 * e], &h[2 * e + 1]);
             // Half of the lanes store their second unit first: 8 lanes then meet 8 units.
             const bool swap = (chunk >> 2) & 1;
             const uint4 lo = make_uint4(h[0], h[1], h[2], h[3]), hi = make_uint4(h[4], h[5], h[6], h[7]);
-            const int t64 = 16 * w + t;
             if (chunk < used) {
-              *reinterpret_cast<uint4*>(lines + unit_at(t64, 2 * chunk + (swap ? 1 : 0))) = swap ? hi : lo;
-              *reinterpret_cast<uint4*>(lines + unit_at(t64, 2 * chunk + (swap ? 0 : 1))) = swap ? lo : hi;
+              *reinterpret_cast<uint4*>(to + unit_at(row, 2 * chunk + (swap ? 1 : 0))) = swap ? hi : lo;
+              *reinterpret_cast<uint4*>(to + unit_at(row, 2 * chunk + (swap ? 0 : 1))) = swap ? lo : hi;
             }
           }
-        }
-      };
-      // 16-bit rows straight to their lines.
-      auto copy = [&](int s, unsigned char* lines, long long the_off, unsigned the_bits) {
-        if constexpr (!kQuantised) {
-          const unsigned to = shared_at(lines);
-          if (a.plain_copies && the_bits == 0xffffu) {
-            const unsigned units = static_cast<unsigned>(the_off >> 4);
-            const unsigned char* const base = s ? v_base : k_base;
+        } else {
+          // 16-bit rows straight to their lines.
+          const unsigned to_shared = shared_at(to);
+          if (a.plain_copies && bits == 0xffffffffu) {
+            const unsigned units = static_cast<unsigned>(off >> 4);
 #pragma unroll
-            for (int u = 0; u < kRounds; ++u) {
-              const int t = token_of(u), chunk = chunk_of(u);
-              const unsigned from = __shfl_sync(0xffffffffu, units, t) + chunk;
-              copy16(to + unit_at(16 * w + t, chunk), base + static_cast<unsigned long long>(from) * 16);
+            for (int u = 0; u < kChunks; ++u) {
+              const int in = token_of(u), chunk = chunk_of(u);
+              const unsigned from = __shfl_sync(0xffffffffu, units, in) + chunk;
+              copy16(to_shared + unit_at(32 * w + in, chunk), base + static_cast<unsigned long long>(from) * 16);
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            return;
+          } else {
+#pragma unroll 4
+            for (int u = 0; u < kChunks; ++u) {
+              const int in = token_of(u), chunk = chunk_of(u);
+              const long long from = __shfl_sync(0xffffffffu, off, in);
+              if (chunk < used)
+                copy16(to_shared + unit_at(32 * w + in, chunk), base + from + chunk * 16, (bits >> in) & 1);
+            }
           }
-#pragma unroll
-          for (int u = 0; u < kRounds; ++u) {
-            const int t = token_of(u), chunk = chunk_of(u);
-            const long long from = __shfl_sync(0xffffffffu, the_off, s * 16 + t);
-            if (chunk < used)
-              copy16(to + unit_at(16 * w + t, chunk), (s ? v_base : k_base) + from + chunk * 16, (the_bits >> t) & 1);
-          }
-          asm volatile("cp.async.commit_group;" ::: "memory");
-        }
-      };
-      // Infinities and NaNs of V out of the lines of tokens that some node may not see.
-      auto clean = [&](unsigned char* lines, int t_block) {
-        if constexpr (!kQuantised) {
+          if (is_v && partly) {
+            asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll 1
-          for (int u = 0; u < kRounds; ++u) {
-            const int t = token_of(u), chunk = chunk_of(u);
-            if (chunk >= used) continue;
-            uint32_t* const unit = reinterpret_cast<uint32_t*>(lines + unit_at(16 * w + t, chunk));
-            bool odd = false;
-            for (int e = 0; e < 4; ++e) {
-              uint32_t x = unit[e];
-              constexpr uint32_t ones = kBf16 ? 0x7f80u : 0x7c00u;
-              if ((x & ones) == ones) x &= 0xffff0000u, odd = true;
-              if ((x & (ones << 16)) == (ones << 16)) x &= 0xffffu, odd = true;
-              unit[e] = x;
+            for (int u = 0; u < kChunks; ++u) {
+              const int in = token_of(u), chunk = chunk_of(u);
+              if (chunk >= used) continue;
+              uint32_t* const unit = reinterpret_cast<uint32_t*>(to + unit_at(32 * w + in, chunk));
+              for (int e = 0; e < 4; ++e) {
+                uint32_t x = unit[e];
+                constexpr uint32_t ones_of = kBf16 ? 0x7f80u : 0x7c00u;
+                if ((x & ones_of) == ones_of) x &= 0xffff0000u, odd |= 1u << in;
+                if ((x & (ones_of << 16)) == (ones_of << 16)) x &= 0xffffu, odd |= 1u << in;
+                unit[e] = x;
+              }
             }
-            if (odd) atomicOr(&slots[t_block % kTcSlots].odd[w >> 1], 1u << (16 * (w & 1) + t));
           }
         }
-      };
-
-      look_up();
-      step();
-      if constexpr (kQuantised) {
-        fetch(0);
-        fetch(1);
-        for (int i = 0; i < n && good; ++i) {
-          const int t = tiles_done + i, stage = t % kTcStages;
-          const unsigned turn = (t / kTcStages) & 1;
-          const bool partly = (at.tile + i + 1) * kTile > context;
-          const unsigned now_bits = bits;
-          const float now_scale = scale;
-          good = barrier_wait(&bar->k_empty[stage], turn ^ 1, failed);
-          if (!good) break;
-          describe(t, now_bits, now_scale);
-          unpack(0, k_lines(stage), t, false);
-          fence_async();
-          barrier_arrive(&bar->k_full[stage]);
-          step();
-          if (i + 1 < n) fetch(0);
-          good = barrier_wait(&bar->v_empty[stage], turn ^ 1, failed);
-          if (!good) break;
-          unpack(1, v_lines(stage), t, partly);
-          fence_async();
-          barrier_arrive(&bar->v_full[stage]);
-          if (i + 1 < n) fetch(1);
+        if (Kind != T4A_I8 && is_v && partly) {
+          odd = __reduce_or_sync(0xffffffffu, odd);
+          if (lane == 0) slots[t % kTcSlots].odd[w] = odd;
+          __syncwarp();
         }
-      } else {
-        // Tile i is announced while tile i + 1 is on its way.
-        auto announce = [&](int i) {
-          const int t = tiles_done + i, stage = t % kTcStages;
-          if ((at.tile + i + 1) * kTile > context) clean(v_lines(stage), t);
+        if (kQuantised || (is_v && partly)) {
           fence_async();
-          barrier_arrive(&bar->k_full[stage]);
-          barrier_arrive(&bar->v_full[stage]);
-        };
-        for (int i = 0; i < n && good; ++i) {
-          const int t = tiles_done + i, stage = t % kTcStages;
-          const unsigned turn = (t / kTcStages) & 1;
-          const unsigned now_bits = bits;
-          const long long now_off = off;
-          good = barrier_wait(&bar->k_empty[stage], turn ^ 1, failed);
-          if (!good) break;
-          describe(t, now_bits, 0.0f);
-          copy(0, k_lines(stage), now_off, now_bits);
-          step();
-          if (i > 0) {
-            asm volatile("cp.async.wait_group 1;" ::: "memory");  // all of tile i - 1
-            announce(i - 1);
-          }
-          good = barrier_wait(&bar->v_empty[stage], turn ^ 1, failed);
-          if (!good) break;
-          copy(1, v_lines(stage), now_off, now_bits);
+          barrier_arrive(&full[stage]);
+        } else {
+          // Arrives when this thread's copies have.
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(shared_at(&full[stage])) : "memory");
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        if (good) announce(n - 1);
+        step();
+        if (kQuantised && i + 1 < n) fetch();
       }
       tiles_done += n;
       at.left -= n;
       if (at.left > 0) next_unit(a, &at);
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp >= 8) {
     // ---- products ----
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTcIssueRegisters));
@@ -569,6 +520,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
             const int t = tiles_done + i, stage = t % kTcStages;
             good = barrier_wait(&bar->k_full[stage], (t / kTcStages) & 1, failed);
             if (!good) break;
+            fence_async();  // the rows were written by ordinary stores and copies
             tc_after();
             const unsigned k_at = shared_at(k_lines(stage));
 #pragma unroll
@@ -583,6 +535,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
             good = barrier_wait(&bar->v_full[stage], (t / kTcStages) & 1, failed) &&
                    barrier_wait(&bar->p_full[t & 1], (t >> 1) & 1, failed);
             if (!good) break;
+            fence_async();
             tc_after();
             const unsigned v_at = shared_at(v_lines(stage));
 #pragma unroll
@@ -705,11 +658,10 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
           const TcSlot& slot = slots[t % kTcSlots];
           const int pos0 = (at.tile + i) * kTile;
           const unsigned s_at = tmem + (t & 1) * 64 + lanes;
-          const uint2 there4 = *reinterpret_cast<const uint2*>(slot.there);
-          const unsigned there_lo = there4.x, there_hi = there4.y;
+          const unsigned there_lo = slot.there[0], there_hi = slot.there[1];
           const bool partly = (there_lo & there_hi) != 0xffffffffu || pos0 + kTile > context;
-          const uint2 zero4 = *reinterpret_cast<const uint2*>(slot.zero);
-          const bool rare = partly || (kQuantised && (zero4.x | zero4.y) != 0);
+          const unsigned zero_lo = kQuantised ? slot.zero[0] : 0u, zero_hi = kQuantised ? slot.zero[1] : 0u;
+          const bool rare = partly || (zero_lo | zero_hi) != 0;
           float now_factor = factor;
           const float *ks = slot.ks, *lv = slot.lv;
           unsigned see_lo = there_lo, see_hi = there_hi;
@@ -730,7 +682,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
               uint32_t s[32];
               tc_load(s, s_at + 32 * half);
               tc_loaded();
-              const unsigned see = half ? see_hi : see_lo, zero = kQuantised ? (half ? zero4.y : zero4.x) : 0u;
+              const unsigned see = half ? see_hi : see_lo, zero = half ? zero_hi : zero_lo;
               float high = -INFINITY;
 #pragma unroll
               for (int j = 0; j < 32; ++j) {
