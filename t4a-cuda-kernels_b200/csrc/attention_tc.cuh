@@ -32,28 +32,35 @@ namespace cache {
 #endif
 
 constexpr int kTcRows = 128;
-constexpr int kTcThreads = 384;
-// Registers of a thread of each role: 80 at launch, moved between the roles.
-constexpr int kTcSoftmaxRegisters = 136, kTcLoaderRegisters = 72, kTcIssueRegisters = 32;
-static_assert(kTcSoftmaxRegisters + kTcLoaderRegisters + kTcIssueRegisters == 3 * 80, "a larger sum would wait for good");
-constexpr int kTcLoaders = 64;  // threads, of K's rows and of V's
+constexpr int kTcSoftmax = 128;  // threads; the issuing warp has a warpgroup of its own
 constexpr int kTcStages = 2;
 constexpr int kTcSlots = 4;  // of tiles' scales and flags: they outlive a stage by two tiles
 constexpr unsigned kTcColumns = 256;
 
 // What a tile's rows carry beside their values.
+template <typename Flags>
 struct alignas(16) TcSlot {
   float ks[kTile];  // K's scale
   float lv[kTile];  // log2 of V's scale, -infinity for a scale of 0
   float rv[kTile];  // 1 / V's scale
-  unsigned there[2], zero[2], odd[2];  // a bit a token
+  // A bit a token, in the words or half words that K's (of odd: V's) warps write.
+  alignas(8) Flags there[8 / sizeof(Flags)];
+  alignas(8) Flags zero[8 / sizeof(Flags)];
+  alignas(8) Flags odd[8 / sizeof(Flags)];
 };
 
-static_assert(sizeof(TcSlot) % 16 == 0, "slots are read 16 bytes at a time");
+static_assert(sizeof(TcSlot<unsigned>) % 16 == 0 && sizeof(TcSlot<unsigned short>) == sizeof(TcSlot<unsigned>),
+              "slots are read 16 bytes at a time");
+
+template <typename Flags>
+__device__ __forceinline__ const unsigned* flags_of(const Flags* f) {
+  return reinterpret_cast<const unsigned*>(f);
+}
 
 // Scales that change nothing, for scores that have had theirs.
 struct alignas(16) TcNeutral {
   float ones[kTile], zeros[kTile];
+  long long row_at[kTcRows];  // and where the unit's rows of q lie, -1 for none
 };
 
 struct TcBarriers {
@@ -61,13 +68,27 @@ struct TcBarriers {
       p_full[2], o_done[2], slot_full[kTcSlots];
 };
 
+// Threads of the roles and their registers: equal at launch, then moved between the roles.  Codes
+// take twice the warps, so that unpacking keeps up with the products.
+template <bool Quantised>
+struct TcRoles {
+  static constexpr int loaders = Quantised ? 256 : 128;  // half of them K's rows, half V's
+  static constexpr int threads = kTcSoftmax + loaders + 128;
+  static constexpr int at_launch = Quantised ? 64 : 80;
+  static constexpr int softmax = Quantised ? 128 : 128, loader = Quantised ? 48 : 72, issue = Quantised ? 32 : 40;
+  static_assert(kTcSoftmax * softmax + loaders * loader + 128 * issue == threads * at_launch,
+                "a larger sum would wait for good");
+  static constexpr int side_warps = loaders / 64;         // of K, and of V
+  static constexpr int warp_tokens = kTile / side_warps;  // of a tile
+};
+
 template <int Dim>
 struct TcShape {
   static constexpr int blocks = Dim / 64;  // of 64 values, a line each
-  static constexpr int q_bytes = kTcRows * Dim * 2;
+  static constexpr int q_bytes = kTcRows * (Dim < 128 ? 128 : Dim) * 2;  // parts take 256 bytes a row
   static constexpr int tile_bytes = kTile * Dim * 2;
   static constexpr int slots_at = q_bytes + 2 * kTcStages * tile_bytes;
-  static constexpr int neutral_at = slots_at + kTcSlots * static_cast<int>(sizeof(TcSlot));
+  static constexpr int neutral_at = slots_at + kTcSlots * static_cast<int>(sizeof(TcSlot<unsigned>));
   static constexpr int barriers_at = neutral_at + static_cast<int>(sizeof(TcNeutral));
   static constexpr int shared = barriers_at + static_cast<int>(sizeof(TcBarriers)) + 16 + 1024;  // and alignment
   static constexpr int per_sm = 2;
@@ -264,17 +285,22 @@ __device__ __forceinline__ void weights(const uint32_t (&s)[32], uint32_t* p, fl
 }
 
 template <int Kind, int Dim>
-__global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(const AttendArgs a) {
+__global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcShape<Dim>::per_sm) k_attend_tc(const AttendArgs a) {
   using Shape = TcShape<Dim>;
   constexpr bool kQuantised = KindOf<Kind>::quantised, kBf16 = KindOf<Kind>::bf16;
+  using Roles = TcRoles<kQuantised>;
+  constexpr int kIssueWarp = (kTcSoftmax + Roles::loaders) / 32;
   extern __shared__ unsigned char raw[];
   unsigned char* const smem = raw + ((1024 - (shared_at(raw) & 1023)) & 1023);
   unsigned char* const q_lines = smem;
+  unsigned char* const part_lines = smem;
   auto k_lines = [&](int stage) { return smem + Shape::q_bytes + stage * Shape::tile_bytes; };
   auto v_lines = [&](int stage) { return smem + Shape::q_bytes + (kTcStages + stage) * Shape::tile_bytes; };
-  TcSlot* const slots = reinterpret_cast<TcSlot*>(smem + Shape::slots_at);
+  using Flags = std::conditional_t<kQuantised, unsigned short, unsigned>;
+  TcSlot<Flags>* const slots = reinterpret_cast<TcSlot<Flags>*>(smem + Shape::slots_at);
   float* const ones = reinterpret_cast<TcNeutral*>(smem + Shape::neutral_at)->ones;
   float* const zeros = reinterpret_cast<TcNeutral*>(smem + Shape::neutral_at)->zeros;
+  long long* const row_at = reinterpret_cast<TcNeutral*>(smem + Shape::neutral_at)->row_at;
   TcBarriers* const bar = reinterpret_cast<TcBarriers*>(smem + Shape::barriers_at);
   unsigned* const tmem_at = reinterpret_cast<unsigned*>(bar + 1);
   volatile int* const failed = reinterpret_cast<int*>(tmem_at + 1);
@@ -289,8 +315,8 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
   if (threadIdx.x == 0) {
     barrier_init(&bar->q_full, kTcRows);
     for (int i = 0; i < kTcStages; ++i) {
-      barrier_init(&bar->k_full[i], kTcLoaders);
-      barrier_init(&bar->v_full[i], kTcLoaders);
+      barrier_init(&bar->k_full[i], Roles::loaders / 2);
+      barrier_init(&bar->v_full[i], Roles::loaders / 2);
       barrier_init(&bar->k_empty[i], 1);
       barrier_init(&bar->v_empty[i], 1);
     }
@@ -300,11 +326,11 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
       barrier_init(&bar->p_full[i], kTcRows);
       barrier_init(&bar->o_done[i], 1);
     }
-    for (int i = 0; i < kTcSlots; ++i) barrier_init(&bar->slot_full[i], 2);
+    for (int i = 0; i < kTcSlots; ++i) barrier_init(&bar->slot_full[i], Roles::side_warps);
     *failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 8) {
+  if (warp == kIssueWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_at(tmem_at)),
                  "n"(kTcColumns)
                  : "memory");
@@ -312,23 +338,26 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
   }
   // The pads past dim meet zeros of Q, or make columns that are not stored; they have to be finite.
   if (dim < Dim)
-    for (int i = threadIdx.x; i < Shape::slots_at / 16; i += kTcThreads)
+    for (int i = threadIdx.x; i < Shape::slots_at / 16; i += Roles::threads)
       reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+  Cursor at = find_start(a, blockIdx.x);
   tc_before();
   fence_async();
   __syncthreads();
   tc_after();
   const unsigned tmem = *tmem_at, tmem_o = tmem + 128;
 
-  Cursor at = find_start(a, blockIdx.x);
   int tiles_done = 0;  // of the block, in all its units: phases and slots go by it
 
-  if (warp >= 4 && warp < 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTcLoaderRegisters));
-    // ---- cache rows: warps 4 and 5 K's, 6 and 7 V's, 32 of a tile's tokens each ----
-    const bool is_v = warp >= 6;
-    const int w = warp & 1;
-    constexpr int kChunks = Dim * KindOf<Kind>::bytes / 16;  // of a padded row; as many rounds of 32 lanes
+  if (warp >= 4 && warp < kIssueWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Roles::loader));
+    // ---- cache rows: half of the warps K's, half V's, an equal part of a tile's tokens each ----
+    constexpr int kTokens = Roles::warp_tokens;
+    const bool is_v = warp - 4 >= Roles::side_warps;
+    const int first_token = ((warp - 4) % Roles::side_warps) * kTokens;
+    constexpr int kChunks = Dim * KindOf<Kind>::bytes / 16;  // of a padded row
+    constexpr int kRounds = kTokens * kChunks / 32;
+    constexpr unsigned kAllThere = static_cast<unsigned>((1ull << kTokens) - 1);
     const int used = dim * KindOf<Kind>::bytes / 16;
     const Pages& mine = is_v ? a.cache.v : a.cache.k;
     unsigned long long* const full = is_v ? bar->v_full : bar->k_full;
@@ -349,7 +378,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
       const int n = min(at.left, at.tiles - at.tile);
       const unsigned char* const base = mine.base + at.head * mine.head;
       const int* const my_table = a.table + b * a.table_batch;
-      int pos = at.tile * kTile + 32 * w + lane;  // the lane's token of the next tile to look up
+      int pos = at.tile * kTile + first_token + lane % kTokens;  // the lane's token of the next tile to look up
       int in_table = pos / a.cache.page_size, place = pos - in_table * a.cache.page_size;
       const int end = min(length, (at.tile + n) * kTile);
       int page_ahead, place_ahead;
@@ -372,7 +401,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
         const int page = page_ahead, at_place = place_ahead;
         look_up();
         const bool there = static_cast<unsigned>(page) < static_cast<unsigned>(a.cache.pages);
-        bits = __ballot_sync(0xffffffffu, there);
+        bits = __ballot_sync(0xffffffffu, there) & kAllThere;
         off = there ? page * mine.page + at_place * mine.place : 0;
         if (kQuantised && !is_v) {
           ks = vs = 1.0f;
@@ -383,11 +412,11 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
           }
         }
       };
-      uint4 code[kQuantised ? kChunks : 1];
+      uint4 code[kQuantised ? kRounds : 1];
       auto fetch = [&] {
         if constexpr (kQuantised) {
 #pragma unroll
-          for (int u = 0; u < kChunks; ++u) {
+          for (int u = 0; u < kRounds; ++u) {
             const int t = token_of(u), chunk = chunk_of(u);
             const long long from = __shfl_sync(0xffffffffu, off, t);
             code[u] = make_uint4(0, 0, 0, 0);
@@ -397,17 +426,19 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
       };
       // K's warps say what the tile's tokens are.
       auto describe = [&](int t) {
-        TcSlot& slot = slots[t % kTcSlots];
-        if (lane == 0) slot.there[w] = bits;
+        TcSlot<Flags>& slot = slots[t % kTcSlots];
+        if (lane == 0) slot.there[first_token / kTokens] = static_cast<Flags>(bits);
         if constexpr (kQuantised) {
           const bool zero = vs < kLeastScale;
-          const unsigned zeros_of = __ballot_sync(0xffffffffu, zero);
-          if (lane == 0) slot.zero[w] = zeros_of;
+          const unsigned zeros_of = __ballot_sync(0xffffffffu, zero) & kAllThere;
+          if (lane == 0) slot.zero[first_token / kTokens] = static_cast<Flags>(zeros_of);
           const float lv = zero ? -INFINITY : __log2f(vs);
-          slot.ks[32 * w + lane] = ks;
-          slot.lv[32 * w + lane] = lv;
-          // A NaN has made the score a NaN where the row is seen, and must not touch l elsewhere.
-          slot.rv[32 * w + lane] = zero ? 0.0f : vs == vs ? exp2_fast(-lv) : 1.0f;
+          if (lane < kTokens) {
+            slot.ks[first_token + lane] = ks;
+            slot.lv[first_token + lane] = lv;
+            // A NaN has made the score a NaN where the row is seen, and must not touch l elsewhere.
+            slot.rv[first_token + lane] = zero ? 0.0f : vs == vs ? exp2_fast(-lv) : 1.0f;
+          }
         }
         __syncwarp();
         if (lane == 0) barrier_arrive(&bar->slot_full[t % kTcSlots]);
@@ -426,8 +457,8 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
         if constexpr (kQuantised) {
           // Codes to F16 lines.
 #pragma unroll
-          for (int u = 0; u < kChunks; ++u) {
-            const int in = token_of(u), chunk = chunk_of(u), row = 32 * w + in;
+          for (int u = 0; u < kRounds; ++u) {
+            const int in = token_of(u), chunk = chunk_of(u), row = first_token + in;
             uint32_t x[4] = {code[u].x, code[u].y, code[u].z, code[u].w}, h[8];
             if (Kind == T4A_E4M3 && is_v && partly) {
 #pragma unroll
@@ -450,30 +481,30 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
         } else {
           // 16-bit rows straight to their lines.
           const unsigned to_shared = shared_at(to);
-          if (a.plain_copies && bits == 0xffffffffu) {
+          if (a.plain_copies && bits == kAllThere) {
             const unsigned units = static_cast<unsigned>(off >> 4);
 #pragma unroll
-            for (int u = 0; u < kChunks; ++u) {
+            for (int u = 0; u < kRounds; ++u) {
               const int in = token_of(u), chunk = chunk_of(u);
               const unsigned from = __shfl_sync(0xffffffffu, units, in) + chunk;
-              copy16(to_shared + unit_at(32 * w + in, chunk), base + static_cast<unsigned long long>(from) * 16);
+              copy16(to_shared + unit_at(first_token + in, chunk), base + static_cast<unsigned long long>(from) * 16);
             }
           } else {
 #pragma unroll 4
-            for (int u = 0; u < kChunks; ++u) {
+            for (int u = 0; u < kRounds; ++u) {
               const int in = token_of(u), chunk = chunk_of(u);
               const long long from = __shfl_sync(0xffffffffu, off, in);
               if (chunk < used)
-                copy16(to_shared + unit_at(32 * w + in, chunk), base + from + chunk * 16, (bits >> in) & 1);
+                copy16(to_shared + unit_at(first_token + in, chunk), base + from + chunk * 16, (bits >> in) & 1);
             }
           }
           if (is_v && partly) {
             asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll 1
-            for (int u = 0; u < kChunks; ++u) {
+            for (int u = 0; u < kRounds; ++u) {
               const int in = token_of(u), chunk = chunk_of(u);
               if (chunk >= used) continue;
-              uint32_t* const unit = reinterpret_cast<uint32_t*>(to + unit_at(32 * w + in, chunk));
+              uint32_t* const unit = reinterpret_cast<uint32_t*>(to + unit_at(first_token + in, chunk));
               for (int e = 0; e < 4; ++e) {
                 uint32_t x = unit[e];
                 constexpr uint32_t ones_of = kBf16 ? 0x7f80u : 0x7c00u;
@@ -486,7 +517,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
         }
         if (Kind != T4A_I8 && is_v && partly) {
           odd = __reduce_or_sync(0xffffffffu, odd);
-          if (lane == 0) slots[t % kTcSlots].odd[w] = odd;
+          if (lane == 0) slots[t % kTcSlots].odd[first_token / kTokens] = static_cast<Flags>(odd);
           __syncwarp();
         }
         if (kQuantised || (is_v && partly)) {
@@ -504,10 +535,10 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
       if (at.left > 0) next_unit(a, &at);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-  } else if (warp >= 8) {
+  } else if (warp >= kIssueWarp) {
     // ---- products ----
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTcIssueRegisters));
-    if (warp == 8 && lane == 0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Roles::issue));
+    if (warp == kIssueWarp && lane == 0) {
       const unsigned form_s = tc_form<kBf16>(kTile, false), form_o = tc_form<kBf16>(Dim, true);
       const unsigned q_at = shared_at(q_lines);
       bool good = true;
@@ -554,7 +585,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
     __syncwarp();
   } else {
     // ---- softmax: thread r has query row r of the tile ----
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTcSoftmaxRegisters));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Roles::softmax));
     const unsigned lanes = static_cast<unsigned>(warp * 32) << 16;
     const int r = threadIdx.x;
     bool good = true;
@@ -576,18 +607,20 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
           return reinterpret_cast<uint4*>(q_lines + (unit >> 3) * (kTcRows * 128) + q_row * 128 +
                                           (((unit & 7) ^ (q_row & 7)) << 4));
         };
+        row_at[r] = here ? b * a.q_batch + node * a.q_node +
+                               (static_cast<long long>(at.head) * a.group + (row - node * a.group)) * a.q_head
+                         : -1;
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        const int unit = r % kUnits;
 #pragma unroll 1
         for (int u0 = 0; u0 < kUnits; u0 += 8) {
           uint4 x[8];
 #pragma unroll
           for (int u = 0; u < 8; ++u) {
-            const int k = (u0 + u) * kTcRows + r, of = k / kUnits, unit = k % kUnits;
-            const int q_row = at.row_tile * kTcRows + of, q_node = q_row / a.group;
+            const long long from_at = row_at[(u0 + u) * (kTcRows / kUnits) + r / kUnits];
             x[u] = make_uint4(0, 0, 0, 0);
-            if (q_row < a.rows && q_node < live && 8 * unit < dim) {
-              const unsigned short* const from =
-                  static_cast<const unsigned short*>(a.q) + b * a.q_batch + q_node * a.q_node +
-                  (static_cast<long long>(at.head) * a.group + (q_row - q_node * a.group)) * a.q_head + 8 * unit;
+            if (from_at >= 0 && 8 * unit < dim) {
+              const unsigned short* const from = static_cast<const unsigned short*>(a.q) + from_at + 8 * unit;
               if (a.q_units) {
                 x[u] = *reinterpret_cast<const uint4*>(from);
               } else {
@@ -599,9 +632,8 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
           }
 #pragma unroll
           for (int u = 0; u < 8; ++u) {
-            const int k = (u0 + u) * kTcRows + r;
             x[u].x ^= flip, x[u].y ^= flip, x[u].z ^= flip, x[u].w ^= flip;
-            *line_of(k / kUnits, k % kUnits) = x[u];
+            *line_of((u0 + u) * (kTcRows / kUnits) + r / kUnits, unit) = x[u];
           }
         }
         if constexpr (kQuantised) {
@@ -655,12 +687,13 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
         if (!good) break;
         tc_after();
         if (any_here) {
-          const TcSlot& slot = slots[t % kTcSlots];
+          const TcSlot<Flags>& slot = slots[t % kTcSlots];
           const int pos0 = (at.tile + i) * kTile;
           const unsigned s_at = tmem + (t & 1) * 64 + lanes;
-          const unsigned there_lo = slot.there[0], there_hi = slot.there[1];
+          const unsigned there_lo = flags_of(slot.there)[0], there_hi = flags_of(slot.there)[1];
           const bool partly = (there_lo & there_hi) != 0xffffffffu || pos0 + kTile > context;
-          const unsigned zero_lo = kQuantised ? slot.zero[0] : 0u, zero_hi = kQuantised ? slot.zero[1] : 0u;
+          const unsigned zero_lo = kQuantised ? flags_of(slot.zero)[0] : 0u,
+                         zero_hi = kQuantised ? flags_of(slot.zero)[1] : 0u;
           const bool rare = partly || (zero_lo | zero_hi) != 0;
           float now_factor = factor;
           const float *ks = slot.ks, *lv = slot.lv;
@@ -749,7 +782,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
           if (Kind != T4A_I8 && partly) {
             // What was cleaned out of V reaches the rows that see it.
             good = good && barrier_wait(&bar->v_full[t % kTcStages], (t / kTcStages) & 1, failed);
-            const volatile unsigned* const odd = slot.odd;
+            const volatile unsigned* const odd = flags_of(slot.odd);
             const uint2 odd4 = make_uint2(odd[0], odd[1]);
             if (good && (odd4.x | odd4.y)) {
               if (i > 0) good = barrier_wait(&bar->o_done[(t - 1) & 1], ((t - 1) >> 1) & 1, failed);
@@ -797,42 +830,94 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
       if (good) good = barrier_wait(&bar->o_done[(tiles_done - 1) & 1], ((tiles_done - 1) >> 1) & 1, failed);
       tc_after();
       const bool begun = at.tile == 0, whole = begun && n == at.tiles;
-      if (any_here || whole) {
-        // Sums relative to the larger reference; O stays relative to its own.
-        const float mo = m == -INFINITY ? 0.0f : less;
-        const float ml = kQuantised ? fmaxf(m == -INFINITY ? -INFINITY : less, mz) : (m == -INFINITY ? -INFINITY : less);
-        const float less_l = ml == -INFINITY ? 0.0f : ml;
-        float ll = l != 0.0f ? l * exp2_fast(mo - less_l) : 0.0f;
-        if (kQuantised && lz != 0.0f) ll += lz * exp2_fast(mz - less_l);
-        const bool dead = !here || ll == 0.0f;
-        float over = dead ? 0.0f : (mo == less_l ? 1.0f : exp2_fast(mo - less_l)) / ll;
-        float lse2 = dead ? -INFINITY : less_l + log2f(ll);
-        if (!good) over = lse2 = __uint_as_float(0x7fc00000u);
-        const long long part = (static_cast<long long>(blockIdx.x) * 2 + (begun ? 1 : 0)) * kTcRows + r;
-        const long long to = row < a.rows ? out_row(a, b, at.head, row) : 0;
+      // Sums relative to the larger reference; O stays relative to its own.
+      const float mo = m == -INFINITY ? 0.0f : less;
+      const float ml = kQuantised ? fmaxf(m == -INFINITY ? -INFINITY : less, mz) : (m == -INFINITY ? -INFINITY : less);
+      const float less_l = ml == -INFINITY ? 0.0f : ml;
+      float ll = l != 0.0f ? l * exp2_fast(mo - less_l) : 0.0f;
+      if (kQuantised && lz != 0.0f) ll += lz * exp2_fast(mz - less_l);
+      const bool dead = !here || ll == 0.0f;
+      float over = dead ? 0.0f : (mo == less_l ? 1.0f : exp2_fast(mo - less_l)) / ll;
+      float lse2 = dead ? -INFINITY : less_l + log2f(ll);
+      if (!good) over = lse2 = __uint_as_float(0x7fc00000u);
+      const long long part = (static_cast<long long>(blockIdx.x) * 2 + (begun ? 1 : 0)) * kTcRows;
+      if (row < a.rows) {
+        if (whole) store_lse(a, b, at.head, row, lse2);
+        else a.part_lse[part + r] = lse2;
+      }
+      // Results through Q's lines, which no product reads any more, so that a warp writes whole rows:
+      // 16-bit results all at once, parts in F32 by halves of a row's line block.
+      row_at[r] = row < a.rows ? (whole ? out_row(a, b, at.head, row) : (part + r) * dim) : -1;
+      if (whole) {
 #pragma unroll 1
-        for (int d = 0; d < Dim; d += 32) {
-          uint32_t o[32];
-          tc_load(o, tmem_o + lanes + d);
+        for (int d = 0; d < Dim; d += 16) {
+          uint32_t o[16], h[8];
+          tc_load16(o, tmem_o + lanes + d);
           tc_loaded();
-          if (row >= a.rows) continue;
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            if (d + e >= dim) break;
-            const float x = dead && good ? 0.0f : __uint_as_float(o[e]) * over;
-            const float y = dead && good ? 0.0f : __uint_as_float(o[e + 1]) * over;
-            if (whole) store_out(a, to + d + e, x, y, true);
-            else *reinterpret_cast<float2*>(a.part_out + part * dim + d + e) = make_float2(x, y);
+          for (int e = 0; e < 8; ++e) {
+            const float x = dead && good ? 0.0f : __uint_as_float(o[2 * e]) * over;
+            const float y = dead && good ? 0.0f : __uint_as_float(o[2 * e + 1]) * over;
+            h[e] = a.q_bf16 ? pack2<true>(x, y) : pack2<false>(x, y);
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int unit = d / 8 + e;
+            *reinterpret_cast<uint4*>(q_lines + r * (Dim * 2) + ((unit ^ (r & 7)) << 4)) =
+                make_uint4(h[4 * e], h[4 * e + 1], h[4 * e + 2], h[4 * e + 3]);
           }
         }
-        if (row < a.rows) {
-          if (whole) store_lse(a, b, at.head, row, lse2);
-          else a.part_lse[part] = lse2;
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        constexpr int kUnits = Dim / 8;
+        const int unit = r % kUnits;
+        if (8 * unit < dim) {
+#pragma unroll 4
+          for (int u = 0; u < kUnits; ++u) {
+            const int of = u * (kTcRows / kUnits) + r / kUnits;
+            const long long to = row_at[of];
+            if (to < 0) continue;
+            const uint4 x = *reinterpret_cast<const uint4*>(q_lines + of * (Dim * 2) + ((unit ^ (of & 7)) << 4));
+            unsigned short* const out = static_cast<unsigned short*>(a.out) + to + 8 * unit;
+            if (a.out_units) {
+              *reinterpret_cast<uint4*>(out) = x;
+            } else {
+              const uint32_t h[4] = {x.x, x.y, x.z, x.w};
+              for (int e = 0; e < 8; ++e) out[e] = static_cast<unsigned short>(h[e >> 1] >> (16 * (e & 1)));
+            }
+          }
         }
-      } else if (row < a.rows) {
-        a.part_lse[(static_cast<long long>(blockIdx.x) * 2 + (begun ? 1 : 0)) * kTcRows + r] = -INFINITY;
-        float* const to = a.part_out + ((static_cast<long long>(blockIdx.x) * 2 + (begun ? 1 : 0)) * kTcRows + r) * dim;
-        for (int d = 0; d < dim; ++d) to[d] = 0.0f;
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+      } else {
+#pragma unroll 1
+        for (int half = 0; half < Dim; half += 64) {
+#pragma unroll 1
+          for (int d = 0; d < 64; d += 16) {
+            uint32_t o[16];
+            tc_load16(o, tmem_o + lanes + half + d);
+            tc_loaded();
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float x[4];
+#pragma unroll
+              for (int f = 0; f < 4; ++f) x[f] = dead && good ? 0.0f : __uint_as_float(o[4 * e + f]) * over;
+              *reinterpret_cast<float4*>(part_lines + r * 256 + (((d / 4 + e) ^ (r & 7)) << 4)) =
+                  make_float4(x[0], x[1], x[2], x[3]);
+            }
+          }
+          asm volatile("bar.sync 1, 128;" ::: "memory");
+          const int unit = r % 16;  // of 4 values
+          if (half + 4 * unit < dim) {
+#pragma unroll 4
+            for (int u = 0; u < 16; ++u) {
+              const int of = u * 8 + r / 16;
+              const long long to = row_at[of];
+              if (to < 0) continue;
+              *reinterpret_cast<float4*>(a.part_out + to + half + 4 * unit) =
+                  *reinterpret_cast<const float4*>(part_lines + of * 256 + ((unit ^ (of & 7)) << 4));
+            }
+          }
+          asm volatile("bar.sync 1, 128;" ::: "memory");
+        }
       }
       tc_before();
       at.left -= n;
@@ -840,7 +925,7 @@ __global__ void __launch_bounds__(kTcThreads, TcShape<Dim>::per_sm) k_attend_tc(
     }
   }
   __syncthreads();
-  if (warp == 8) {
+  if (warp == kIssueWarp) {
     tc_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kTcColumns) : "memory");
   }

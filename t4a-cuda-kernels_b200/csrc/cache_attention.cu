@@ -236,6 +236,7 @@ extern "C" int t4a_tree_attention(void* stream, int dtype, const t4a_kv_cache* c
   a.out_node = out_layout->strides[2];
   a.out_batch = out_layout->strides[3];
   a.q_units = rows_aligned(q, *q_layout, 2, 16);
+  a.out_units = rows_aligned(out, *out_layout, 2, 16);
   a.pairs = rows_aligned(q, *q_layout, 2, 4) && rows_aligned(out, *out_layout, 2, 4);
   const Pages &k = a.cache.k, &v = a.cache.v;
   const long long last = (a.cache.pages - 1) * k.page + (a.cache.page_size - 1ll) * k.place + a.cache.dim * 2;
