@@ -1,8 +1,6 @@
 // Launches of k_attend for one cache kind: the padded dim and the row tiles pick the instance.
 #pragma once
 
-#include <atomic>
-
 #include "attention_mma.cuh"
 #include "runtime.h"
 
@@ -10,23 +8,6 @@ namespace t4a {
 namespace cache {
 
 constexpr int kSms = 148;
-
-// Allows a kernel its dynamic shared memory, once a device.
-template <typename Kernel>
-int allow_shared(Kernel kernel, int bytes, std::atomic<unsigned long long>* done) {
-  int device = 0;
-  cudaError_t err = cudaGetDevice(&device);
-  const unsigned long long bit = 1ull << (device & 63);
-  if (err == cudaSuccess && device < 64 && (done->load(std::memory_order_acquire) & bit)) return T4A_OK;
-  if (err == cudaSuccess) err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (err != cudaSuccess) {
-    runtime::last_error() = static_cast<int>(err);
-    cudaGetLastError();
-    return T4A_ERR_CUDA;
-  }
-  done->fetch_or(bit, std::memory_order_release);
-  return T4A_OK;
-}
 
 // With `blocks`, only says how many blocks to launch: as many as the SMs hold at once.
 template <int Kind, int Dim, int kRowTiles>
@@ -37,7 +18,7 @@ int launch_one(const AttendArgs& a, cudaStream_t stream, int* blocks) {
     return T4A_OK;
   }
   static std::atomic<unsigned long long> allowed{0};
-  T4A_TRY(allow_shared(k_attend<Kind, Dim, kRowTiles>, Shape::shared, &allowed));
+  T4A_TRY(runtime::allow_shared(k_attend<Kind, Dim, kRowTiles>, Shape::shared, &allowed));
   k_attend<Kind, Dim, kRowTiles><<<a.groups * a.row_tiles, kMmaThreads, Shape::shared, stream>>>(a);
   return runtime::check_launch();
 }

@@ -88,12 +88,12 @@ struct Choice {
 // Up to 32 rows a head: warp-level products over tiles of 8 rows, as few as hold them (2 at most for
 // a dim over 128, whose outputs would not fit the registers).  More rows: 128 in tensor memory; a
 // dim over 128 does not fit there beside a second block.
-Choice choose(int dim, int rows) {
+Choice choose(int kind, int dim, int rows) {
   Choice c;
   c.padded = dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : 256;
   c.row_tiles = rows <= 8 ? 1 : rows <= 16 || c.padded == 256 ? 2 : 4;
   c.rows = 8 * c.row_tiles;
-  if (rows > 32 && c.padded <= 128) {
+  if (rows > (is_quantised(kind) ? 32 : 16) && c.padded <= 128) {
     c.padded = dim <= 64 ? 64 : 128;
     c.row_tiles = 0;
     c.rows = kTcTileRows;
@@ -142,7 +142,7 @@ int plan_attention(int dtype, const t4a_kv_cache* cache, const t4a_cuda_layout* 
   a->places = static_cast<int>(places);
   a->tile_pages = kTile / a->cache.page_size;
   a->tile_places = kTile % a->cache.page_size;
-  *choice = choose(a->cache.dim, a->rows);
+  *choice = choose(cache->kind, a->cache.dim, a->rows);
   a->tile_rows = choice->rows;
   a->row_tiles = (a->rows + choice->rows - 1) / choice->rows;
   // The line of tiles is counted in 32 bits.

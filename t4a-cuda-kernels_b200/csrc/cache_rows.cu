@@ -24,7 +24,7 @@ constexpr int kThreads = 256;
 constexpr int kPerThread = 16;               // values of a row that a thread holds
 constexpr float kLeastRow = 7.8886091e-31f;  // 2^-100: Q / a stays finite above it
 
-// What one launch does: `rows` x heads rows of K (blockIdx.y 0) and of V (1).
+// What one launch does: rows x heads rows of K and of V.
 struct RowsArgs {
   View cache;
   unsigned char* act[2];  // key and value rows
@@ -149,28 +149,31 @@ struct E4m3 {
   }
 };
 
-// Where task `task` of this block row lies: its activation row, and its slot split into page
-// and place.  Tasks run head by head within a row, as activations usually lie.
+// Where a thread's row lies: its activation rows, its slot split into page and place.  A thread has
+// the same part of K's row and of V's, so that both loads are on their way before the first is
+// used.  Rows run head by head, as activations usually lie.
 struct Place {
-  const unsigned char* act;
-  long long page;
-  int place, head;
-  bool inside;
+  long long page, n;
+  int place, head, lane;
+  bool live, inside;
 };
 
-__device__ __forceinline__ Place find(const RowsArgs& a, long long task, int side) {
+__device__ __forceinline__ Place find(const RowsArgs& a) {
   Place w;
-  long long n;
+  w.lane = threadIdx.x & ((1 << a.group_shift) - 1);
+  const long long task = (static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x) >> a.group_shift;
+  w.live = task < a.tasks && w.lane * kPerThread < a.cache.dim;
+  w.inside = false;
+  if (!w.live) return w;
   if (a.tasks <= 0x7fffffffll) {  // 32-bit divisions where they serve: a 64-bit one is some 100 instructions
     const unsigned t = static_cast<unsigned>(task), q = t / static_cast<unsigned>(a.cache.heads);
-    n = q;
+    w.n = q;
     w.head = static_cast<int>(t - q * static_cast<unsigned>(a.cache.heads));
   } else {
-    n = task / a.cache.heads;
-    w.head = static_cast<int>(task - n * a.cache.heads);
+    w.n = task / a.cache.heads;
+    w.head = static_cast<int>(task - w.n * a.cache.heads);
   }
-  w.act = a.act[side] + n * a.act_row[side] + w.head * a.act_head[side];
-  const long long slot = load_slot(a, n);
+  const long long slot = load_slot(a, w.n);
   w.inside = slot >= 0 && slot < a.cache.pages * a.cache.page_size;
   if (slot <= 0x7fffffffll) {
     const unsigned s = static_cast<unsigned>(slot), q = s / static_cast<unsigned>(a.cache.page_size);
@@ -183,117 +186,133 @@ __device__ __forceinline__ Place find(const RowsArgs& a, long long task, int sid
   return w;
 }
 
+template <typename T>
+__device__ __forceinline__ unsigned char* act_at(const RowsArgs& a, const Place& w, int side) {
+  return a.act[side] + w.n * a.act_row[side] + w.head * a.act_head[side] + w.lane * kPerThread * sizeof(T);
+}
+
+__device__ __forceinline__ unsigned char* row_at(const Pages& p, const Place& w) {
+  return p.base + w.page * p.page + w.place * p.place + w.head * p.head;
+}
+
+__device__ __forceinline__ float* scale_at(const Pages& p, const Place& w) {
+  return p.scale + w.page * p.scale_page + w.place * p.scale_place + w.head * p.scale_head;
+}
+
 template <typename T, typename Code, bool Vec>
 __global__ void __launch_bounds__(kThreads) k_write_quantised(const RowsArgs a) {
-  const int side = blockIdx.y, lane = threadIdx.x & ((1 << a.group_shift) - 1);
-  const Pages& to = side ? a.cache.v : a.cache.k;
-  const long long task = (static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x) >> a.group_shift;
-  const bool live = task < a.tasks && lane * kPerThread < a.cache.dim;
-  float x[kPerThread];
-  Place w;
-  w.inside = false;
+  const Place w = find(a);
+  float x[2][kPerThread];
 #pragma unroll
-  for (int i = 0; i < kPerThread; ++i) x[i] = 0.0f;
-  if (live) {
-    w = find(a, task, side);
-    load16<T, Vec>(w.act + lane * kPerThread * sizeof(T), x);
+  for (int side = 0; side < 2; ++side) {
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) x[side][i] = 0.0f;
+    if (w.live) load16<T, Vec>(act_at<T>(a, w, side), x[side]);
   }
-  // The largest magnitude as bits: for non-negative floats they order like integers, with
-  // infinity and then NaN on top, so that neither is lost as fmaxf would lose a NaN.
-  unsigned most = 0;
 #pragma unroll
-  for (int i = 0; i < kPerThread; ++i) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
-  for (int d = 1; d < (1 << a.group_shift); d <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
-  if (!live || !w.inside) return;
-  const bool fine = most < 0x7f800000u;
-  const float top = __uint_as_float(most);
-  const bool kept = fine && top >= kLeastRow;
-  const float inverse = kept ? __fdiv_rn(Code::kMost, top) : 0.0f;
-  uint32_t code[4];
+  for (int side = 0; side < 2; ++side) {
+    // The largest magnitude as bits: for non-negative floats they order like integers, with
+    // infinity and then NaN on top, so that neither is lost as fmaxf would lose a NaN.
+    unsigned most = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float y[4];
+    for (int i = 0; i < kPerThread; ++i) most = max(most, __float_as_uint(x[side][i]) & 0x7fffffffu);
+    for (int d = 1; d < (1 << a.group_shift); d <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
+    if (!w.inside) continue;
+    const bool fine = most < 0x7f800000u;
+    const float top = __uint_as_float(most);
+    const bool kept = fine && top >= kLeastRow;
+    const float inverse = kept ? __fdiv_rn(Code::kMost, top) : 0.0f;
+    uint32_t code[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = kept ? x[4 * i + j] * inverse : 0.0f;
-    code[i] = Code::encode4(y);
+    for (int i = 0; i < 4; ++i) {
+      float y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] = kept ? x[side][4 * i + j] * inverse : 0.0f;
+      code[i] = Code::encode4(y);
+    }
+    const Pages& to = side ? a.cache.v : a.cache.k;
+    *reinterpret_cast<uint4*>(row_at(to, w) + w.lane * kPerThread) = make_uint4(code[0], code[1], code[2], code[3]);
+    if (w.lane == 0)
+      *scale_at(to, w) = kept ? top * (1.0f / Code::kMost) : fine ? 0.0f : __uint_as_float(0x7fc00000u);
   }
-  unsigned char* row = to.base + w.page * to.page + w.place * to.place + w.head * to.head;
-  *reinterpret_cast<uint4*>(row + lane * kPerThread) = make_uint4(code[0], code[1], code[2], code[3]);
-  if (lane == 0)
-    to.scale[w.page * to.scale_page + w.place * to.scale_place + w.head * to.scale_head] =
-        kept ? top * (1.0f / Code::kMost) : fine ? 0.0f : __uint_as_float(0x7fc00000u);
 }
 
 // 16-bit rows (16-byte aligned) kept as they are, rounded from T.
 template <typename T, typename C, bool Vec>
 __global__ void __launch_bounds__(kThreads) k_write_plain(const RowsArgs a) {
-  const int side = blockIdx.y, lane = threadIdx.x & ((1 << a.group_shift) - 1);
-  const Pages& to = side ? a.cache.v : a.cache.k;
-  const long long task = (static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x) >> a.group_shift;
-  if (task >= a.tasks || lane * kPerThread >= a.cache.dim) return;
-  const Place w = find(a, task, side);
-  float x[kPerThread];
-  load16<T, Vec>(w.act + lane * kPerThread * sizeof(T), x);
+  const Place w = find(a);
   if (!w.inside) return;
-  uint32_t r[8];
+  float x[2][kPerThread];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    C h[2] = {rounded<C>(x[2 * i]), rounded<C>(x[2 * i + 1])};
-    r[i] = *reinterpret_cast<const uint32_t*>(h);
+  for (int side = 0; side < 2; ++side) load16<T, Vec>(act_at<T>(a, w, side), x[side]);
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {
+    uint32_t r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      C h[2] = {rounded<C>(x[side][2 * i]), rounded<C>(x[side][2 * i + 1])};
+      r[i] = *reinterpret_cast<const uint32_t*>(h);
+    }
+    uint4* row = reinterpret_cast<uint4*>(row_at(side ? a.cache.v : a.cache.k, w) + w.lane * kPerThread * sizeof(C));
+    row[0] = make_uint4(r[0], r[1], r[2], r[3]);
+    row[1] = make_uint4(r[4], r[5], r[6], r[7]);
   }
-  uint4* row = reinterpret_cast<uint4*>(to.base + w.page * to.page + w.place * to.place + w.head * to.head +
-                                        lane * kPerThread * sizeof(C));
-  row[0] = make_uint4(r[0], r[1], r[2], r[3]);
-  row[1] = make_uint4(r[4], r[5], r[6], r[7]);
 }
 
 template <typename T, typename Code, bool Vec>
 __global__ void __launch_bounds__(kThreads) k_read_quantised(const RowsArgs a) {
-  const int side = blockIdx.y, lane = threadIdx.x & ((1 << a.group_shift) - 1);
-  const Pages& from = side ? a.cache.v : a.cache.k;
-  const long long task = (static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x) >> a.group_shift;
-  if (task >= a.tasks || lane * kPerThread >= a.cache.dim) return;
-  const Place w = find(a, task, side);
-  float x[kPerThread];
+  const Place w = find(a);
+  if (!w.live) return;
+  uint4 code[2];
+  float scale[2];
 #pragma unroll
-  for (int i = 0; i < kPerThread; ++i) x[i] = 0.0f;
-  if (w.inside) {
-    const uint4 code = *reinterpret_cast<const uint4*>(from.base + w.page * from.page + w.place * from.place +
-                                                       w.head * from.head + lane * kPerThread);
-    const float scale =
-        from.scale[w.page * from.scale_page + w.place * from.scale_place + w.head * from.scale_head];
-    const uint32_t r[4] = {code.x, code.y, code.z, code.w};
+  for (int side = 0; side < 2; ++side) {
+    const Pages& from = side ? a.cache.v : a.cache.k;
+    code[side] = make_uint4(0, 0, 0, 0);
+    scale[side] = 0.0f;
+    if (!w.inside) continue;
+    code[side] = *reinterpret_cast<const uint4*>(row_at(from, w) + w.lane * kPerThread);
+    scale[side] = *scale_at(from, w);
+  }
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {
+    const uint32_t r[4] = {code[side].x, code[side].y, code[side].z, code[side].w};
+    float x[kPerThread];
 #pragma unroll
     for (int i = 0; i < 4; ++i) Code::decode4(r[i], x + 4 * i);
 #pragma unroll
-    for (int i = 0; i < kPerThread; ++i) x[i] *= scale;
+    for (int i = 0; i < kPerThread; ++i) x[i] *= scale[side];
+    store16<T, Vec>(act_at<T>(a, w, side), x);
   }
-  store16<T, Vec>(const_cast<unsigned char*>(w.act) + lane * kPerThread * sizeof(T), x);
 }
 
 template <typename T, typename C, bool Vec>
 __global__ void __launch_bounds__(kThreads) k_read_plain(const RowsArgs a) {
-  const int side = blockIdx.y, lane = threadIdx.x & ((1 << a.group_shift) - 1);
-  const Pages& from = side ? a.cache.v : a.cache.k;
-  const long long task = (static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x) >> a.group_shift;
-  if (task >= a.tasks || lane * kPerThread >= a.cache.dim) return;
-  const Place w = find(a, task, side);
-  float x[kPerThread];
+  const Place w = find(a);
+  if (!w.live) return;
+  uint4 half[2][2];
 #pragma unroll
-  for (int i = 0; i < kPerThread; ++i) x[i] = 0.0f;
-  if (w.inside) {
-    const uint4* row = reinterpret_cast<const uint4*>(from.base + w.page * from.page + w.place * from.place +
-                                                      w.head * from.head + lane * kPerThread * sizeof(C));
-    const uint4 lo = row[0], hi = row[1];
+  for (int side = 0; side < 2; ++side) {
+    half[side][0] = half[side][1] = make_uint4(0, 0, 0, 0);
+    if (!w.inside) continue;
+    const uint4* row =
+        reinterpret_cast<const uint4*>(row_at(side ? a.cache.v : a.cache.k, w) + w.lane * kPerThread * sizeof(C));
+    half[side][0] = row[0];
+    half[side][1] = row[1];
+  }
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {
+    const uint4 lo = half[side][0], hi = half[side][1];
     const uint32_t r[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    float x[kPerThread];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const C* h = reinterpret_cast<const C*>(&r[i]);
       x[2 * i] = static_cast<float>(h[0]);
       x[2 * i + 1] = static_cast<float>(h[1]);
     }
+    store16<T, Vec>(act_at<T>(a, w, side), x);
   }
-  store16<T, Vec>(const_cast<unsigned char*>(w.act) + lane * kPerThread * sizeof(T), x);
 }
 
 template <typename T, bool Vec>
@@ -350,7 +369,7 @@ int run_rows(void* stream, int dtype, int index_dtype, const t4a_kv_cache* cache
   while ((kPerThread << a.group_shift) < a.cache.dim) ++a.group_shift;
   unsigned long long blocks;
   T4A_TRY(plan::grid_of(a.tasks, kThreads >> a.group_shift, &blocks));
-  const dim3 grid(static_cast<unsigned>(blocks), 2);
+  const dim3 grid(static_cast<unsigned>(blocks));
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
     case T4A_CUDA_F32:

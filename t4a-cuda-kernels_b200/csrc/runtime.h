@@ -3,6 +3,8 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "../../include/t4a_b200.h"
 
 namespace t4a {
@@ -19,6 +21,23 @@ inline int check_launch() {
     last_error() = static_cast<int>(err);
     return T4A_ERR_CUDA;
   }
+  return T4A_OK;
+}
+
+// Allows a kernel its dynamic shared memory, once a device.
+template <typename Kernel>
+int allow_shared(Kernel kernel, int bytes, std::atomic<unsigned long long>* done) {
+  int device = 0;
+  cudaError_t err = cudaGetDevice(&device);
+  const unsigned long long bit = 1ull << (device & 63);
+  if (err == cudaSuccess && device < 64 && (done->load(std::memory_order_acquire) & bit)) return T4A_OK;
+  if (err == cudaSuccess) err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err != cudaSuccess) {
+    last_error() = static_cast<int>(err);
+    cudaGetLastError();
+    return T4A_ERR_CUDA;
+  }
+  done->fetch_or(bit, std::memory_order_release);
   return T4A_OK;
 }
 

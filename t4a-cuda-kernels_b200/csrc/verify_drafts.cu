@@ -1,24 +1,26 @@
 // Verification of a tree of drafted tokens against the target's logits (t4a_verify_drafts).
 //
 // One cluster of 1, 2, 4 or 8 blocks walks one sequence's tree.  Only the rows of nodes that are
-// taken are read: a tree of 32 nodes has some 4 on its path, so reading ahead all rows at once
-// would read 8 times as much.  At a node
+// taken are read: a tree of 32 nodes has some 4 on its path, so reading all rows at once would
+// read 8 times as much.  At a node
 //   r = e / Z,  e_x = exp(l_x - m),  m = max l,  Z = sum e
-// is spread over the blocks' shared memory, each thread keeping the same vectors of the row in
-// every pass, so that no pass waits for another thread's values.  The blocks exchange one record
-// (maximum, sum, argmax key) per reduction through distributed shared memory; all of them then
-// take the same decisions from the same numbers.
+// Each block holds a slice of the row in shared memory as it came, each thread the same 16-byte
+// vectors in every pass, so that no pass waits for another thread's values.  A warp's record
+// (maximum, sum relative to it, argmax key) goes to all blocks of the cluster through distributed
+// shared memory, and every warp joins all records in the same order: one cluster barrier a node.
 //   Without a draft the children's tokens are left out of the row's own sum, and
 //   mass = Z_rest + (children not yet turned down): sums of positive terms only, where Z - e_x
 //   would cancel when a likely token is turned down.  So a node costs one exchange, whatever the
 //   number of its children.
 //   With a draft each child turned down costs one pass, r <- max(r - q, 0), and an exchange.  The
 //   next child's r is a scalar recursion from the masses, which every block does for itself.
-// Bound by latency: a node is a dependent load of its row (64 KB a block at 128k F32), two block
-// reductions and a cluster barrier; sequences run beside each other.
+// Bound by latency: a node is a dependent load of its row, a pass over some 32 values a thread and
+// a cluster barrier.  The race's row, wanted last, is prefetched into L2 at the start.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+
+#include <atomic>
 
 #include "cache_plan.h"
 #include "runtime.h"
@@ -31,7 +33,7 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMostCluster = 8;
 constexpr int kMostNodes = 1024;
-constexpr int kMostSlice = 49152;  // values of a row that a block keeps, F32
+constexpr int kMostBytes = 196608;  // of a block's slice: the logits, and with a draft r in F32
 
 struct VerifyArgs {
   const void* logits;
@@ -48,7 +50,7 @@ struct VerifyArgs {
   int* said;
   float* logs;
   long long vocab;
-  int nodes, greedy, slots;  // slots: vectors of a row that a block keeps
+  int nodes, slots;  // slots: vectors of a row that a block keeps
   float inverse_temperature;
 };
 
@@ -68,8 +70,8 @@ __device__ __forceinline__ unsigned long long make_key(unsigned value, long long
   return (static_cast<unsigned long long>(value) << 32) | (0xffffffffu - static_cast<unsigned>(index));
 }
 
-__device__ __forceinline__ long long key_index(unsigned long long key) {
-  return 0xffffffffu - static_cast<unsigned>(key);
+__device__ __forceinline__ int key_index(unsigned long long key) {
+  return static_cast<int>(0xffffffffu - static_cast<unsigned>(key));
 }
 
 __device__ __forceinline__ unsigned cluster_rank() {
@@ -89,10 +91,7 @@ __device__ __forceinline__ void cluster_barrier() {
 }
 
 struct Shared {
-  Record exchange[2][kMostCluster];
-  float warp_m[kWarps];
-  float warp_s[kWarps];
-  unsigned long long warp_key[kWarps];
+  Record exchange[2][kMostCluster * kWarps];
   int children, child[kMostNodes], token[kMostNodes], parent[kMostNodes];
   float child_x[kMostNodes];
   float mass[kMostNodes];  // without a draft: of what the children from here on hold; else the passes' sums
@@ -103,13 +102,22 @@ struct Shared {
   int reset_at;
 };
 
-template <typename T>
+enum Mode { kGreedy, kPlain, kDraft };
+
+template <typename T, Mode kMode>
 class Walk {
  public:
   static constexpr int kVec = 16 / sizeof(T);
+  static constexpr int kBatch = 4;  // vectors of a thread in flight
 
-  __device__ Walk(const VerifyArgs& args, Shared& shared, float* kept)
-      : a(args), sh(shared), x(kept), rank(cluster_rank()), blocks(cluster_blocks()), b(blockIdx.x / cluster_blocks()) {}
+  __device__ Walk(const VerifyArgs& args, Shared& shared, unsigned char* kept)
+      : a(args),
+        sh(shared),
+        held(reinterpret_cast<uint4*>(kept)),
+        left(reinterpret_cast<float*>(kept + static_cast<size_t>(args.slots) * 16)),
+        rank(cluster_rank()),
+        blocks(cluster_blocks()),
+        b(blockIdx.x / cluster_blocks()) {}
 
   __device__ void run() {
     const int tid = threadIdx.x;
@@ -117,29 +125,26 @@ class Walk {
       sh.token[i] = a.tokens[static_cast<long long>(b) * a.nodes + i];
       sh.parent[i] = a.parents[static_cast<long long>(b) * a.nodes + i];
     }
-    __syncthreads();
+    first = static_cast<int>(rank) * a.slots;
+    if (kMode != kGreedy && a.race_stride == 1) {
+      const float* const race = a.race + static_cast<long long>(b) * a.race_batch;
+      for (int i = first * kVec + tid * 32; i < min(static_cast<int>(a.vocab), (first + a.slots) * kVec); i += kThreads * 32)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(race + i));
+    }
     if (blocks > 1) cluster_barrier();  // every block runs before its shared memory is written from another
     int at = 0, taken = 0;
     while (true) {
-      find_children(at);
-      load_row(at);
-      const Record all = sum_row();
-      // -infinity for a row without any finite logit: it then has no probability anywhere.
-      int next;
-      float total;
-      if (a.greedy) {
-        total = all.s;
-        next = -1;
+      const Record all = read_node(at);
+      int next = -1;
+      float total = all.s;
+      if (kMode == kGreedy) {
         for (int c = 0; c < sh.children && next < 0; ++c)
           if (sh.token[sh.child[c]] == key_index(all.key)) next = c;
-      } else if (a.draft == nullptr) {
-        next = choose_plain(all, &total);
-      } else {
-        total = all.s;
-        next = choose_against_draft(at, all);
+      } else if (sh.children != 0) {
+        next = kMode == kPlain ? choose_plain(all, &total) : choose_against_draft(at, all);
       }
       if (next < 0) {
-        finish(at, taken, all, total);
+        finish(taken, all, total);
         return;
       }
       if (rank == 0 && tid == 0) {
@@ -157,29 +162,61 @@ class Walk {
  private:
   const VerifyArgs& a;
   Shared& sh;
-  float* x;  // [kVec][slots]: element e of vector j at e * slots + j, so that lanes touch neighbours
+  uint4* const held;  // [slots]: this block's vectors of the row
+  float* const left;  // [kVec][slots], with a draft: element e of vector j at e * slots + j, lanes side by side
   const unsigned rank, blocks;
   const int b;
-  int turn = 0;      // exchanges so far
+  int turn = 0;  // exchanges so far
   const T* row = nullptr;
-  int skew = 0;      // the row's first element within its 16-byte vector
-  long long first = 0, vectors = 0;  // this block's vectors of the row
-  float local_m = 0.0f;  // this block's maximum
+  int skew = 0;               // the row's first element within its 16-byte vector
+  int first = 0, vectors = 0;  // this block's vectors of the row
+  float factor = 1.0f;        // left * factor is r
+  int passes = 0;             // of r <- max(r - q, 0) at this node
 
-  __device__ float fix(float v) const { return v == v ? v * (a.greedy ? 1.0f : a.inverse_temperature) : -INFINITY; }
+  // NaN counts as -infinity (fmaxf takes the other operand).
+  __device__ float fix(float v) const { return fmaxf(kMode == kGreedy ? v : v * a.inverse_temperature, -INFINITY); }
 
   // exp(v - m), with the whole mass on infinite entries where there are some.
   static __device__ __forceinline__ float weight(float v, float m) {
-    return v == m ? (m == -INFINITY ? 0.0f : 1.0f) : expf(v - m);
+    return v == m ? (m == -INFINITY ? 0.0f : 1.0f) : exp2_of(v - m);
+  }
+  static __device__ __forceinline__ float exp2_of(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+    return r;
   }
 
   static __device__ __forceinline__ float log_of(float v, float m, float total) {
     return v == -INFINITY ? -INFINITY : (v == m ? 0.0f : v - m) - logf(total);
   }
 
-  __device__ void find_children(int at) {
-    const int lane = threadIdx.x & 31;
-    if (threadIdx.x < 32) {
+  __device__ bool in_vocab(int token) const { return token >= 0 && token < a.vocab; }
+
+  __device__ __forceinline__ uint4 load_vector(int j) const {
+    const int i = (first + j) * kVec - skew;
+    if (i >= 0 && i + kVec <= a.vocab) return __ldcs(reinterpret_cast<const uint4*>(row + i));
+    uint4 v;  // the row's ragged ends
+    T* const r = reinterpret_cast<T*>(&v);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) r[e] = i + e >= 0 && i + e < a.vocab ? row[i + e] : static_cast<T>(-INFINITY);
+    return v;
+  }
+
+  // The node's children, and its row into `held`; the cluster's record of it.
+  __device__ Record read_node(int at) {
+    const int tid = threadIdx.x, lane = tid & 31;
+    row = static_cast<const T*>(a.logits) + static_cast<long long>(b) * a.logits_batch +
+          static_cast<long long>(at) * a.logits_node;
+    skew = static_cast<int>((reinterpret_cast<uintptr_t>(row) / sizeof(T)) % kVec);
+    const int all = static_cast<int>((a.vocab + skew + kVec - 1) / kVec);
+    vectors = max(0, min(a.slots, all - first));
+    passes = 0;
+    uint4 raw[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+      if (tid + u * kThreads < vectors) raw[u] = load_vector(tid + u * kThreads);
+    if (at == 0) __syncthreads();  // tokens and parents
+    if (tid < 32) {
       int n = 0;
       for (int i0 = at + 1; i0 < a.nodes; i0 += 32) {
         const int i = i0 + lane;
@@ -191,162 +228,118 @@ class Walk {
       if (lane == 0) sh.children = n;
     }
     __syncthreads();
-  }
-
-  __device__ bool in_vocab(int token) const { return token >= 0 && token < a.vocab; }
-
-  // The node's row into `x`, its scaled values; the block's maximum and, when greedy, its argmax.
-  __device__ void load_row(int at) {
-    const int tid = threadIdx.x;
-    row = static_cast<const T*>(a.logits) + static_cast<long long>(b) * a.logits_batch +
-          static_cast<long long>(at) * a.logits_node;
-    skew = static_cast<int>((reinterpret_cast<uintptr_t>(row) / sizeof(T)) % kVec);
-    const long long all = (a.vocab + skew + kVec - 1) / kVec;
-    first = static_cast<long long>(rank) * a.slots;
-    vectors = max(0ll, min(static_cast<long long>(a.slots), all - first));
-    for (int c = tid; c < sh.children; c += kThreads) {
+    const int children = sh.children;
+    for (int c = tid; c < children; c += kThreads) {
       const int token = sh.token[sh.child[c]];
       sh.child_x[c] = in_vocab(token) ? fix(static_cast<float>(row[token])) : -INFINITY;
+      if (kMode == kPlain) {
+        int elder = c;
+        for (int k = 0; k < c && elder == c; ++k)
+          if (sh.token[sh.child[k]] == token) elder = k;
+        sh.elder[c] = elder;
+        sh.mark[c] = 0;
+      }
     }
-    float m = -INFINITY;
-    long long best = 0;
-    bool any = false;
-    constexpr int kBatch = 4;
-    for (long long j0 = tid; j0 < vectors; j0 += kBatch * kThreads) {
-      uint4 raw[kBatch];
+    Record mine;
+    mine.m = -INFINITY;
+    mine.key = 0;
+    for (int j0 = tid; j0 < vectors; j0 += kBatch * kThreads) {
+      if (j0 != tid) {
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        const long long j = j0 + u * kThreads, i = (first + j) * kVec - skew;
-        if (j >= vectors) continue;
-        if (i >= 0 && i + kVec <= a.vocab) {
-          raw[u] = __ldcs(reinterpret_cast<const uint4*>(row + i));
-        } else {  // the row's ragged ends
-          T* r = reinterpret_cast<T*>(&raw[u]);
-#pragma unroll
-          for (int e = 0; e < kVec; ++e)
-            r[e] = i + e >= 0 && i + e < a.vocab ? row[i + e] : static_cast<T>(-INFINITY);
-        }
+        for (int u = 0; u < kBatch; ++u)
+          if (j0 + u * kThreads < vectors) raw[u] = load_vector(j0 + u * kThreads);
       }
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
-        const long long j = j0 + u * kThreads, i = (first + j) * kVec - skew;
+        const int j = j0 + u * kThreads;
         if (j >= vectors) continue;
-        const T* r = reinterpret_cast<const T*>(&raw[u]);
+        held[j] = raw[u];
+        const T* const r = reinterpret_cast<const T*>(&raw[u]);
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
           const float v = fix(static_cast<float>(r[e]));
-          x[e * a.slots + j] = v;
-          if (i + e >= 0 && i + e < a.vocab && (v > m || !any)) {
-            m = v;
-            best = i + e;
-            any = true;
+          if (kMode == kGreedy) {
+            // Indices rise along a thread's walk, so the first of equals is its lowest.
+            const int i = (first + j) * kVec - skew + e;
+            if (i >= 0 && i < a.vocab && (v > mine.m || mine.key == 0)) mine.key = make_key(ordered(v), i);
           }
+          mine.m = fmaxf(mine.m, v);
         }
       }
     }
-    // Indices rise along a thread's walk, so `best` is its lowest.
-    unsigned long long key = any ? make_key(ordered(m), best) : 0;
-    block_reduce(&m, nullptr, &key);
-    local_m = m;
-    greedy_key = key;
-  }
-
-  unsigned long long greedy_key = 0;
-
-  // The sum of the row's weights over the cluster.  Without a draft (and unless greedy) the
-  // children's tokens are left out: `x` then holds -infinity at them.  With a draft `x` holds the
-  // weights themselves.
-  __device__ Record sum_row() {
-    const int tid = threadIdx.x;
-    const bool apart = !a.greedy && a.draft == nullptr, keep = !a.greedy && a.draft != nullptr;
-    if (apart) {
-      for (int c = tid; c < sh.children; c += kThreads) {
+    if (kMode == kPlain) {  // the children's tokens out of the sum, by the threads that hold them
+      for (int c = 0; c < children; ++c) {
         const int token = sh.token[sh.child[c]];
         if (!in_vocab(token)) continue;
-        const long long v = (token + static_cast<long long>(skew)) / kVec - first;
-        if (v >= 0 && v < vectors) x[(token + skew) % kVec * a.slots + v] = -INFINITY;
+        const int v = (token + skew) / kVec - first;
+        if (v >= 0 && v < vectors && v % kThreads == tid)
+          reinterpret_cast<T*>(&held[v])[(token + skew) % kVec] = static_cast<T>(-INFINITY);
       }
-      __syncthreads();
     }
-    float s = 0.0f;
-    for (long long j = tid; j < vectors; j += kThreads)
+    mine.s = 0.0f;
+    for (int j = tid; j < vectors; j += kThreads) {
+      const uint4 v = held[j];
+      const T* const r = reinterpret_cast<const T*>(&v);
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) {
-        const float w = weight(x[e * a.slots + j], local_m);
-        s += w;
-        if (keep) x[e * a.slots + j] = w;
-      }
-    block_reduce(nullptr, &s, nullptr);
-    Record mine;
-    mine.m = local_m;
-    mine.s = s;
-    mine.key = greedy_key;
+      for (int e = 0; e < kVec; ++e) mine.s += weight(fix(static_cast<float>(r[e])), mine.m);
+    }
     return exchange(mine);
   }
 
-  // Block-wide maximum, sum and largest key, in a fixed order; every thread gets them.
-  __device__ void block_reduce(float* m, float* s, unsigned long long* key) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) {
-      if (m) *m = fmaxf(*m, __shfl_xor_sync(0xffffffffu, *m, d));
-      if (s) *s += __shfl_xor_sync(0xffffffffu, *s, d);
-      if (key) *key = max(*key, __shfl_xor_sync(0xffffffffu, *key, d));
-    }
-    __syncthreads();
-    if (lane == 0) {
-      if (m) sh.warp_m[warp] = *m;
-      if (s) sh.warp_s[warp] = *s;
-      if (key) sh.warp_key[warp] = *key;
-    }
-    __syncthreads();
-    if (m) *m = sh.warp_m[0];
-    if (s) *s = sh.warp_s[0];
-    if (key) *key = sh.warp_key[0];
-    for (int w = 1; w < kWarps; ++w) {
-      if (m) *m = fmaxf(*m, sh.warp_m[w]);
-      if (s) *s += sh.warp_s[w];
-      if (key) *key = max(*key, sh.warp_key[w]);
-    }
+  static __device__ __forceinline__ Record joined(const Record& x, const Record& y) {
+    Record r;
+    r.m = fmaxf(x.m, y.m);
+    r.s = x.s * weight(x.m, r.m) + y.s * weight(y.m, r.m);
+    r.key = max(x.key, y.key);
+    return r;
   }
 
-  // All blocks' records into every block, then their combination in rank order.  Two buffers in
-  // turn: a block writes into one again only after a barrier that every block reached after its
-  // reads of it.
-  __device__ Record exchange(const Record& mine) {
-    const int buffer = turn++ & 1;
-    if (blocks == 1) return mine;
-    if (threadIdx.x < blocks) {
-      const unsigned local = static_cast<unsigned>(__cvta_generic_to_shared(&sh.exchange[buffer][rank]));
-      unsigned remote;
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(threadIdx.x));
-      asm volatile("st.shared::cluster.v2.f32 [%0], {%1,%2};" ::"r"(remote), "f"(mine.m), "f"(mine.s) : "memory");
-      asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(remote + 8), "l"(mine.key) : "memory");
+  static __device__ __forceinline__ Record across(Record r) {
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+      Record o;
+      o.m = __shfl_xor_sync(0xffffffffu, r.m, d);
+      o.s = __shfl_xor_sync(0xffffffffu, r.s, d);
+      o.key = __shfl_xor_sync(0xffffffffu, r.key, d);
+      r = joined(r, o);
     }
-    __syncwarp();
-    cluster_barrier();
-    Record all = sh.exchange[buffer][0];
-    for (unsigned r = 1; r < blocks; ++r) all.m = fmaxf(all.m, sh.exchange[buffer][r].m);
+    // The two sides of a join may round apart; decisions need one value.
+    r.m = __shfl_sync(0xffffffffu, r.m, 0);
+    r.s = __shfl_sync(0xffffffffu, r.s, 0);
+    return r;
+  }
+
+  // All threads' records joined, in one order for every warp of the cluster.  Two buffers in turn: a
+  // warp writes into one again only after a barrier that all warps reached after their reads of it.
+  __device__ Record exchange(Record mine) {
+    const int buffer = turn++ & 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    mine = across(mine);
+    const int place = static_cast<int>(rank) * kWarps + warp;
+    if (blocks == 1) {
+      if (lane == 0) sh.exchange[buffer][place] = mine;
+      __syncthreads();
+    } else {
+      if (lane < static_cast<int>(blocks)) {
+        const unsigned local = static_cast<unsigned>(__cvta_generic_to_shared(&sh.exchange[buffer][place]));
+        unsigned remote;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(lane));
+        asm volatile("st.shared::cluster.v2.f32 [%0], {%1,%2};" ::"r"(remote), "f"(mine.m), "f"(mine.s) : "memory");
+        asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(remote + 8), "l"(mine.key) : "memory");
+      }
+      __syncwarp();
+      cluster_barrier();
+    }
+    Record all;
+    all.m = -INFINITY;
     all.s = 0.0f;
-    for (unsigned r = 0; r < blocks; ++r) {
-      const Record& o = sh.exchange[buffer][r];
-      all.s += o.s * weight(o.m, all.m);
-      all.key = max(all.key, o.key);
-    }
-    return all;
+    all.key = 0;
+    for (int i = lane; i < static_cast<int>(blocks) * kWarps; i += 32) all = joined(all, sh.exchange[buffer][i]);
+    return across(all);
   }
 
   // The first child taken, -1 without one; *total is the row's whole sum.
   __device__ int choose_plain(const Record& all, float* total) {
     const int n = sh.children;
-    for (int c = threadIdx.x; c < n; c += kThreads) {
-      int first_one = c;
-      for (int k = 0; k < c && first_one == c; ++k)
-        if (sh.token[sh.child[k]] == sh.token[sh.child[c]]) first_one = k;
-      sh.elder[c] = first_one;
-      sh.mark[c] = 0;
-    }
-    __syncthreads();
     if (threadIdx.x == 0) {
       float behind = 0.0f;  // what the children from i on hold, a token once
       for (int i = n - 1; i >= 0; --i) {
@@ -388,7 +381,6 @@ class Walk {
 
   __device__ int choose_against_draft(int at, const Record& all) {
     const float* q = a.draft + static_cast<long long>(b) * a.draft_batch + static_cast<long long>(at) * a.draft_node;
-    factor = weight(local_m, all.m) / all.s;
     int masses = 0;  // passes since the node's softmax
     for (int c = 0; c < sh.children; ++c) {
       const int token = sh.token[sh.child[c]];
@@ -398,32 +390,24 @@ class Walk {
       if (in_vocab(token) && a.uniforms[static_cast<long long>(b) * a.nodes + sh.child[c]] * qx < r) return c;
       Record mine;
       mine.m = 0.0f;
-      mine.s = subtract(q);
+      mine.s = subtract(q, all, passes > 0);
       mine.key = 0;
       const float mass = exchange(mine).s;
       if (mass > 0.0f) {
         factor = 1.0f / mass;
+        ++passes;
         if (threadIdx.x == 0) sh.mass[masses] = mass;
         ++masses;
         __syncthreads();
-      } else {
-        masses = 0;
-        for (long long j = threadIdx.x; j < vectors; j += kThreads)
-#pragma unroll
-          for (int e = 0; e < kVec; ++e) {
-            const long long i = (first + j) * kVec - skew + e;
-            x[e * a.slots + j] = i >= 0 && i < a.vocab ? weight(fix(static_cast<float>(row[i])), local_m) : 0.0f;
-          }
-        factor = weight(local_m, all.m) / all.s;
+      } else {  // nothing is left: the node's softmax again
+        masses = passes = 0;
       }
     }
     return -1;
   }
 
-  float factor = 1.0f;  // x * factor is r
-
   // 16 bytes of F32 at once where they lie so.
-  static __device__ __forceinline__ void load_f32(const float* p, bool whole, long long i, long long n, float (&v)[kVec],
+  static __device__ __forceinline__ void load_f32(const float* p, bool whole, int i, long long n, float (&v)[kVec],
                                                   long long stride = 1) {
     if (whole && stride == 1 && (reinterpret_cast<uintptr_t>(p + i) & 15) == 0) {
 #pragma unroll
@@ -440,45 +424,62 @@ class Walk {
     }
   }
 
-  // x <- max(x * factor - q, 0); the block's sum of it.
-  __device__ float subtract(const float* q) {
+  // r of this thread's vector j; `again`: after a pass, else from the logits.
+  __device__ __forceinline__ void residual(int j, const Record& all, bool again, float (&r)[kVec]) const {
+    if (again) {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) r[e] = left[e * a.slots + j] * factor;
+    } else {
+      const uint4 v = held[j];
+      const T* const h = reinterpret_cast<const T*>(&v);
+      const float over = kMode == kDraft ? 1.0f / all.s : 1.0f;  // the race goes by ratios
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) r[e] = weight(fix(static_cast<float>(h[e])), all.m) * over;
+    }
+  }
+
+  // left <- max(r - q, 0); the thread's sum of it.
+  __device__ float subtract(const float* q, const Record& all, bool again) {
     float s = 0.0f;
-    for (long long j = threadIdx.x; j < vectors; j += kThreads) {
-      const long long i = (first + j) * kVec - skew;
-      float v[kVec];
+    for (int j = threadIdx.x; j < vectors; j += kThreads) {
+      const int i = (first + j) * kVec - skew;
+      float v[kVec], r[kVec];
       load_f32(q, i >= 0 && i + kVec <= a.vocab, i, a.vocab, v);
+      residual(j, all, again, r);
 #pragma unroll
       for (int e = 0; e < kVec; ++e) {
-        const float r = fmaxf(x[e * a.slots + j] * factor - v[e], 0.0f);
-        x[e * a.slots + j] = r;
-        s += r;
+        const float x = fmaxf(r[e] - v[e], 0.0f);
+        left[e * a.slots + j] = x;
+        s += x;
       }
     }
-    block_reduce(nullptr, &s, nullptr);
     return s;
   }
 
   // The last token, its log-probability, and the places that nothing was written to.
-  __device__ void finish(int at, int taken, const Record& all, float total) {
+  __device__ void finish(int taken, const Record& all, float total) {
     const int tid = threadIdx.x;
-    long long last;
-    if (a.greedy) {
+    int last;
+    if (kMode == kGreedy) {
       last = key_index(all.key);
     } else {
       const float* race = a.race + static_cast<long long>(b) * a.race_batch;
-      unsigned long long key = rank == 0 && tid == 0 ? make_key(0, 0) : 0;
-      for (long long j = tid; j < vectors; j += kThreads) {
-        const long long i = (first + j) * kVec - skew;
-        float v[kVec];
+      Record mine;
+      mine.m = mine.s = 0.0f;
+      mine.key = rank == 0 && tid == 0 ? make_key(0, 0) : 0;
+#pragma unroll 2
+      for (int j = tid; j < vectors; j += kThreads) {
+        const int i = (first + j) * kVec - skew;
+        float v[kVec], r[kVec];
         load_f32(race, i >= 0 && i + kVec <= a.vocab, i, a.vocab, v, a.race_stride);
+        residual(j, all, passes > 0, r);
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
-          const float r = a.draft ? x[e * a.slots + j] * factor : weight(x[e * a.slots + j], all.m);
-          const float score = r * v[e];
-          if (score > 0.0f) key = max(key, make_key(__float_as_uint(score), i + e));
+          const float score = r[e] * v[e];
+          if (score > 0.0f) mine.key = max(mine.key, make_key(__float_as_uint(score), i + e));
         }
       }
-      if (a.draft == nullptr && rank == 0 && tid == 0) {
+      if (kMode == kPlain && sh.children != 0 && rank == 0 && tid == 0) {
         // Children turned down before the node's softmax was taken again are back in it.
         for (int c = 0; c < sh.reset_at; ++c) {
           const int token = sh.token[sh.child[c]];
@@ -486,13 +487,9 @@ class Walk {
           for (int k = sh.reset_at; k < sh.children && back; ++k) back = sh.token[sh.child[k]] != token;
           if (!back) continue;
           const float score = weight(sh.child_x[c], all.m) * race[token * a.race_stride];
-          if (score > 0.0f) key = max(key, make_key(__float_as_uint(score), token));
+          if (score > 0.0f) mine.key = max(mine.key, make_key(__float_as_uint(score), token));
         }
       }
-      block_reduce(nullptr, nullptr, &key);
-      Record mine;
-      mine.m = mine.s = 0.0f;
-      mine.key = key;
       last = key_index(exchange(mine).key);
     }
     if (rank != 0) return;
@@ -504,33 +501,28 @@ class Walk {
     }
     if (tid == 0) {
       a.count[b] = taken;
-      a.said[o + taken] = static_cast<int>(last);
+      a.said[o + taken] = last;
       if (a.logs) a.logs[o + taken] = log_of(fix(static_cast<float>(row[last])), all.m, total);
     }
   }
 };
 
-template <typename T>
+template <typename T, Mode kMode>
 __global__ void __launch_bounds__(kThreads) k_verify(const VerifyArgs a) {
   extern __shared__ __align__(16) unsigned char raw[];
   __shared__ Shared sh;
-  Walk<T> walk(a, sh, reinterpret_cast<float*>(raw));
+  Walk<T, kMode> walk(a, sh, raw);
   walk.run();
 }
 
-template <typename T>
-int launch_verify(const VerifyArgs& a, int batch, int blocks, cudaStream_t stream) {
-  const size_t smem = static_cast<size_t>(a.slots) * Walk<T>::kVec * 4;
-  const cudaError_t set = cudaFuncSetAttribute(k_verify<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               kMostSlice * 4);
-  if (set != cudaSuccess) {
-    runtime::last_error() = static_cast<int>(set);
-    return T4A_ERR_CUDA;
-  }
+template <typename T, Mode kMode>
+int launch_verify(const VerifyArgs& a, int batch, int blocks, size_t bytes, cudaStream_t stream) {
+  static std::atomic<unsigned long long> allowed{0};
+  T4A_TRY(runtime::allow_shared(k_verify<T, kMode>, kMostBytes, &allowed));
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(batch) * blocks);
   config.blockDim = dim3(kThreads);
-  config.dynamicSmemBytes = smem;
+  config.dynamicSmemBytes = bytes;
   config.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -538,13 +530,21 @@ int launch_verify(const VerifyArgs& a, int batch, int blocks, cudaStream_t strea
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   config.attrs = attr;
   config.numAttrs = 1;
-  const cudaError_t err = cudaLaunchKernelEx(&config, k_verify<T>, a);
+  const cudaError_t err = cudaLaunchKernelEx(&config, k_verify<T, kMode>, a);
   if (err != cudaSuccess) {
     runtime::last_error() = static_cast<int>(err);
     cudaGetLastError();
     return T4A_ERR_CUDA;
   }
   return T4A_OK;
+}
+
+template <typename T>
+int launch_mode(const VerifyArgs& a, bool greedy, int batch, int blocks, cudaStream_t stream) {
+  const size_t logits = static_cast<size_t>(a.slots) * 16, r = static_cast<size_t>(a.slots) * (16 / sizeof(T)) * 4;
+  if (greedy) return launch_verify<T, kGreedy>(a, batch, blocks, logits, stream);
+  if (a.draft == nullptr) return launch_verify<T, kPlain>(a, batch, blocks, logits, stream);
+  return launch_verify<T, kDraft>(a, batch, blocks, logits + r, stream);
 }
 
 }  // namespace
@@ -568,13 +568,13 @@ extern "C" int t4a_verify_drafts(void* stream, int dtype, const void* logits, co
   if (!(temperature >= 0.0f) || temperature > 3.0e38f || (temperature > 0.0f && temperature < 1e-30f))
     return T4A_ERR_UNSUPPORTED_OP;
   VerifyArgs a = {};
-  a.greedy = temperature == 0.0f;
+  const bool greedy = temperature == 0.0f;
   if (nodes > kMostNodes) return T4A_ERR_DOMAIN_TOO_LARGE;
   if (logits == nullptr || tokens == nullptr || parents == nullptr || count == nullptr || path == nullptr ||
       said == nullptr)
     return T4A_ERR_NULL_ARGUMENT;
   if (!aligned(logits, esize)) return T4A_ERR_INVALID_STRIDE;
-  if (!a.greedy) {
+  if (!greedy) {
     if (uniforms == nullptr || race == nullptr) return T4A_ERR_NULL_ARGUMENT;
     T4A_TRY(check_tensor(race_layout, 2, race_len, 4));
     if (race_layout->extents[0] != vocab || race_layout->extents[1] != batch) return T4A_ERR_SHAPE_MISMATCH;
@@ -602,7 +602,7 @@ extern "C" int t4a_verify_drafts(void* stream, int dtype, const void* logits, co
   a.logs = logs;
   a.vocab = vocab;
   a.nodes = static_cast<int>(nodes);
-  a.inverse_temperature = a.greedy ? 1.0f : static_cast<float>(1.0 / static_cast<double>(temperature));
+  a.inverse_temperature = greedy ? 1.0f : static_cast<float>(1.0 / static_cast<double>(temperature));
   // Blocks of a cluster: a slice of at least 4096 values each, so that a block's load outweighs
   // its barriers, and as many as it takes for a slice to fit a block's shared memory.
   const int vec = 16 / esize;
@@ -610,13 +610,14 @@ extern "C" int t4a_verify_drafts(void* stream, int dtype, const void* logits, co
   while (blocks < kMostCluster && vocab >= blocks * 2 * 4096ll) blocks *= 2;
   const long long vectors = (vocab + 2 * vec - 2) / vec;  // at the worst skew
   const long long slots = (vectors + blocks - 1) / blocks;
-  if (slots * vec > kMostSlice || vocab > 0x7fffffffll) return T4A_ERR_DOMAIN_TOO_LARGE;
+  const long long bytes = slots * (16 + (a.draft != nullptr ? vec * 4 : 0));
+  if (bytes > kMostBytes) return T4A_ERR_DOMAIN_TOO_LARGE;
   if (batch * blocks > 0x7fffffffll) return T4A_ERR_LAUNCH_LIMIT;
   a.slots = static_cast<int>(slots);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
-    case T4A_CUDA_F32: return launch_verify<float>(a, static_cast<int>(batch), blocks, s);
-    case T4A_F16: return launch_verify<__half>(a, static_cast<int>(batch), blocks, s);
-    default: return launch_verify<__nv_bfloat16>(a, static_cast<int>(batch), blocks, s);
+    case T4A_CUDA_F32: return launch_mode<float>(a, greedy, static_cast<int>(batch), blocks, s);
+    case T4A_F16: return launch_mode<__half>(a, greedy, static_cast<int>(batch), blocks, s);
+    default: return launch_mode<__nv_bfloat16>(a, greedy, static_cast<int>(batch), blocks, s);
   }
 }
