@@ -9,44 +9,52 @@ namespace {
 
 constexpr int kJoinThreads = 128, kJoinWarps = kJoinThreads / 32;
 
-// One block a query row of a head: nothing where one block of the attention had the whole unit;
-// zeros where the sequence has nothing to see; else the row's parts weighed by 2^(lse - max).  The
-// warps take every fourth part, so that a long sequence's parts (some 60 of them) come in a few
-// rounds of loads, and are added in a fixed order.  It is launched beside the attention and finds
-// its place on the line of tiles while that runs.
+// Joins the parts of a query row of a head: nothing where one group of the attention had the whole
+// unit; zeros where the sequence has nothing to see; else its parts weighed by 2^(lse - max), in a
+// fixed order.  kWarps warps take a row's parts in turn: one where units have a few parts, four
+// where a long sequence has dozens, which then come in a few rounds of loads.  Launched beside the
+// attention, it finds its place on the line of tiles while that runs.
+template <int kWarps>
 __global__ void __launch_bounds__(kJoinThreads) k_join(const AttendArgs a) {
-  __shared__ float sums[kJoinWarps][kMaxDim], weights[kJoinWarps], tops[kJoinWarps];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, dim = a.cache.dim;
+  __shared__ float sums[kWarps == 1 ? 1 : kWarps][kMaxDim], weights[kWarps], tops[kWarps];
+  const int lane = threadIdx.x & 31, warp = kWarps == 1 ? 0 : threadIdx.x >> 5, dim = a.cache.dim;
+  const unsigned task = blockIdx.x * (kJoinWarps / kWarps) + (kWarps == 1 ? threadIdx.x >> 5 : 0);
   const unsigned rows = static_cast<unsigned>(a.cache.heads) * a.rows;
-  const int b = blockIdx.x / rows, in = blockIdx.x - b * rows, head = in / a.rows, row = in - head * a.rows;
+  const int b = task / rows, in = task - b * rows, head = in / a.rows, row = in - head * a.rows;
+  const bool any = b < a.batch;
   const int row_tile = row / a.tile_rows, r = row - row_tile * a.tile_rows;
-  const int tiles = sequence_tiles(a, b);
+  const int tiles = any ? sequence_tiles(a, b) : 0;
   const Line line = read_line(a, b);
   const int quota = quota_of(a, line.total), start = line.before + head * tiles;
   const int c0 = start / quota, c1 = tiles == 0 ? c0 : (start + tiles - 1) / quota;
-  const long long to = out_row(a, b, head, row);
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!any) return;
+  const long long to = out_row(a, b, head, row);
   if (tiles == 0) {
-    for (int d = 2 * threadIdx.x; d < dim; d += 2 * kJoinThreads) store_out(a, to + d, 0.0f, 0.0f, true);
-    if (threadIdx.x == 0) store_lse(a, b, head, row, -INFINITY);
+    for (int d = 2 * (warp * 32 + lane); d < dim; d += 64 * kWarps) store_out(a, to + d, 0.0f, 0.0f, true);
+    if (warp == 0 && lane == 0) store_lse(a, b, head, row, -INFINITY);
     return;
   }
   if (c0 == c1) return;
-  auto part = [&](int c) { return ((static_cast<long long>(c) * a.row_tiles + row_tile) * 2 + (c == c0 ? 1 : 0)) * a.tile_rows + r; };
+  auto part = [&](int c) {
+    return ((static_cast<long long>(c) * a.row_tiles + row_tile) * 2 + (c == c0 ? 1 : 0)) * a.tile_rows + r;
+  };
   float most = -INFINITY;
-  for (int c = c0 + threadIdx.x; c <= c1; c += kJoinThreads) most = fmaxf(most, a.part_lse[part(c)]);
+  for (int c = c0 + warp * 32 + lane; c <= c1; c += 32 * kWarps) most = fmaxf(most, a.part_lse[part(c)]);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-  if (lane == 0) tops[warp] = most;
-  __syncthreads();
+  if constexpr (kWarps > 1) {
+    if (lane == 0) tops[warp] = most;
+    __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) most = fmaxf(most, tops[w]);
+    for (int w = 0; w < kWarps; ++w) most = fmaxf(most, tops[w]);
+  }
   const float less = most == -INFINITY ? 0.0f : most;
   float x[8], sum = 0.0f;  // columns 2 * lane + 64 * k and the next
 #pragma unroll
   for (int k = 0; k < 8; ++k) x[k] = 0.0f;
-#pragma unroll 8
-  for (int c = c0 + warp; c <= c1; c += kJoinWarps) {
+#pragma unroll 4
+  for (int c = c0 + warp; c <= c1; c += kWarps) {
     const long long at = part(c);
     const float w = exp2f(a.part_lse[at] - less);
     sum += w;
@@ -59,26 +67,35 @@ __global__ void __launch_bounds__(kJoinThreads) k_join(const AttendArgs a) {
       x[2 * k + 1] += w * v.y;
     }
   }
+  if constexpr (kWarps > 1) {
 #pragma unroll
-  for (int k = 0; k < 4; ++k) *reinterpret_cast<float2*>(&sums[warp][2 * lane + 64 * k]) = make_float2(x[2 * k], x[2 * k + 1]);
-  if (lane == 0) weights[warp] = sum;
-  __syncthreads();
-  sum = 0.0f;
+    for (int k = 0; k < 4; ++k)
+      *reinterpret_cast<float2*>(&sums[warp][2 * lane + 64 * k]) = make_float2(x[2 * k], x[2 * k + 1]);
+    if (lane == 0) weights[warp] = sum;
+    __syncthreads();
+    if (warp != 0) return;
+    sum = 0.0f;
 #pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) sum += weights[w];
+    for (int k = 0; k < 8; ++k) x[k] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      sum += weights[w];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 v = *reinterpret_cast<const float2*>(&sums[w][2 * lane + 64 * k]);
+        x[2 * k] += v.x;
+        x[2 * k + 1] += v.y;
+      }
+    }
+  }
   const bool empty = sum == 0.0f;
   const float over = empty ? 0.0f : 1.0f / sum;
-  const int d = 2 * threadIdx.x;
-  if (d < dim) {
-    float2 v = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) {
-      v.x += sums[w][d];
-      v.y += sums[w][d + 1];
-    }
-    store_out(a, to + d, v.x * over, v.y * over, true);
+  for (int k = 0; k < 4; ++k) {
+    const int d = 2 * lane + 64 * k;
+    if (d < dim) store_out(a, to + d, x[2 * k] * over, x[2 * k + 1] * over, true);
   }
-  if (threadIdx.x == 0) store_lse(a, b, head, row, empty ? -INFINITY : less + log2f(sum));
+  if (lane == 0) store_lse(a, b, head, row, empty ? -INFINITY : less + log2f(sum));
 }
 
 struct Choice {
@@ -254,7 +271,10 @@ extern "C" int t4a_tree_attention(void* stream, int dtype, const t4a_kv_cache* c
   T4A_TRY(dispatch(cache->kind, a, choice, s, nullptr));
 
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(static_cast<unsigned>(a.batch) * a.cache.heads * a.rows);
+  // At most so many parts to a unit where all are as long as each other.
+  const long long rows = static_cast<long long>(a.batch) * a.cache.heads * a.rows;
+  const bool few = a.groups <= 6ll * a.batch * a.cache.heads;
+  config.gridDim = dim3(static_cast<unsigned>(few ? (rows + kJoinWarps - 1) / kJoinWarps : rows));
   config.blockDim = dim3(kJoinThreads);
   config.stream = s;
   cudaLaunchAttribute attr[1];
@@ -262,7 +282,7 @@ extern "C" int t4a_tree_attention(void* stream, int dtype, const t4a_kv_cache* c
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attr;
   config.numAttrs = 1;
-  const cudaError_t err = cudaLaunchKernelEx(&config, k_join, a);
+  const cudaError_t err = few ? cudaLaunchKernelEx(&config, k_join<1>, a) : cudaLaunchKernelEx(&config, k_join<kJoinWarps>, a);
   if (err != cudaSuccess) {
     runtime::last_error() = static_cast<int>(err);
     cudaGetLastError();

@@ -116,14 +116,12 @@ __device__ __forceinline__ void store16(unsigned char* p, const float (&x)[kPerT
 // The two 8-bit codes.
 struct Int8 {
   static constexpr float kMost = 127.0f;
+  // |x| <= 127.00001: adding 1.5 * 2^23 leaves the nearest integer, ties to even, in the low bits.
   static __device__ __forceinline__ uint32_t encode4(const float* x) {
-    uint32_t r = 0;
+    uint32_t r[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int c = max(-127, min(127, __float2int_rn(x[i])));
-      r |= static_cast<uint32_t>(c & 0xff) << (8 * i);
-    }
-    return r;
+    for (int i = 0; i < 4; ++i) r[i] = __float_as_uint(__fadd_rn(x[i], 12582912.0f));
+    return __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
   }
   static __device__ __forceinline__ void decode4(uint32_t r, float* x) {
 #pragma unroll
@@ -199,36 +197,77 @@ __device__ __forceinline__ float* scale_at(const Pages& p, const Place& w) {
   return p.scale + w.page * p.scale_page + w.place * p.scale_place + w.head * p.scale_head;
 }
 
+// 16 values of a row as they lie.
+template <typename T, bool Vec>
+__device__ __forceinline__ void load_raw(const unsigned char* p, uint32_t (&r)[4 * sizeof(T)]) {
+  if constexpr (Vec) {
+#pragma unroll
+    for (unsigned h = 0; h < sizeof(T) / 2; ++h) load32(p + 32 * h, reinterpret_cast<uint32_t(&)[8]>(r[8 * h]));
+  } else if constexpr (sizeof(T) == 2) {
+    const unsigned short* t = reinterpret_cast<const unsigned short*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = t[2 * i] | static_cast<uint32_t>(t[2 * i + 1]) << 16;
+  } else {
+    const uint32_t* t = reinterpret_cast<const uint32_t*>(p);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) r[i] = t[i];
+  }
+}
+
+// Value i of them.
+template <typename T>
+__device__ __forceinline__ float raw_value(const uint32_t* r, int i) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(r[i]);
+  else if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    return __uint_as_float(i & 1 ? r[i >> 1] & 0xffff0000u : r[i >> 1] << 16);
+  else return __half2float(__ushort_as_half(static_cast<unsigned short>(r[i >> 1] >> (16 * (i & 1)))));
+}
+
+// The largest magnitude of a row over its group of lanes, and whether the row is finite.  Magnitudes
+// are compared as bits: of non-negative floats they order like integers, with infinity and then NaN
+// on top, so that neither is lost as a maximum of floats would lose a NaN; 16-bit ones in pairs.
+template <typename T>
+__device__ __forceinline__ float largest(const uint32_t (&r)[4 * sizeof(T)], int group, bool* fine) {
+  unsigned most = 0;
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = __vmaxu2(most, r[i] & 0x7fff7fffu);
+    most = max(most >> 16, most & 0xffffu);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) most = max(most, r[i] & 0x7fffffffu);
+  }
+  for (int d = 1; d < group; d <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
+  constexpr unsigned infinity =
+      sizeof(T) == 4 ? 0x7f800000u : std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+  *fine = most < infinity;
+  return raw_value<T>(&most, 0);
+}
+
 template <typename T, typename Code, bool Vec>
 __global__ void __launch_bounds__(kThreads) k_write_quantised(const RowsArgs a) {
   const Place w = find(a);
-  float x[2][kPerThread];
+  uint32_t raw[2][4 * sizeof(T)];
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
 #pragma unroll
-    for (int i = 0; i < kPerThread; ++i) x[side][i] = 0.0f;
-    if (w.live) load16<T, Vec>(act_at<T>(a, w, side), x[side]);
+    for (unsigned i = 0; i < 4 * sizeof(T); ++i) raw[side][i] = 0;
+    if (w.live) load_raw<T, Vec>(act_at<T>(a, w, side), raw[side]);
   }
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
-    // The largest magnitude as bits: for non-negative floats they order like integers, with
-    // infinity and then NaN on top, so that neither is lost as fmaxf would lose a NaN.
-    unsigned most = 0;
-#pragma unroll
-    for (int i = 0; i < kPerThread; ++i) most = max(most, __float_as_uint(x[side][i]) & 0x7fffffffu);
-    for (int d = 1; d < (1 << a.group_shift); d <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
+    bool fine;
+    const float top = largest<T>(raw[side], 1 << a.group_shift, &fine);
     if (!w.inside) continue;
-    const bool fine = most < 0x7f800000u;
-    const float top = __uint_as_float(most);
     const bool kept = fine && top >= kLeastRow;
-    const float inverse = kept ? __fdiv_rn(Code::kMost, top) : 0.0f;
+    const float inverse = __fdiv_rn(Code::kMost, kept ? top : 1.0f);
     uint32_t code[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float y[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] = kept ? x[side][4 * i + j] * inverse : 0.0f;
-      code[i] = Code::encode4(y);
+      for (int j = 0; j < 4; ++j) y[j] = __fmul_rn(raw_value<T>(raw[side], 4 * i + j), inverse);
+      code[i] = kept ? Code::encode4(y) : 0u;
     }
     const Pages& to = side ? a.cache.v : a.cache.k;
     *reinterpret_cast<uint4*>(row_at(to, w) + w.lane * kPerThread) = make_uint4(code[0], code[1], code[2], code[3]);

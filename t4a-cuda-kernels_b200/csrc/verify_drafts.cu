@@ -33,7 +33,7 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMostCluster = 8;
 constexpr int kMostNodes = 1024;
-constexpr int kMostBytes = 196608;  // of a block's slice: the logits, and with a draft r in F32
+constexpr int kMostBytes = 188416;  // of a block's slice: the logits, and with a draft r in F32
 
 struct VerifyArgs {
   const void* logits;
@@ -93,7 +93,7 @@ __device__ __forceinline__ void cluster_barrier() {
 struct Shared {
   Record exchange[2][kMostCluster * kWarps];
   int children, child[kMostNodes], token[kMostNodes], parent[kMostNodes];
-  float child_x[kMostNodes];
+  float child_x[kMostNodes], child_q[kMostNodes], child_u[kMostNodes];  // scaled logit, draft, uniform
   float mass[kMostNodes];  // without a draft: of what the children from here on hold; else the passes' sums
   int elder[kMostNodes];   // the first child with the same token
   int mark[kMostNodes];    // of a child that is its own elder: the count of resets when it was turned down, plus 1
@@ -232,6 +232,11 @@ class Walk {
     for (int c = tid; c < children; c += kThreads) {
       const int token = sh.token[sh.child[c]];
       sh.child_x[c] = in_vocab(token) ? fix(static_cast<float>(row[token])) : -INFINITY;
+      if (kMode != kGreedy) sh.child_u[c] = a.uniforms[static_cast<long long>(b) * a.nodes + sh.child[c]];
+      if (kMode == kDraft)
+        sh.child_q[c] = in_vocab(token) ? a.draft[static_cast<long long>(b) * a.draft_batch +
+                                                  static_cast<long long>(at) * a.draft_node + token]
+                                        : 0.0f;
       if (kMode == kPlain) {
         int elder = c;
         for (int k = 0; k < c && elder == c; ++k)
@@ -352,7 +357,7 @@ class Walk {
       for (int i = 0; i < n && whole > 0.0f; ++i) {
         const int e = sh.elder[i];
         const float r = sh.mark[e] == resets + 1 ? 0.0f : weight(sh.child_x[i], all.m);
-        if (a.uniforms[static_cast<long long>(b) * a.nodes + sh.child[i]] * mass < r) {
+        if (sh.child_u[i] * mass < r) {
           found = i;
           break;
         }
@@ -384,10 +389,10 @@ class Walk {
     int masses = 0;  // passes since the node's softmax
     for (int c = 0; c < sh.children; ++c) {
       const int token = sh.token[sh.child[c]];
-      const float qx = in_vocab(token) ? q[token] : 0.0f;
+      const float qx = sh.child_q[c];
       float r = weight(sh.child_x[c], all.m) / all.s;
       for (int i = 0; i < masses; ++i) r = fmaxf(r - qx, 0.0f) / sh.mass[i];
-      if (in_vocab(token) && a.uniforms[static_cast<long long>(b) * a.nodes + sh.child[c]] * qx < r) return c;
+      if (in_vocab(token) && sh.child_u[c] * qx < r) return c;
       Record mine;
       mine.m = 0.0f;
       mine.s = subtract(q, all, passes > 0);
