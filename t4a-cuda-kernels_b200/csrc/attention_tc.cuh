@@ -27,9 +27,10 @@
 namespace t4a {
 namespace cache {
 
-#ifndef T4A_STAGE_WAIT_LIMIT
-#define T4A_STAGE_WAIT_LIMIT (1u << 20)
-#endif
+// Rounds of a wait (a round is some 100 cycles) between looks at the other roles' failure, and looks
+// before it gives up.  The inner loop is as short as it can be: a warp that polls takes issue slots
+// from the warps it waits for.
+constexpr unsigned kTcWaitRounds = 1u << 14, kTcWaitLooks = 1u << 10;
 
 constexpr int kTcRows = 128;
 constexpr int kTcSoftmax = 128;  // threads; the issuing warp has a warpgroup of its own
@@ -105,12 +106,15 @@ __device__ __forceinline__ void barrier_arrive(unsigned long long* b) {
 // False when the phase did not complete within the limit, or another role's wait ran out.
 __device__ __forceinline__ bool barrier_wait(unsigned long long* b, unsigned parity, volatile int* failed) {
   const unsigned at = shared_at(b);
-  for (unsigned i = 0; i < T4A_STAGE_WAIT_LIMIT; ++i) {
+  for (unsigned i = 0; i < kTcWaitLooks; ++i) {
     unsigned ok;
     asm volatile(
-        "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+        "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\tmov.u32 n, %3;\n"
+        "WAIT:\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra DONE;\n\t"
+        "sub.u32 n, n, 1;\n\tsetp.ne.u32 q, n, 0;\n\t@q bra WAIT;\n"
+        "DONE:\n\tselp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
-        : "r"(at), "r"(parity)
+        : "r"(at), "r"(parity), "n"(kTcWaitRounds)
         : "memory");
     if (ok) return true;
     if (*failed) return false;
@@ -364,8 +368,11 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
     unsigned long long* const empty = is_v ? bar->v_empty : bar->k_empty;
     auto lines = [&](int stage) { return is_v ? v_lines(stage) : k_lines(stage); };
     // The row and chunk of a lane in round u.
-    auto token_of = [&](int u) { return (u * 32 + lane) / kChunks; };
-    auto chunk_of = [&](int u) { return (u * 32 + lane) % kChunks; };
+    // Codes become two units each: 8 lanes then take 4 chunks of two rows, whose units the swizzle
+    // keeps apart, rather than 8 of one.
+    constexpr bool kPairs = kQuantised && kChunks == 8;
+    auto token_of = [&](int u) { return kPairs ? u * 4 + (lane >> 4) * 2 + ((lane >> 2) & 1) : (u * 32 + lane) / kChunks; };
+    auto chunk_of = [&](int u) { return kPairs ? ((lane >> 3) & 1) * 4 + (lane & 3) : (u * 32 + lane) % kChunks; };
     // Swizzled place of a 16-byte unit of 8 values of row t.
     auto unit_at = [&](int t, int unit) {
       return (unit >> 3) * (kTile * 128) + t * 128 + (((unit & 7) ^ (t & 7)) << 4);
@@ -470,12 +477,9 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) neighbours<Kind>(x[e], &h[2 * e], &h[2 * e + 1]);
-            // Half of the lanes store their second unit first: 8 lanes then meet 8 units.
-            const bool swap = (chunk >> 2) & 1;
-            const uint4 lo = make_uint4(h[0], h[1], h[2], h[3]), hi = make_uint4(h[4], h[5], h[6], h[7]);
             if (chunk < used) {
-              *reinterpret_cast<uint4*>(to + unit_at(row, 2 * chunk + (swap ? 1 : 0))) = swap ? hi : lo;
-              *reinterpret_cast<uint4*>(to + unit_at(row, 2 * chunk + (swap ? 0 : 1))) = swap ? lo : hi;
+              *reinterpret_cast<uint4*>(to + unit_at(row, 2 * chunk)) = make_uint4(h[0], h[1], h[2], h[3]);
+              *reinterpret_cast<uint4*>(to + unit_at(row, 2 * chunk + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
             }
           }
         } else {
