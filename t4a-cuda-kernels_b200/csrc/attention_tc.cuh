@@ -41,7 +41,7 @@ constexpr unsigned kTcColumns = 256;
 // What a tile's rows carry beside their values.
 template <typename Flags>
 struct alignas(16) TcSlot {
-  float ks[kTile];  // K's scale
+  float ks[kTile];  // K's scale, times the magnitude of the score's
   float lv[kTile];  // log2 of V's scale, -infinity for a scale of 0
   float rv[kTile];  // 1 / V's scale
   // A bit a token, in the words or half words that K's (of odd: V's) warps write.
@@ -103,11 +103,23 @@ __device__ __forceinline__ void barrier_arrive(unsigned long long* b) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_at(b)) : "memory");
 }
 
-// False when the phase did not complete within the limit, or another role's wait ran out.
+// False when the phase did not complete within the limit, or another role's wait ran out.  A patient
+// wait sleeps between polls: for roles that run ahead of the products.
+template <bool Patient = false>
 __device__ __forceinline__ bool barrier_wait(unsigned long long* b, unsigned parity, volatile int* failed) {
   const unsigned at = shared_at(b);
   for (unsigned i = 0; i < kTcWaitLooks; ++i) {
     unsigned ok;
+    if constexpr (Patient) {
+      asm volatile(
+          "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\tmov.u32 n, %3;\n"
+          "WAIT:\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra DONE;\n\tnanosleep.u32 100;\n\t"
+          "sub.u32 n, n, 1;\n\tsetp.ne.u32 q, n, 0;\n\t@q bra WAIT;\n"
+          "DONE:\n\tselp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(ok)
+          : "r"(at), "r"(parity), "n"(kTcWaitRounds)
+          : "memory");
+    } else
     asm volatile(
         "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\tmov.u32 n, %3;\n"
         "WAIT:\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra DONE;\n\t"
@@ -130,6 +142,10 @@ __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_
 __device__ __forceinline__ void tc_commit(unsigned long long* b) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(shared_at(b))
                : "memory");
+}
+
+__device__ __forceinline__ void store16(unsigned at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
 // 32 columns of the warp's 32 lanes.
@@ -207,32 +223,6 @@ __device__ __forceinline__ void tc_store16(unsigned at, const uint32_t (&r)[16])
       : "memory");
 }
 
-// Two F32 operations in one instruction.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  unsigned long long r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(r)
-      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)),
-        "l"(*reinterpret_cast<unsigned long long*>(&c)));
-  return *reinterpret_cast<float2*>(&r);
-}
-
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  unsigned long long r;
-  asm("add.rn.f32x2 %0, %1, %2;"
-      : "=l"(r)
-      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
-  return *reinterpret_cast<float2*>(&r);
-}
-
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  unsigned long long r;
-  asm("mul.rn.f32x2 %0, %1, %2;"
-      : "=l"(r)
-      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
-  return *reinterpret_cast<float2*>(&r);
-}
-
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -251,40 +241,43 @@ __device__ __forceinline__ float highest(const uint32_t (&s)[32]) {
 }
 
 // Products of codes to base-2 scores.
-__device__ __forceinline__ void scale_scores(uint32_t (&s)[32], const float* ks, const float* lv, float factor) {
-  const float2 f = make_float2(factor, factor);
+__device__ __forceinline__ void scale_scores(uint32_t (&s)[32], const float* ks, const float* lv) {
 #pragma unroll
   for (int j = 0; j < 32; j += 4) {
     const float4 k = *reinterpret_cast<const float4*>(ks + j), v = *reinterpret_cast<const float4*>(lv + j);
-    const float2 lo = fma2(make_float2(__uint_as_float(s[j]), __uint_as_float(s[j + 1])),
-                           mul2(make_float2(k.x, k.y), f), make_float2(v.x, v.y));
-    const float2 hi = fma2(make_float2(__uint_as_float(s[j + 2]), __uint_as_float(s[j + 3])),
-                           mul2(make_float2(k.z, k.w), f), make_float2(v.z, v.w));
-    s[j] = __float_as_uint(lo.x);
-    s[j + 1] = __float_as_uint(lo.y);
-    s[j + 2] = __float_as_uint(hi.x);
-    s[j + 3] = __float_as_uint(hi.y);
+    s[j] = __float_as_uint(fmaf(__uint_as_float(s[j]), k.x, v.x));
+    s[j + 1] = __float_as_uint(fmaf(__uint_as_float(s[j + 1]), k.y, v.y));
+    s[j + 2] = __float_as_uint(fmaf(__uint_as_float(s[j + 2]), k.z, v.z));
+    s[j + 3] = __float_as_uint(fmaf(__uint_as_float(s[j + 3]), k.w, v.w));
   }
 }
 
-// Weights 2^(s * factor - less) as pairs of 16-bit values, and their sums (over V's scale).
+// Weights 2^(s * factor - less) as pairs of 16-bit values, and their sums (over V's scale).  (Packed
+// F32 arithmetic was slower: its register pairs cost more moves than it saved.)
 template <bool Quantised, bool Bf16>
 __device__ __forceinline__ void weights(const uint32_t (&s)[32], uint32_t* p, float factor, float less, const float* rv,
-                                        float2 (&l)[2]) {
-  const float2 f = make_float2(factor, factor), minus = make_float2(-less, -less);
+                                        float (&l)[4]) {
 #pragma unroll
   for (int j = 0; j < 32; j += 4) {
     float4 r;
     if constexpr (Quantised) r = *reinterpret_cast<const float4*>(rv + j);
+    float w[4];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const float2 x = make_float2(__uint_as_float(s[j + 2 * e]), __uint_as_float(s[j + 2 * e + 1]));
-      const float2 y = Quantised ? add2(x, minus) : fma2(x, f, minus);
-      const float2 w = make_float2(exp2_fast(y.x), exp2_fast(y.y));
-      if constexpr (Quantised) l[e] = fma2(w, e ? make_float2(r.z, r.w) : make_float2(r.x, r.y), l[e]);
-      else l[e] = add2(l[e], w);
-      p[(j >> 1) + e] = pack2<Bf16>(w.x, w.y);
+    for (int e = 0; e < 4; ++e) {
+      const float x = __uint_as_float(s[j + e]);
+      w[e] = exp2_fast(Quantised ? x - less : fmaf(x, factor, -less));
     }
+    if constexpr (Quantised) {
+      l[0] = fmaf(w[0], r.x, l[0]);
+      l[1] = fmaf(w[1], r.y, l[1]);
+      l[2] = fmaf(w[2], r.z, l[2]);
+      l[3] = fmaf(w[3], r.w, l[3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) l[e] += w[e];
+    }
+    p[j >> 1] = pack2<Bf16>(w[0], w[1]);
+    p[(j >> 1) + 1] = pack2<Bf16>(w[2], w[3]);
   }
 }
 
@@ -368,14 +361,23 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
     unsigned long long* const empty = is_v ? bar->v_empty : bar->k_empty;
     auto lines = [&](int stage) { return is_v ? v_lines(stage) : k_lines(stage); };
     // The row and chunk of a lane in round u.
+    // The row and chunk of a lane in round u: round u's rows are kStep further on than round 0's.
     // Codes become two units each: 8 lanes then take 4 chunks of two rows, whose units the swizzle
     // keeps apart, rather than 8 of one.
     constexpr bool kPairs = kQuantised && kChunks == 8;
-    auto token_of = [&](int u) { return kPairs ? u * 4 + (lane >> 4) * 2 + ((lane >> 2) & 1) : (u * 32 + lane) / kChunks; };
-    auto chunk_of = [&](int u) { return kPairs ? ((lane >> 3) & 1) * 4 + (lane & 3) : (u * 32 + lane) % kChunks; };
+    constexpr int kStep = 32 / kChunks;
+    const int lane_token = kPairs ? (lane >> 4) * 2 + ((lane >> 2) & 1) : lane / kChunks;
+    const int chunk = kPairs ? ((lane >> 3) & 1) * 4 + (lane & 3) : lane % kChunks;
     // Swizzled place of a 16-byte unit of 8 values of row t.
     auto unit_at = [&](int t, int unit) {
       return (unit >> 3) * (kTile * 128) + t * 128 + (((unit & 7) ^ (t & 7)) << 4);
+    };
+    // first_token is a multiple of 8, so row u's swizzle is round 0's with (u * kStep) & 7 flipped into it
+    // (lane_token < kStep, a power of 2).
+    const int unit = kQuantised ? 2 * chunk : chunk;
+    const unsigned lane_unit = unit_at(first_token + lane_token, unit);
+    auto round_unit = [&](unsigned stage_at, int u) {
+      return ((stage_at + lane_unit) ^ (((u * kStep) & 7) << 4)) + u * kStep * 128;
     };
     bool good = true;
     while (at.left > 0 && good) {
@@ -422,9 +424,18 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
       uint4 code[kQuantised ? kRounds : 1];
       auto fetch = [&] {
         if constexpr (kQuantised) {
+          if (a.plain_copies && bits == kAllThere) {
+            const unsigned units = static_cast<unsigned>(off >> 4);
+#pragma unroll
+            for (int u = 0; u < kRounds; ++u) {
+              const unsigned from = __shfl_sync(0xffffffffu, units, u * kStep + lane_token) + chunk;
+              code[u] = *reinterpret_cast<const uint4*>(base + static_cast<unsigned long long>(from) * 16);
+            }
+            return;
+          }
 #pragma unroll
           for (int u = 0; u < kRounds; ++u) {
-            const int t = token_of(u), chunk = chunk_of(u);
+            const int t = u * kStep + lane_token;
             const long long from = __shfl_sync(0xffffffffu, off, t);
             code[u] = make_uint4(0, 0, 0, 0);
             if (((bits >> t) & 1) && chunk < used) code[u] = *reinterpret_cast<const uint4*>(base + from + chunk * 16);
@@ -441,7 +452,7 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
           if (lane == 0) slot.zero[first_token / kTokens] = static_cast<Flags>(zeros_of);
           const float lv = zero ? -INFINITY : __log2f(vs);
           if (lane < kTokens) {
-            slot.ks[first_token + lane] = ks;
+            slot.ks[first_token + lane] = ks * fabsf(a.scale_log2);
             slot.lv[first_token + lane] = lv;
             // A NaN has made the score a NaN where the row is seen, and must not touch l elsewhere.
             slot.rv[first_token + lane] = zero ? 0.0f : vs == vs ? exp2_fast(-lv) : 1.0f;
@@ -456,57 +467,55 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
       for (int i = 0; i < n; ++i) {
         const int t = tiles_done + i, stage = t % kTcStages;
         const bool partly = (at.tile + i + 1) * kTile > context;
-        good = barrier_wait(&empty[stage], ((t / kTcStages) & 1) ^ 1, failed);
+        good = barrier_wait<true>(&empty[stage], ((t / kTcStages) & 1) ^ 1, failed);
         if (!good) break;
         unsigned char* const to = lines(stage);
+        const unsigned to_shared = shared_at(to);
         if (!is_v) describe(t);
         unsigned odd = 0;  // tokens with an infinity or a NaN in V, where some node may not see them
         if constexpr (kQuantised) {
           // Codes to F16 lines.
 #pragma unroll
           for (int u = 0; u < kRounds; ++u) {
-            const int in = token_of(u), chunk = chunk_of(u), row = first_token + in;
             uint32_t x[4] = {code[u].x, code[u].y, code[u].z, code[u].w}, h[8];
             if (Kind == T4A_E4M3 && is_v && partly) {
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const uint32_t nan = __vcmpeq4(x[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-                if (nan != 0) odd |= 1u << in;
+                if (nan != 0) odd |= 1u << (u * kStep + lane_token);
                 x[e] &= ~nan;
               }
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) neighbours<Kind>(x[e], &h[2 * e], &h[2 * e + 1]);
             if (chunk < used) {
-              *reinterpret_cast<uint4*>(to + unit_at(row, 2 * chunk)) = make_uint4(h[0], h[1], h[2], h[3]);
-              *reinterpret_cast<uint4*>(to + unit_at(row, 2 * chunk + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
+              const unsigned place_at = round_unit(to_shared, u);
+              store16(place_at, h[0], h[1], h[2], h[3]);
+              store16(place_at ^ 16, h[4], h[5], h[6], h[7]);
             }
           }
         } else {
           // 16-bit rows straight to their lines.
-          const unsigned to_shared = shared_at(to);
           if (a.plain_copies && bits == kAllThere) {
             const unsigned units = static_cast<unsigned>(off >> 4);
 #pragma unroll
             for (int u = 0; u < kRounds; ++u) {
-              const int in = token_of(u), chunk = chunk_of(u);
-              const unsigned from = __shfl_sync(0xffffffffu, units, in) + chunk;
-              copy16(to_shared + unit_at(first_token + in, chunk), base + static_cast<unsigned long long>(from) * 16);
+              const unsigned from = __shfl_sync(0xffffffffu, units, u * kStep + lane_token) + chunk;
+              copy16(round_unit(to_shared, u), base + static_cast<unsigned long long>(from) * 16);
             }
           } else {
 #pragma unroll 4
             for (int u = 0; u < kRounds; ++u) {
-              const int in = token_of(u), chunk = chunk_of(u);
+              const int in = u * kStep + lane_token;
               const long long from = __shfl_sync(0xffffffffu, off, in);
-              if (chunk < used)
-                copy16(to_shared + unit_at(first_token + in, chunk), base + from + chunk * 16, (bits >> in) & 1);
+              if (chunk < used) copy16(round_unit(to_shared, u), base + from + chunk * 16, (bits >> in) & 1);
             }
           }
           if (is_v && partly) {
             asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll 1
             for (int u = 0; u < kRounds; ++u) {
-              const int in = token_of(u), chunk = chunk_of(u);
+              const int in = u * kStep + lane_token;
               if (chunk >= used) continue;
               uint32_t* const unit = reinterpret_cast<uint32_t*>(to + unit_at(first_token + in, chunk));
               for (int e = 0; e < 4; ++e) {
@@ -602,7 +611,9 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
       const bool here = row < a.rows && node < live, any_here = __any_sync(0xffffffffu, here);
       // A negative scale is Q's sign, so that the largest product is the largest score.
       const unsigned flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
-      float factor = fabsf(a.scale_log2);
+      // Codes: K's scales have the score's; what is left is the row's power of two.
+      float factor = kQuantised ? 1.0f : fabsf(a.scale_log2);
+      bool shifted = false;  // whether some row of the warp has one
       {
         // The rows into their lines: units of 8 values, so that a warp reads whole rows; then zeros
         // into the thread's lanes of O.
@@ -640,36 +651,32 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
             *line_of((u0 + u) * (kTcRows / kUnits) + r / kUnits, unit) = x[u];
           }
         }
-        if constexpr (kQuantised) {
-          // Each thread its own row, in place: to F16 and scaled.
+        if (kQuantised && a.q_bf16) {
+          // Each thread its own row, in place: BF16 to F16, exact for 2^-14 to 2^16 and off by 2^-25 below,
+          // so a row whose largest magnitude is outside [1/4, 2^15) is first brought to [2^14, 2^15).
           asm volatile("bar.sync 1, 128;" ::: "memory");
-          auto value = [&](uint32_t x, int e) {
-            const unsigned short h = static_cast<unsigned short>(e ? x >> 16 : x);
-            return a.q_bf16 ? __uint_as_float(static_cast<uint32_t>(h) << 16) : __half2float(__ushort_as_half(h));
-          };
-          float most = 0.0f;
+          unsigned most = 0;
 #pragma unroll 4
-          for (int unit = 0; unit < kUnits; ++unit) {
-            const uint4 x = *line_of(r, unit);
-            const uint32_t h[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float v = fabsf(value(h[e >> 1], e & 1));
-              if (v < INFINITY) most = fmaxf(most, v);
-            }
+          for (int u = 0; u < kUnits; ++u) {
+            const uint4 x = *line_of(r, u);
+            most = __vmaxu2(most, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu),
+                                           __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
           }
-          int e = static_cast<int>(__float_as_uint(most) >> 23);  // biased exponent
-          e = most == 0.0f ? 127 : max(e, 16);
-          const float down = __uint_as_float(static_cast<unsigned>(min(127 + 14 + 127 - e, 253)) << 23);
-          factor /= down;
+          most = max(most >> 16, most & 0xffffu);
+          float down = 1.0f;
+          if (most != 0 && most < 0x7f80u && (most < 0x3e80u || most >= 0x4700u)) {
+            const int e = max(static_cast<int>(most >> 7), 16);  // biased exponent
+            down = __uint_as_float(static_cast<unsigned>(min(127 + 14 + 127 - e, 253)) << 23);
+            factor = 1.0f / down;
+          }
+          shifted = __any_sync(0xffffffffu, down != 1.0f);
+          auto f16_pair = [&](uint32_t h) {
+            return pack2<false>(__uint_as_float(h << 16) * down, __uint_as_float(h & 0xffff0000u) * down);
+          };
 #pragma unroll 4
-          for (int unit = 0; unit < kUnits; ++unit) {
-            const uint4 x = *line_of(r, unit);
-            const uint32_t h[4] = {x.x, x.y, x.z, x.w};
-            uint32_t y[4];
-#pragma unroll
-            for (int e2 = 0; e2 < 4; ++e2) y[e2] = pack2<false>(value(h[e2], 0) * down, value(h[e2], 1) * down);
-            *line_of(r, unit) = make_uint4(y[0], y[1], y[2], y[3]);
+          for (int u = 0; u < kUnits; ++u) {
+            const uint4 x = *line_of(r, u);
+            *line_of(r, u) = make_uint4(f16_pair(x.x), f16_pair(x.y), f16_pair(x.z), f16_pair(x.w));
           }
         }
         uint32_t zero[32];
@@ -683,11 +690,13 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
         barrier_arrive(&bar->q_full);
       }
       float m = -INFINITY, less = -1e30f, mz = -INFINITY, lz = 0.0f;
-      float2 l2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+      float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       for (int i = 0; i < n && good; ++i) {
         const int t = tiles_done + i;
-        good = barrier_wait(&bar->slot_full[t % kTcSlots], (t / kTcSlots) & 1, failed) &&
-               barrier_wait(&bar->s_full[t & 1], (t >> 1) & 1, failed);
+        // Warps without a live row only keep step.
+        good = any_here ? barrier_wait(&bar->slot_full[t % kTcSlots], (t / kTcSlots) & 1, failed) &&
+                              barrier_wait(&bar->s_full[t & 1], (t >> 1) & 1, failed)
+                        : barrier_wait<true>(&bar->s_full[t & 1], (t >> 1) & 1, failed);
         if (!good) break;
         tc_after();
         if (any_here) {
@@ -698,8 +707,8 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
           const bool partly = (there_lo & there_hi) != 0xffffffffu || pos0 + kTile > context;
           const unsigned zero_lo = kQuantised ? flags_of(slot.zero)[0] : 0u,
                          zero_hi = kQuantised ? flags_of(slot.zero)[1] : 0u;
-          const bool rare = partly || (zero_lo | zero_hi) != 0;
-          float now_factor = factor;
+          const bool rare = partly || (zero_lo | zero_hi) != 0 || (kQuantised && shifted);
+          float now_factor = kQuantised ? 1.0f : factor;
           const float *ks = slot.ks, *lv = slot.lv;
           unsigned see_lo = there_lo, see_hi = there_hi;
           if (rare) {
@@ -754,8 +763,8 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
           tc_load(s1, s_at + 32);
           tc_loaded();
           if constexpr (kQuantised) {
-            scale_scores(s0, ks, lv, now_factor);
-            scale_scores(s1, ks + 32, lv + 32, now_factor);
+            scale_scores(s0, ks, lv);
+            scale_scores(s1, ks + 32, lv + 32);
           }
           float top = fmaxf(highest(s0), highest(s1));
           if constexpr (!kQuantised) top *= now_factor;  // factors are not negative
@@ -766,7 +775,7 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
               shrink = exp2_fast(m - top);
               m = top;
               less = top - kLift;
-              l2[0].x *= shrink, l2[0].y *= shrink, l2[1].x *= shrink, l2[1].y *= shrink;
+              l4[0] *= shrink, l4[1] *= shrink, l4[2] *= shrink, l4[3] *= shrink;
             }
             if (i > 0) {
               good = barrier_wait(&bar->o_done[(t - 1) & 1], ((t - 1) >> 1) & 1, failed);
@@ -821,15 +830,15 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
           }
           uint32_t p[32];
           const float first_factor = kQuantised ? 1.0f : now_factor;
-          weights<kQuantised, kBf16>(s0, p, first_factor, less, slot.rv, l2);
-          weights<kQuantised, kBf16>(s1, p + 16, first_factor, less, slot.rv + 32, l2);
+          weights<kQuantised, kBf16>(s0, p, first_factor, less, slot.rv, l4);
+          weights<kQuantised, kBf16>(s1, p + 16, first_factor, less, slot.rv + 32, l4);
           tc_store(s_at, p);
           tc_stored();
           tc_before();
         }
         barrier_arrive(&bar->p_full[t & 1]);
       }
-      const float l = (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
+      const float l = (l4[0] + l4[1]) + (l4[2] + l4[3]);
       tiles_done += n;
       if (good) good = barrier_wait(&bar->o_done[(tiles_done - 1) & 1], ((tiles_done - 1) >> 1) & 1, failed);
       tc_after();
