@@ -76,7 +76,7 @@ struct TcRoles {
   static constexpr int loaders = Quantised ? 256 : 128;  // half of them K's rows, half V's
   static constexpr int threads = kTcSoftmax + loaders + 128;
   static constexpr int at_launch = Quantised ? 64 : 80;
-  static constexpr int softmax = Quantised ? 128 : 128, loader = Quantised ? 48 : 72, issue = Quantised ? 32 : 40;
+  static constexpr int softmax = Quantised ? 96 : 120, loader = Quantised ? 64 : 72, issue = Quantised ? 32 : 48;
   static_assert(kTcSoftmax * softmax + loaders * loader + 128 * issue == threads * at_launch,
                 "a larger sum would wait for good");
   static constexpr int side_warps = loaders / 64;         // of K, and of V
@@ -278,6 +278,17 @@ __device__ __forceinline__ void weights(const uint32_t (&s)[32], uint32_t* p, fl
     }
     p[j >> 1] = pack2<Bf16>(w[0], w[1]);
     p[(j >> 1) + 1] = pack2<Bf16>(w[2], w[3]);
+  }
+}
+
+// A pair of weights, times x.
+template <bool Bf16>
+__device__ __forceinline__ uint32_t scaled_pair(uint32_t pair, float x) {
+  if constexpr (Bf16) {
+    return pack2<true>(__uint_as_float(pair << 16) * x, __uint_as_float(pair & 0xffff0000u) * x);
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pair));
+    return pack2<false>(f.x * x, f.y * x);
   }
 }
 
@@ -710,7 +721,7 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
           const bool rare = partly || (zero_lo | zero_hi) != 0 || (kQuantised && shifted);
           float now_factor = kQuantised ? 1.0f : factor;
           const float *ks = slot.ks, *lv = slot.lv;
-          unsigned see_lo = there_lo, see_hi = there_hi;
+          unsigned see_lo = there_lo, see_hi = there_hi, odd_lo = 0, odd_hi = 0;
           if (rare) {
             // Scores with what is not seen at -infinity, back to tensor memory for the common path;
             // V rows with a scale of 0 into their own sum.
@@ -758,57 +769,69 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
             ks = ones;
             lv = zeros;
           }
-          uint32_t s0[32], s1[32];
-          tc_load(s0, s_at);
-          tc_load(s1, s_at + 32);
-          tc_loaded();
-          if constexpr (kQuantised) {
-            scale_scores(s0, ks, lv);
-            scale_scores(s1, ks + 32, lv + 32);
+          if (Kind != T4A_I8 && partly) {
+            // Whether something was cleaned out of V, for the rows that see it.
+            good = barrier_wait(&bar->v_full[t % kTcStages], (t / kTcStages) & 1, failed);
+            const volatile unsigned* const odd = flags_of(slot.odd);
+            odd_lo = odd[0];
+            odd_hi = odd[1];
           }
-          float top = fmaxf(highest(s0), highest(s1));
-          if constexpr (!kQuantised) top *= now_factor;  // factors are not negative
-          const bool rises = here && top > less + (kSlack + kLift);
-          if (__any_sync(0xffffffffu, rises)) {
-            float shrink = 1.0f;
-            if (rises) {
-              shrink = exp2_fast(m - top);
-              m = top;
-              less = top - kLift;
-              l4[0] *= shrink, l4[1] *= shrink, l4[2] *= shrink, l4[3] *= shrink;
-            }
-            if (i > 0) {
-              good = barrier_wait(&bar->o_done[(t - 1) & 1], ((t - 1) >> 1) & 1, failed);
-              tc_after();
+          // By halves of 32 tokens, so that a thread needs few registers; P's first half overwrites
+          // scores that have been read.
 #pragma unroll 1
-              for (int d = 0; d < Dim; d += 16) {
-                uint32_t o[16];
-                tc_load16(o, tmem_o + lanes + d);
+          for (int half = 0; half < 2; ++half) {
+            uint32_t s[32];
+            tc_load(s, s_at + 32 * half);
+            tc_loaded();
+            if constexpr (kQuantised) scale_scores(s, ks + 32 * half, lv + 32 * half);
+            float top = highest(s);
+            if constexpr (!kQuantised) top *= now_factor;  // factors are not negative
+            const bool rises = here && top > less + (kSlack + kLift);
+            if (__any_sync(0xffffffffu, rises)) {
+              float shrink = 1.0f;
+              if (rises) {
+                shrink = exp2_fast(m - top);
+                m = top;
+                less = top - kLift;
+                l4[0] *= shrink, l4[1] *= shrink, l4[2] *= shrink, l4[3] *= shrink;
+              }
+              if (half == 1) {
+                // The first half's weights go by the old reference.
+                uint32_t p[16];
+                tc_load16(p, s_at);
                 tc_loaded();
 #pragma unroll
-                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink);
-                tc_store16(tmem_o + lanes + d, o);
+                for (int e = 0; e < 16; ++e) p[e] = scaled_pair<kBf16>(p[e], shrink);
+                tc_store16(s_at, p);
               }
-              tc_stored();
+              if (i > 0) {
+                good = good && barrier_wait(&bar->o_done[(t - 1) & 1], ((t - 1) >> 1) & 1, failed);
+                tc_after();
+#pragma unroll 1
+                for (int d = 0; d < Dim; d += 16) {
+                  uint32_t o[16];
+                  tc_load16(o, tmem_o + lanes + d);
+                  tc_loaded();
+#pragma unroll
+                  for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink);
+                  tc_store16(tmem_o + lanes + d, o);
+                }
+                tc_stored();
+              }
             }
-          }
-          if (Kind != T4A_I8 && partly) {
-            // What was cleaned out of V reaches the rows that see it.
-            good = good && barrier_wait(&bar->v_full[t % kTcStages], (t / kTcStages) & 1, failed);
-            const volatile unsigned* const odd = flags_of(slot.odd);
-            const uint2 odd4 = make_uint2(odd[0], odd[1]);
-            if (good && (odd4.x | odd4.y)) {
+            if (Kind != T4A_I8 && (half ? odd_hi : odd_lo) != 0 && good) {
               if (i > 0) good = barrier_wait(&bar->o_done[(t - 1) & 1], ((t - 1) >> 1) & 1, failed);
               tc_after();
 #pragma unroll 1
-              for (int j = 0; j < kTile; ++j) {
-                if (!(((j < 32 ? odd4.x : odd4.y) >> (j & 31)) & 1)) continue;
+              for (int j = 0; j < 32; ++j) {
+                if (!(((half ? odd_hi : odd_lo) >> j) & 1)) continue;
                 uint32_t score;
-                tc_load1(&score, s_at + j);
+                tc_load1(&score, s_at + 32 * half + j);
                 tc_loaded();
-                const bool sees = here && (((j < 32 ? see_lo : see_hi) >> (j & 31)) & 1);
+                const bool sees = here && (((half ? see_hi : see_lo) >> j) & 1);
                 const float w = exp2_fast(__uint_as_float(score) - less);
-                const int at_pos = pos0 + j, page = a.table[b * a.table_batch + (at_pos / a.cache.page_size) * a.table_page];
+                const int at_pos = pos0 + 32 * half + j;
+                const int page = a.table[b * a.table_batch + (at_pos / a.cache.page_size) * a.table_page];
                 const unsigned char* const v_row = a.cache.v.base + at.head * a.cache.v.head + page * a.cache.v.page +
                                                    (at_pos % a.cache.page_size) * a.cache.v.place;
 #pragma unroll 1
@@ -827,13 +850,11 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
                 tc_stored();
               }
             }
+            uint32_t p[16];
+            weights<kQuantised, kBf16>(s, p, kQuantised ? 1.0f : now_factor, less, slot.rv + 32 * half, l4);
+            tc_store16(s_at + 16 * half, p);
+            tc_stored();
           }
-          uint32_t p[32];
-          const float first_factor = kQuantised ? 1.0f : now_factor;
-          weights<kQuantised, kBf16>(s0, p, first_factor, less, slot.rv, l4);
-          weights<kQuantised, kBf16>(s1, p + 16, first_factor, less, slot.rv + 32, l4);
-          tc_store(s_at, p);
-          tc_stored();
           tc_before();
         }
         barrier_arrive(&bar->p_full[t & 1]);
