@@ -42,7 +42,7 @@ struct AttendArgs {
   int places;       // table pages * page_size, or the most that 32 bits allow
   int tile_pages, tile_places;  // kTile / page_size and kTile % page_size
   int q_bf16;      // q and out are BF16, else F16
-  int plain_copies;  // K and V have the same strides, rows fill the padded dim, and offsets / 16 fit 32 bits
+  int plain_copies;  // K and V have the same strides, rows fill the padded dim, and offsets fit 32 bits
   int q_units, out_units;  // q and out rows start on 16-byte boundaries
   int pairs;       // q and out rows start on 4-byte boundaries
   float* part_out;  // [groups][row_tiles][2][tile_rows][dim]

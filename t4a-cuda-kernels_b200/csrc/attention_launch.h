@@ -19,8 +19,8 @@ int launch_one(const AttendArgs& a, cudaStream_t stream, int* blocks) {
   }
   static std::atomic<unsigned long long> allowed{0};
   T4A_TRY(runtime::allow_shared(k_attend<Kind, Dim, kRowTiles>, Shape::shared, &allowed));
-  k_attend<Kind, Dim, kRowTiles><<<a.groups * a.row_tiles, kMmaThreads, Shape::shared, stream>>>(a);
-  return runtime::check_launch();
+  return runtime::launch_early<AttendArgs>(k_attend<Kind, Dim, kRowTiles>, a.groups * a.row_tiles, kMmaThreads,
+                                           Shape::shared, stream, a);
 }
 
 template <int Kind, int Dim>

@@ -113,6 +113,19 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// The first product of a sum.
+template <bool Bf16>
+__device__ __forceinline__ void mma_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (Bf16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
 template <bool Bf16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   if constexpr (Bf16) {
@@ -263,6 +276,7 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
   unsigned char* const q_rows = smem + Shape::ring;
   float* const most_of = reinterpret_cast<float*>(q_rows + kRows * Shape::q_pitch);
 
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   Cursor at = find_start(a, blockIdx.x);
 
@@ -291,6 +305,9 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
     const unsigned char* const k_base = a.cache.k.base + at.head * a.cache.k.head;
     const unsigned char* const v_base = a.cache.v.base + at.head * a.cache.v.head;
     const float* const head_scale = kQuantised ? side.scale + at.head * side.scale_head : nullptr;
+    // 32-bit strides, in 16-byte units and in scales, where plain copies serve.
+    const unsigned page_units = static_cast<unsigned>(side.page >> 4), place_units = static_cast<unsigned>(side.place >> 4);
+    const int scale_page = static_cast<int>(side.scale_page), scale_place = static_cast<int>(side.scale_place);
     const int* const my_table = a.table + b * a.table_batch;
     int pos = tile0 * kTile + 16 * warp + (lane & 15);  // of the next page to look up
     int in_table = pos / a.cache.page_size, place = pos - in_table * a.cache.page_size;
@@ -317,14 +334,12 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
         const bool there = static_cast<unsigned>(page) < static_cast<unsigned>(a.cache.pages);
         const unsigned bits = __ballot_sync(0xffffffffu, there) & 0xffffu;
         if (lane == 0) reinterpret_cast<unsigned*>(stage + kSeen)[warp] = bits;
-        if constexpr (kQuantised)
-          copy4(shared_at(stage + kScales + ((lane >> 4) * kTile + 16 * warp + (lane & 15)) * 4),
-                head_scale + (there ? page * side.scale_page + at_place * side.scale_place : 0), there);
-        const long long off = there ? page * side.page + at_place * side.place : 0;
         const unsigned to = shared_at(my_rows + to_stage * Shape::stage);
+        const unsigned scale_to = shared_at(stage + kScales + ((lane >> 4) * kTile + 16 * warp + (lane & 15)) * 4);
         if (a.plain_copies && bits == 0xffffu) {
           // All tokens are there, K and V lie alike, and 16-byte units of an offset fit 32 bits.
-          const unsigned units = static_cast<unsigned>(off >> 4);
+          const unsigned units = page * page_units + at_place * place_units;
+          if constexpr (kQuantised) copy4(scale_to, head_scale + page * scale_page + at_place * scale_place, true);
 #pragma unroll
           for (int u = 0; u < 16 * Shape::chunks / 32; ++u) {
             const int k = u * 32 + lane, t = k / Shape::chunks, chunk = k - t * Shape::chunks;
@@ -334,6 +349,9 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
             copy16(to + kV + t * Shape::pitch + chunk * 16, v_base + from);
           }
         } else {
+          const long long off = there ? page * side.page + at_place * side.place : 0;
+          if constexpr (kQuantised)
+            copy4(scale_to, head_scale + (there ? page * side.scale_page + at_place * side.scale_place : 0), there);
 #pragma unroll
           for (int s = 0; s < 2; ++s)
 #pragma unroll 4
@@ -379,14 +397,15 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
       for (int j = 0; j < kRowTiles; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[k][j][e] = 0.0f;
-    // Of rows 8j + 2c + e; m is the same in all lanes of a row, l a lane's own part.
-    float m[kRowTiles][2], l[kRowTiles][2], less[kRowTiles][2];  // less: m - kLift, 0 before any score
+    // Of rows 8j + 2c + e, l a lane's own part, the others the same in all lanes of a row: at what
+    // score the reference m moves, m + kSlack, and what weights are relative to, m - kLift.
+    float moves[kRowTiles][2], l[kRowTiles][2], less[kRowTiles][2];
     float mz[kQuantised ? kRowTiles : 1][2], lz[kQuantised ? kRowTiles : 1][2];  // of V rows with a scale of 0
 #pragma unroll
     for (int j = 0; j < kRowTiles; ++j)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        m[j][e] = -INFINITY;
+        moves[j][e] = -INFINITY;
         l[j][e] = 0.0f;
         less[j][e] = 0.0f;
         if constexpr (kQuantised) {
@@ -408,16 +427,15 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
       if (there == 0) continue;
 
       float s[kRowTiles][4];  // tokens g / g + 8, rows 2c, 2c + 1
-#pragma unroll
-      for (int j = 0; j < kRowTiles; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[j][e] = 0.0f;
       // Matrices: tokens 0-7 and 8-15 of one 16-byte column, then of the next.
       const unsigned k_at = rows_at + (lane & 15) * Shape::pitch + (lane >> 4) * 16;
       auto times_q = [&](int k, const uint32_t(&x)[4]) {
         if constexpr (Shape::hold_q) {
 #pragma unroll
-          for (int j = 0; j < kRowTiles; ++j) mma<kBf16>(s[j], x, q[k][j][0], q[k][j][1]);
+          for (int j = 0; j < kRowTiles; ++j) {
+            if (k == 0) mma_first<kBf16>(s[j], x, q[k][j][0], q[k][j][1]);
+            else mma<kBf16>(s[j], x, q[k][j][0], q[k][j][1]);
+          }
         } else {
           // Two row tiles to an ldmatrix: rows 0-7 and 8-15, each k 0-7 and 8-15.
 #pragma unroll
@@ -425,8 +443,13 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
             uint32_t r[4];
             ldmatrix4(r, shared_at(q_rows) + (8 * j + (lane & 7) + ((lane >> 4) << 3)) * Shape::q_pitch +
                              ((lane >> 3) & 1) * 16 + k * 32);
-            mma<kBf16>(s[j], x, r[0], r[1]);
-            mma<kBf16>(s[j + 1], x, r[2], r[3]);
+            if (k == 0) {
+              mma_first<kBf16>(s[j], x, r[0], r[1]);
+              mma_first<kBf16>(s[j + 1], x, r[2], r[3]);
+            } else {
+              mma<kBf16>(s[j], x, r[0], r[1]);
+              mma<kBf16>(s[j + 1], x, r[2], r[3]);
+            }
           }
         }
       };
@@ -523,7 +546,7 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float t = fmaxf(s[j][e], s[j][2 + e]);
-          rises = rises || t > m[j][e] + kSlack;
+          rises = rises || t > moves[j][e];
           top[j][e] = t;
         }
       if (__any_sync(0xffffffffu, rises)) {
@@ -533,9 +556,9 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
           for (int e = 0; e < 2; ++e) {
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) top[j][e] = fmaxf(top[j][e], __shfl_xor_sync(0xffffffffu, top[j][e], d));
-            const float to = fmaxf(m[j][e], top[j][e]);
-            const float shrink = to == -INFINITY ? 1.0f : exp2_fast(m[j][e] - to);
-            m[j][e] = to;
+            const float from = moves[j][e] - kSlack, to = fmaxf(from, top[j][e]);
+            const float shrink = to == -INFINITY ? 1.0f : exp2_fast(from - to);
+            moves[j][e] = to + kSlack;
             less[j][e] = to == -INFINITY ? 0.0f : to - kLift;
             l[j][e] *= shrink;
 #pragma unroll
@@ -633,7 +656,7 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int row = warp * kRows + 8 * j + 2 * c + e;
-        float4 st = make_float4(m[j][e] - kLift, l[j][e], -INFINITY, 0.0f);
+        float4 st = make_float4(moves[j][e] == -INFINITY ? -INFINITY : less[j][e], l[j][e], -INFINITY, 0.0f);
         if constexpr (kQuantised) {
           st.z = mz[j][e];
           st.w = lz[j][e];

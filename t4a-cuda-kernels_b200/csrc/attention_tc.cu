@@ -10,8 +10,8 @@ template <int Kind, int Dim>
 int launch_one_tc(const AttendArgs& a, cudaStream_t stream) {
   static std::atomic<unsigned long long> allowed{0};
   T4A_TRY(runtime::allow_shared(k_attend_tc<Kind, Dim>, TcShape<Dim>::shared, &allowed));
-  k_attend_tc<Kind, Dim><<<a.groups * a.row_tiles, TcRoles<KindOf<Kind>::quantised>::threads, TcShape<Dim>::shared, stream>>>(a);
-  return runtime::check_launch();
+  return runtime::launch_early<AttendArgs>(k_attend_tc<Kind, Dim>, a.groups * a.row_tiles,
+                                           TcRoles<KindOf<Kind>::quantised>::threads, TcShape<Dim>::shared, stream, a);
 }
 
 template <int Kind>

@@ -315,7 +315,6 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int dim = a.cache.dim;
 
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x < kTile) {
     ones[threadIdx.x] = 1.0f;
     zeros[threadIdx.x] = 0.0f;
@@ -348,6 +347,8 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
   if (dim < Dim)
     for (int i = threadIdx.x; i < Shape::slots_at / 16; i += Roles::threads)
       reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   Cursor at = find_start(a, blockIdx.x);
   tc_before();
   fence_async();

@@ -257,8 +257,12 @@ extern "C" int t4a_tree_attention(void* stream, int dtype, const t4a_kv_cache* c
   a.pairs = rows_aligned(q, *q_layout, 2, 4) && rows_aligned(out, *out_layout, 2, 4);
   const Pages &k = a.cache.k, &v = a.cache.v;
   const long long last = (a.cache.pages - 1) * k.page + (a.cache.page_size - 1ll) * k.place + a.cache.dim * 2;
+  auto small_scales = [&](const Pages& p) {
+    return p.scale_page >= 0 && p.scale_place >= 0 &&
+           (a.cache.pages - 1) * p.scale_page + (a.cache.page_size - 1ll) * p.scale_place <= INT_MAX;
+  };
   a.plain_copies = k.page == v.page && k.place == v.place && k.page >= 0 && k.place >= 0 &&
-                   a.cache.dim == choice.padded && last / 16 < 0xffffffffll;
+                   a.cache.dim == choice.padded && last / 16 < 0xffffffffll && small_scales(k) && small_scales(v);
   a.table = table + table_layout->offset;
   a.table_page = table_layout->strides[0];
   a.table_batch = table_layout->strides[1];
@@ -270,23 +274,10 @@ extern "C" int t4a_tree_attention(void* stream, int dtype, const t4a_kv_cache* c
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   T4A_TRY(dispatch(cache->kind, a, choice, s, nullptr));
 
-  cudaLaunchConfig_t config = {};
   // At most so many parts to a unit where all are as long as each other.
   const long long rows = static_cast<long long>(a.batch) * a.cache.heads * a.rows;
   const bool few = a.groups <= 6ll * a.batch * a.cache.heads;
-  config.gridDim = dim3(static_cast<unsigned>(few ? (rows + kJoinWarps - 1) / kJoinWarps : rows));
-  config.blockDim = dim3(kJoinThreads);
-  config.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = attr;
-  config.numAttrs = 1;
-  const cudaError_t err = few ? cudaLaunchKernelEx(&config, k_join<1>, a) : cudaLaunchKernelEx(&config, k_join<kJoinWarps>, a);
-  if (err != cudaSuccess) {
-    runtime::last_error() = static_cast<int>(err);
-    cudaGetLastError();
-    return T4A_ERR_CUDA;
-  }
-  return T4A_OK;
+  return runtime::launch_early<AttendArgs>(few ? k_join<1> : k_join<kJoinWarps>,
+                                           static_cast<unsigned>(few ? (rows + kJoinWarps - 1) / kJoinWarps : rows),
+                                           kJoinThreads, 0, s, a);
 }

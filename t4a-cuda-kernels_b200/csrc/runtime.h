@@ -41,5 +41,29 @@ int allow_shared(Kernel kernel, int bytes, std::atomic<unsigned long long>* done
   return T4A_OK;
 }
 
+// Launches a kernel that may be set up while the stream's previous one ends; it waits for that one
+// (griddepcontrol.wait) before it touches memory.
+template <typename Args>
+int launch_early(void (*kernel)(Args), unsigned grid, unsigned block, size_t shared, cudaStream_t stream,
+                 const Args& args) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(grid);
+  config.blockDim = dim3(block);
+  config.dynamicSmemBytes = shared;
+  config.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attr;
+  config.numAttrs = 1;
+  const cudaError_t err = cudaLaunchKernelEx(&config, kernel, args);
+  if (err != cudaSuccess) {
+    last_error() = static_cast<int>(err);
+    cudaGetLastError();
+    return T4A_ERR_CUDA;
+  }
+  return T4A_OK;
+}
+
 }  // namespace runtime
 }  // namespace t4a
