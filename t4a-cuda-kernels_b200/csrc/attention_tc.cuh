@@ -65,8 +65,8 @@ struct alignas(16) TcNeutral {
 };
 
 struct TcBarriers {
-  unsigned long long q_full, k_full[kTcStages], k_empty[kTcStages], v_full[kTcStages], v_empty[kTcStages], s_full[2],
-      p_full[2], o_done[2], slot_full[kTcSlots];
+  unsigned long long q_full, k_full[kTcStages], k_empty[kTcStages], v_full[kTcStages], v_empty[kTcStages],
+      s_full[kTcSlots], p_full[2], o_done[2];
 };
 
 // Threads of the roles and their registers: equal at launch, then moved between the roles.  Codes
@@ -329,11 +329,12 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
     }
     // Two of each, in turn: a fast thread is at most one tile ahead of a slow one.
     for (int i = 0; i < 2; ++i) {
-      barrier_init(&bar->s_full[i], 1);
       barrier_init(&bar->p_full[i], kTcRows);
       barrier_init(&bar->o_done[i], 1);
     }
-    for (int i = 0; i < kTcSlots; ++i) barrier_init(&bar->slot_full[i], Roles::side_warps);
+    // A tile's products and what K's warps say of its tokens: one wait for both.  A slot comes round
+    // again only when its tile is through.
+    for (int i = 0; i < kTcSlots; ++i) barrier_init(&bar->s_full[i], 1 + Roles::side_warps);
     *failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -471,7 +472,7 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
           }
         }
         __syncwarp();
-        if (lane == 0) barrier_arrive(&bar->slot_full[t % kTcSlots]);
+        if (lane == 0) barrier_arrive(&bar->s_full[t % kTcSlots]);
       };
       look_up();
       step();
@@ -584,7 +585,7 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
               tc_mma(tmem + (t & 1) * 64, operand(q_at + (k >> 2) * kTcRows * 128 + (k & 3) * 32, 16, 1024),
                      operand(k_at + (k >> 2) * kTile * 128 + (k & 3) * 32, 16, 1024), form_s, k > 0);
             tc_commit(&bar->k_empty[stage]);
-            tc_commit(&bar->s_full[t & 1]);
+            tc_commit(&bar->s_full[t % kTcSlots]);
           }
           if (i > 0) {
             const int t = tiles_done + i - 1, stage = t % kTcStages;
@@ -706,9 +707,8 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
       for (int i = 0; i < n && good; ++i) {
         const int t = tiles_done + i;
         // Warps without a live row only keep step.
-        good = any_here ? barrier_wait(&bar->slot_full[t % kTcSlots], (t / kTcSlots) & 1, failed) &&
-                              barrier_wait(&bar->s_full[t & 1], (t >> 1) & 1, failed)
-                        : barrier_wait<true>(&bar->s_full[t & 1], (t >> 1) & 1, failed);
+        good = any_here ? barrier_wait(&bar->s_full[t % kTcSlots], (t / kTcSlots) & 1, failed)
+                        : barrier_wait<true>(&bar->s_full[t % kTcSlots], (t / kTcSlots) & 1, failed);
         if (!good) break;
         tc_after();
         if (any_here) {
