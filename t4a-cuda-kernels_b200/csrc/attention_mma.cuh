@@ -55,7 +55,9 @@ struct MmaShape {
   static constexpr int pitch = Dim * bytes + 16;  // an odd number of 16-byte units
   static constexpr int chunks = Dim * bytes / 16;
   static constexpr int stage = kTile * pitch * 2 + (KindOf<Kind>::quantised ? kTile * 8 : 0) + 16;
-  static constexpr int stages = 3;
+  // Codes: two stages and four blocks an SM, 75 us for 32 sequences of up to 8192 tokens where three
+  // and three took 80; 16-bit rows keep more bytes on their way in two blocks of three.
+  static constexpr int stages = bytes == 1 ? 2 : 3;
   static constexpr int q_pitch = Dim * 2 + 16;
   static constexpr int q_bytes = rows * q_pitch + 16;
   static constexpr int out_pitch = Dim + 4;  // floats: the lanes of a store meet 32 banks
@@ -286,12 +288,14 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
   constexpr int kSeen = kScales + (kQuantised ? kTile * 8 : 0);
 
   // The pads past dim meet zeros of Q, or make columns that are not stored; they only have to be
-  // finite, once.
-  if (dim < Dim) {
+  // finite, also after a unit's results have passed through the ring.
+  auto clear_pads = [&] {
+    if (dim == Dim) return;
     for (int i = threadIdx.x; i < Shape::ring / 16; i += kMmaThreads)
       reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-  }
+  };
+  clear_pads();
 
   while (at.left > 0) {
     const int b = at.b;
@@ -505,7 +509,7 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
         const int drafted = pos0 + t - context;
         if (drafted < 0) return true;
         const int node = (first_row + 8 * j + 2 * c + e) / a.group;
-        return node < live && node_sees(a, b, node, drafted);
+        return node < live && drafted < live && node_sees(a, b, node, drafted);
       };
       const bool partly = there != 0xffffu || pos0 + 16 > context;
       if (partly) {
@@ -717,7 +721,10 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
     }
     __syncthreads();
     at.left -= n;
-    if (at.left > 0) next_unit(a, &at);
+    if (at.left > 0) {
+      next_unit(a, &at);
+      clear_pads();
+    }
   }
 }
 

@@ -196,6 +196,11 @@ def test_attention(cuda, kind, dtype, batch, nodes, kv, group, dim, page, contex
     (30, 40, 4, 4, 96, 24, [900, 77, 2000]),
     (24, 64, 5, 8, 64, 32, [1500, 100]),
     (24, 7, 6, 6, 256, 16, [700, 1000]),
+    (64, 1, 8, 4, 80, 16, [700, 3, 1100, 64]),
+    (64, 2, 8, 6, 112, 32, [500, 300, 9]),
+    (64, 4, 8, 6, 48, 16, [400, 130]),
+    (48, 9, 6, 6, 80, 16, [400, 630]),
+    (32, 2, 8, 6, 208, 16, [400, 630]),
 ])
 def test_blocks_that_take_several_tiles_and_units(cuda, kind, dtype, batch, nodes, kv, group, dim, page, contexts):
     c = attention_case(batch, batch, nodes, kv, group, dim, page, contexts, kind, dtype)
