@@ -212,13 +212,13 @@ extern "C" int t4a_tree_attention(void* stream, int dtype, const t4a_kv_cache* c
   T4A_TRY(plan_attention(dtype, cache, q_layout, table_layout, true, &a, &choice, &empty));
   T4A_TRY(check_rows(q_layout, 4, q_len, 2));
   T4A_TRY(check_rows(out_layout, 4, out_len, 2));
-  T4A_TRY(plan::require_destination(*out_layout));
+  T4A_TRY(check_destination(*out_layout));
   for (int d = 0; d < 4; ++d)
     if (out_layout->extents[d] != q_layout->extents[d]) return T4A_ERR_SHAPE_MISMATCH;
   T4A_TRY(check_tensor(table_layout, 2, table_len, 4));
   if (lse != nullptr) {
     T4A_TRY(check_tensor(lse_layout, 3, lse_len, 4));
-    T4A_TRY(plan::require_destination(*lse_layout));
+    T4A_TRY(check_destination(*lse_layout));
     for (int d = 0; d < 3; ++d)
       if (lse_layout->extents[d] != q_layout->extents[d + 1]) return T4A_ERR_SHAPE_MISMATCH;
     if (!aligned(lse, 4)) return T4A_ERR_INVALID_STRIDE;

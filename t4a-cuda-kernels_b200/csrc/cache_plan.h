@@ -41,6 +41,13 @@ inline int check_rows(const t4a_cuda_layout* l, int rank, long long len, int ele
   return T4A_OK;
 }
 
+// A destination's elements are apart; one without elements is.
+inline int check_destination(const t4a_cuda_layout& l) {
+  for (int d = 0; d < l.rank; ++d)
+    if (l.extents[d] == 0) return T4A_OK;
+  return plan::require_destination(l);
+}
+
 // Whether the rows of `l` start on multiples of `bytes`.
 inline bool rows_aligned(const void* base, const t4a_cuda_layout& l, int element_bytes, unsigned bytes) {
   if (!aligned(static_cast<const char*>(base) + l.offset * element_bytes, bytes)) return false;
@@ -67,8 +74,8 @@ inline int check_side(int kind, void* base, float* scale, const t4a_cuda_layout&
                       const t4a_cuda_layout& sl, long long scale_len, bool written, bool pointers, Pages* out) {
   const int esize = element_size(kind);
   T4A_TRY(check_rows(&l, 4, len, esize));
-  if (written) T4A_TRY(plan::require_destination(l));
   if (l.extents[0] <= 0 || l.extents[0] % 16 != 0 || l.extents[0] > kMaxDim) return T4A_ERR_SHAPE_MISMATCH;
+  if (written) T4A_TRY(check_destination(l));
   long long count;
   T4A_TRY(plan::element_count(l, &count));
   if (pointers && count != 0 && base == nullptr) return T4A_ERR_NULL_ARGUMENT;
@@ -81,7 +88,7 @@ inline int check_side(int kind, void* base, float* scale, const t4a_cuda_layout&
   out->scale_head = out->scale_place = out->scale_page = 0;
   if (is_quantised(kind)) {
     T4A_TRY(check_tensor(&sl, 3, scale_len, 4));
-    if (written) T4A_TRY(plan::require_destination(sl));
+    if (written) T4A_TRY(check_destination(sl));
     for (int d = 0; d < 3; ++d)
       if (sl.extents[d] != l.extents[d + 1]) return T4A_ERR_SHAPE_MISMATCH;
     if (pointers && count != 0 && scale == nullptr) return T4A_ERR_NULL_ARGUMENT;

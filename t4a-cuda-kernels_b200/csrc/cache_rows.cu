@@ -386,7 +386,7 @@ int run_rows(void* stream, int dtype, int index_dtype, const t4a_kv_cache* cache
   bool vec = true;
   for (int side = 0; side < 2; ++side) {
     T4A_TRY(check_rows(layout[side], 3, len[side], esize));
-    if (!write) T4A_TRY(plan::require_destination(*layout[side]));
+    if (!write) T4A_TRY(check_destination(*layout[side]));
     if (layout[side]->extents[0] != a.cache.dim || layout[side]->extents[1] != a.cache.heads ||
         layout[side]->extents[2] != rows)
       return T4A_ERR_SHAPE_MISMATCH;
