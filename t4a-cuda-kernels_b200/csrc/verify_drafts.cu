@@ -65,6 +65,10 @@ __device__ __forceinline__ unsigned ordered(float x) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
+__device__ __forceinline__ float from_ordered(unsigned o) {
+  return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+
 // Lowest index first among equal values.
 __device__ __forceinline__ unsigned long long make_key(unsigned value, long long index) {
   return (static_cast<unsigned long long>(value) << 32) | (0xffffffffu - static_cast<unsigned>(index));
@@ -109,6 +113,7 @@ class Walk {
  public:
   static constexpr int kVec = 16 / sizeof(T);
   static constexpr int kBatch = 4;  // vectors of a thread in flight
+  static constexpr int kAhead = 4;  // children whose rows are prefetched
 
   __device__ Walk(const VerifyArgs& args, Shared& shared, unsigned char* kept)
       : a(args),
@@ -229,6 +234,17 @@ class Walk {
     }
     __syncthreads();
     const int children = sh.children;
+    // The rows that may come next, a 128-byte line a thread, into L2: one of them is wanted a few
+    // microseconds from now, when its way from memory would be the longest part of the wait.
+    const int line = tid * 128;
+    for (int c = 0; c < min(children, kAhead); ++c) {
+      const T* const ahead = static_cast<const T*>(a.logits) + static_cast<long long>(b) * a.logits_batch +
+                             static_cast<long long>(sh.child[c]) * a.logits_node;
+      for (int at_byte = line; at_byte < vectors * 16; at_byte += kThreads * 128) {
+        const long long i = static_cast<long long>(first) * kVec + at_byte / static_cast<int>(sizeof(T));
+        if (i < a.vocab) asm volatile("prefetch.global.L2 [%0];" ::"l"(ahead + i));
+      }
+    }
     for (int c = tid; c < children; c += kThreads) {
       const int token = sh.token[sh.child[c]];
       sh.child_x[c] = in_vocab(token) ? fix(static_cast<float>(row[token])) : -INFINITY;
@@ -299,18 +315,19 @@ class Walk {
     return r;
   }
 
+  // The warp's records as one, the same in all lanes: the sums are added in one order, and the value
+  // is lane 0's.
   static __device__ __forceinline__ Record across(Record r) {
+    const float m = from_ordered(__reduce_max_sync(0xffffffffu, ordered(r.m)));
+    r.s *= weight(r.m, m);
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) {
-      Record o;
-      o.m = __shfl_xor_sync(0xffffffffu, r.m, d);
-      o.s = __shfl_xor_sync(0xffffffffu, r.s, d);
-      o.key = __shfl_xor_sync(0xffffffffu, r.key, d);
-      r = joined(r, o);
-    }
-    // The two sides of a join may round apart; decisions need one value.
-    r.m = __shfl_sync(0xffffffffu, r.m, 0);
+    for (int d = 16; d > 0; d >>= 1) r.s += __shfl_xor_sync(0xffffffffu, r.s, d);
     r.s = __shfl_sync(0xffffffffu, r.s, 0);
+    r.m = m;
+    const unsigned high = __reduce_max_sync(0xffffffffu, static_cast<unsigned>(r.key >> 32));
+    const unsigned low = __reduce_max_sync(
+        0xffffffffu, static_cast<unsigned>(r.key >> 32) == high ? static_cast<unsigned>(r.key) : 0u);
+    r.key = static_cast<unsigned long long>(high) << 32 | low;
     return r;
   }
 

@@ -55,9 +55,9 @@ def native():
 
 
 def _call(name, stream, *args):
-    function = getattr(_native or native(), name)
     if stream is None:
-        return function(*args)
+        return getattr(_native or native(), name)(*args)
+    function = getattr(native(), name)
     import torch
     with torch.cuda.stream(stream):
         return function(*args)
