@@ -102,9 +102,13 @@ struct Choice {
   int padded, row_tiles, rows;  // row_tiles 0: the tensor-memory kernel
 };
 
-// Up to 32 rows a head: warp-level products over tiles of 8 rows, as few as hold them (2 at most for
-// a dim over 128, whose outputs would not fit the registers).  More rows: 128 in tensor memory; a
-// dim over 128 does not fit there beside a second block.
+// The kernel by the query rows of a cache head.  Warp-level products over tiles of 8 rows, as few as
+// hold them (2 at most for a dim over 128, whose outputs would not fit the registers), or 128 rows
+// in tensor memory, where a dim over 128 does not fit beside a second block.  Measured at 16 ragged
+// sequences of up to 4096 tokens, 8 cache heads, dim 128, a call warp-level against one in tensor
+// memory: 16-bit cache, 16 rows 53 against 54 us, 32 rows 73 against 55; int8, 16 rows 49 against 70,
+// 32 rows 69 against 72, 48 rows 114 against 77; E4M3, 32 rows 74 against 85, 48 rows 120 against 90.
+// At 131072 tokens in int8 and 32 rows: 119 against 166.
 Choice choose(int kind, int dim, int rows) {
   Choice c;
   c.padded = dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : 256;

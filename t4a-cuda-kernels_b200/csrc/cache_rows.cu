@@ -5,9 +5,12 @@
 // tree over the group, and its codes leave as one 16-byte store a thread.
 //   write: a = max |x|, scale = a * (1/Q), code = nearest(x * (Q/a))
 //   read:  x = code * scale
-// Both are bound by memory: a written row costs dim * (source + code) + 4 bytes, and no
-// arithmetic comes near that (some 3 instructions a value against the 16 that the SMs issue in
-// the time a value's bytes take).
+// A thread has the same part of a K row and of a V row: both loads are under way before the first
+// is used, and the slot's page and place are found once (60 -> 49 us for the reads below).
+// Both are bound by memory.  32768 rows of 8 heads x 128 from BF16 to E4M3, 203 MB: 39 us, 5.2 TB/s,
+// 0.79 of a copy's rate (its arithmetic takes 0.72 of the issue slots; magnitudes compared as bits
+// in packed pairs and integers rounded by an addition brought it from 57 us).  50001 such rows back
+// to BF16, 311 MB: 48 us, 6.4 TB/s, 0.98.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>

@@ -15,7 +15,11 @@
 //   With a draft each child turned down costs one pass, r <- max(r - q, 0), and an exchange.  The
 //   next child's r is a scalar recursion from the masses, which every block does for itself.
 // Bound by latency: a node is a dependent load of its row, a pass over some 32 values a thread and
-// a cluster barrier.  The race's row, wanted last, is prefetched into L2 at the start.
+// a cluster barrier, some 4 us together; sequences run beside each other.  The race's row, wanted
+// last, is prefetched into L2 at the start, the children's rows when their parent is read.  32
+// trees of 32 nodes over a vocabulary of 128256 in BF16, 4 nodes a path: 28 us, 37 MB of rows that
+// are needed (two exchanges a node, a sum and a maximum apart, took 52).  4 chains of 5 over 32003
+// with a draft: 19 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
