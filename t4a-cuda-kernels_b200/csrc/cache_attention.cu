@@ -160,7 +160,7 @@ int plan_attention(int dtype, const t4a_kv_cache* cache, const t4a_cuda_layout* 
   const long long places = table->extents[0] > most_places / a->cache.page_size
                                ? most_places
                                : table->extents[0] * a->cache.page_size;
-  a->places = static_cast<int>(places);
+  a->places = a->cache.pages == 0 ? 0 : static_cast<int>(places);
   a->tile_pages = kTile / a->cache.page_size;
   a->tile_places = kTile % a->cache.page_size;
   *choice = choose(cache->kind, a->cache.dim, a->rows);

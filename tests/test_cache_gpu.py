@@ -180,6 +180,8 @@ KINDS = [(BF16, BF16), (F16, F16), (I8, BF16), (I8, F16), (E4M3, BF16), (E4M3, F
     (2, 64, 1, 8, 128, 64, [1000, 333]),
     (1, 9, 1, 16, 64, 128, [5000]),
     (1, 3, 2, 40, 32, 16, [77]),
+    (2, 200, 1, 4, 128, 16, [300, 40]),
+    (1, 150, 1, 2, 256, 16, [200]),
 ])
 def test_attention(cuda, kind, dtype, batch, nodes, kv, group, dim, page, contexts):
     c = attention_case(batch * 100 + nodes, batch, nodes, kv, group, dim, page, contexts, kind, dtype)
@@ -277,6 +279,106 @@ def test_attention_over_strided_tensors(cuda, kind, dtype):
     lse = torch.zeros(6, 6, 3, device="cuda").permute(2, 1, 0)
     got = check_attention(c, out=out, lse=lse)
     assert got[0] is out and got[1] is lse
+
+
+def test_more_row_tiles_than_blocks(cuda):
+    """300 tiles of query rows: every one passes over the whole cache by itself."""
+    check_attention(attention_case(16, 1, 300, 1, 128, 64, 64, [90], I8, BF16))
+
+
+def test_an_empty_cache(cuda):
+    k, v = (torch.zeros(0, 16, 2, 64, dtype=F16, device="cuda") for _ in range(2))
+    table = torch.zeros(2, 3, dtype=torch.int32, device="cuda")
+    out, lse = t4.tree_attention(torch.ones(2, 3, 4, 64, dtype=F16, device="cuda"), k, v, table,
+                                 torch.full((2,), 20, dtype=torch.int32, device="cuda"))
+    assert (out == 0).all() and (lse == -math.inf).all()
+    slots = torch.tensor([0, -1, 5], device="cuda")
+    rows = torch.ones(3, 2, 64, dtype=F16, device="cuda")
+    t4.cache_write(rows, rows, k, v, slots)
+    assert all((x == 0).all() for x in t4.cache_read(k, v, slots, F32))
+
+
+def test_calls_in_a_graph(cuda):
+    """A captured step gives what the calls give, on new contents of the same tensors too."""
+    gen = generator(17)
+    c = attention_case(18, 3, 5, 2, 4, 64, 16, [90, 40, 200], E4M3, F16)
+    key, value = (torch.randn(15, 2, 64, generator=gen, device="cuda").to(F16) for _ in range(2))
+    places = c["context"][:, None].long() + torch.arange(5, device="cuda")
+    slots = (c["table"].long().gather(1, places // 16) * 16 + places % 16).flatten()
+    logits = torch.randn(3, 5, 3000, generator=gen, device="cuda")
+    tokens = torch.randint(0, 3000, (3, 5), generator=gen, device="cuda", dtype=torch.int32)
+    parents = torch.tensor([[-1, 0, 0, 1, 2]] * 3, dtype=torch.int32, device="cuda")
+    uniforms = torch.rand(3, 5, generator=gen, device="cuda")
+    race = torch.empty(3, 3000, device="cuda").exponential_(generator=gen).reciprocal_()
+
+    def step():
+        t4.cache_write(key, value, c["k"], c["v"], slots, k_scale=c["ks"], v_scale=c["vs"])
+        got = t4.tree_attention(c["q"], c["k"], c["v"], c["table"], c["context"], mask=c["sees"], k_scale=c["ks"],
+                                v_scale=c["vs"])
+        return got + t4.verify_drafts(logits, tokens, parents, uniforms=uniforms, race=race)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for _ in range(2):
+        key.normal_(generator=gen)
+        c["q"].normal_(generator=gen)
+        logits.normal_(generator=gen)
+        want = [t.clone() for t in step()]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want))
+
+
+def test_refusals_from_python(cuda):
+    c = attention_case(19, 2, 3, 2, 2, 64, 16, [30, 7], I8, F16)
+    scales = dict(k_scale=c["ks"], v_scale=c["vs"])
+    rows = torch.zeros(4, 2, 64, dtype=F16, device="cuda")
+    slots = torch.arange(4, device="cuda")
+
+    def attend(q=c["q"], k=c["k"], table=c["table"], context=c["context"], **more):
+        return t4.tree_attention(q, k, c["v"], table, context, **{**scales, **more})
+
+    with pytest.raises(TypeError):
+        t4.cache_write(rows.double(), rows.double(), c["k"], c["v"], slots, **scales)
+    with pytest.raises(TypeError):
+        t4.cache_write(rows, rows.float(), c["k"], c["v"], slots, **scales)
+    with pytest.raises(TypeError):
+        t4.cache_write(rows, rows, c["k"], c["v"], slots.float(), **scales)
+    with pytest.raises(TypeError):
+        t4.cache_read(c["k"], c["v"], slots, torch.float64, **scales)
+    with pytest.raises(ValueError):
+        t4.cache_write(rows, rows, c["k"], c["v"], slots)  # no scales
+    with pytest.raises(ValueError):
+        t4.cache_write(rows, rows, c["k"], c["v"], slots.cpu(), **scales)
+    with pytest.raises(ValueError):
+        t4.cache_write(rows.cpu(), rows.cpu(), c["k"], c["v"], slots, **scales)
+    with pytest.raises(t4.T4AError) as refused:
+        t4.cache_write(rows[:, :1], rows[:, :1], c["k"], c["v"], slots, **scales)
+    assert refused.value.status == 16
+    with pytest.raises(TypeError):
+        attend(q=c["q"].float())
+    with pytest.raises(ValueError):
+        attend(q=c["q"][0])
+    with pytest.raises(TypeError):
+        attend(table=c["table"].long())
+    with pytest.raises(ValueError):
+        attend(context=c["context"][:1])
+    with pytest.raises(TypeError):
+        attend(k=c["k"].view(torch.uint8))
+    with pytest.raises(t4.T4AError):
+        attend(workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))
+    need = t4.tree_attention_workspace_bytes(c["q"], c["k"], c["v"], c["table"], **scales)
+    first, second = attend(), attend(workspace=torch.empty(need, dtype=torch.uint8, device="cuda"))
+    assert torch.equal(first[0], second[0])
+    with pytest.raises(ValueError):
+        t4.verify_drafts(torch.zeros(2, 3, 9, device="cuda"), torch.zeros(2, 4, dtype=torch.int32, device="cuda"),
+                         torch.zeros(2, 3, dtype=torch.int32, device="cuda"), temperature=0.0)
+    with pytest.raises(t4.T4AError):
+        t4.verify_drafts(torch.zeros(2, 3, 9, device="cuda"), torch.zeros(2, 3, dtype=torch.int32, device="cuda"),
+                         torch.zeros(2, 3, dtype=torch.int32, device="cuda"))  # no uniforms
 
 
 def test_pages_outside_the_cache_are_not_seen(cuda):
