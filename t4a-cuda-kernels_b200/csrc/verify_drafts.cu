@@ -13,13 +13,15 @@
 //   would cancel when a likely token is turned down.  So a node costs one exchange, whatever the
 //   number of its children.
 //   With a draft each child turned down costs one pass, r <- max(r - q, 0), and an exchange.  The
-//   next child's r is a scalar recursion from the masses, which every block does for itself.
+//   next child's r is a scalar recursion from the masses, which every block does for itself.  r
+//   takes the logits' place in shared memory: beside them it takes 0.7 us off 4 chains of 5, and
+//   half of the longest F32 row.
 // Bound by latency: a node is a dependent load of its row, a pass over some 32 values a thread and
 // a cluster barrier, some 4 us together; sequences run beside each other.  The race's row, wanted
 // last, is prefetched into L2 at the start, the children's rows when their parent is read.  32
 // trees of 32 nodes over a vocabulary of 128256 in BF16, 4 nodes a path: 28 us, 37 MB of rows that
 // are needed (two exchanges a node, a sum and a maximum apart, took 52).  4 chains of 5 over 32003
-// with a draft: 19 us.
+// with a draft: 20 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -37,7 +39,7 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMostCluster = 8;
 constexpr int kMostNodes = 1024;
-constexpr int kMostBytes = 188416;  // of a block's slice: the logits, and with a draft r in F32
+constexpr int kMostBytes = 188416;  // of a block's slice: the logits, or with a draft r in F32
 
 struct VerifyArgs {
   const void* logits;
@@ -123,7 +125,6 @@ class Walk {
       : a(args),
         sh(shared),
         held(reinterpret_cast<uint4*>(kept)),
-        left(reinterpret_cast<float*>(kept + static_cast<size_t>(args.slots) * 16)),
         rank(cluster_rank()),
         blocks(cluster_blocks()),
         b(blockIdx.x / cluster_blocks()) {}
@@ -171,8 +172,9 @@ class Walk {
  private:
   const VerifyArgs& a;
   Shared& sh;
-  uint4* const held;  // [slots]: this block's vectors of the row
-  float* const left;  // [kVec][slots], with a draft: element e of vector j at e * slots + j, lanes side by side
+  // [slots]: this block's vectors of the row.  With a draft [kVec / 4][slots]: r in F32 takes their
+  // place, its elements 4 h to 4 h + 3 of vector j at h * slots + j, lanes side by side.
+  uint4* const held;
   const unsigned rank, blocks;
   const int b;
   int turn = 0;  // exchanges so far
@@ -425,8 +427,9 @@ class Walk {
         if (threadIdx.x == 0) sh.mass[masses] = mass;
         ++masses;
         __syncthreads();
-      } else {  // nothing is left: the node's softmax again
+      } else {  // nothing is left: the node's softmax again, from its logits
         masses = passes = 0;
+        for (int j = threadIdx.x; j < vectors; j += kThreads) held[j] = load_vector(j);
       }
     }
     return -1;
@@ -453,8 +456,15 @@ class Walk {
   // r of this thread's vector j; `again`: after a pass, else from the logits.
   __device__ __forceinline__ void residual(int j, const Record& all, bool again, float (&r)[kVec]) const {
     if (again) {
+      const float4* const left = reinterpret_cast<const float4*>(held) + j;
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) r[e] = left[e * a.slots + j] * factor;
+      for (int h = 0; h < kVec / 4; ++h) {
+        const float4 x = left[h * a.slots];
+        r[4 * h] = x.x * factor;
+        r[4 * h + 1] = x.y * factor;
+        r[4 * h + 2] = x.z * factor;
+        r[4 * h + 3] = x.w * factor;
+      }
     } else {
       const uint4 v = held[j];
       const T* const h = reinterpret_cast<const T*>(&v);
@@ -464,7 +474,7 @@ class Walk {
     }
   }
 
-  // left <- max(r - q, 0); the thread's sum of it.
+  // r <- max(r - q, 0); the thread's sum of it.
   __device__ float subtract(const float* q, const Record& all, bool again) {
     float s = 0.0f;
     for (int j = threadIdx.x; j < vectors; j += kThreads) {
@@ -474,10 +484,13 @@ class Walk {
       residual(j, all, again, r);
 #pragma unroll
       for (int e = 0; e < kVec; ++e) {
-        const float x = fmaxf(r[e] - v[e], 0.0f);
-        left[e * a.slots + j] = x;
-        s += x;
+        r[e] = fmaxf(r[e] - v[e], 0.0f);
+        s += r[e];
       }
+      float4* const left = reinterpret_cast<float4*>(held) + j;
+#pragma unroll
+      for (int h = 0; h < kVec / 4; ++h)
+        left[h * a.slots] = make_float4(r[4 * h], r[4 * h + 1], r[4 * h + 2], r[4 * h + 3]);
     }
     return s;
   }
@@ -570,7 +583,7 @@ int launch_mode(const VerifyArgs& a, bool greedy, int batch, int blocks, cudaStr
   const size_t logits = static_cast<size_t>(a.slots) * 16, r = static_cast<size_t>(a.slots) * (16 / sizeof(T)) * 4;
   if (greedy) return launch_verify<T, kGreedy>(a, batch, blocks, logits, stream);
   if (a.draft == nullptr) return launch_verify<T, kPlain>(a, batch, blocks, logits, stream);
-  return launch_verify<T, kDraft>(a, batch, blocks, logits + r, stream);
+  return launch_verify<T, kDraft>(a, batch, blocks, r, stream);
 }
 
 }  // namespace
@@ -636,7 +649,7 @@ extern "C" int t4a_verify_drafts(void* stream, int dtype, const void* logits, co
   while (blocks < kMostCluster && vocab >= blocks * 2 * 4096ll) blocks *= 2;
   const long long vectors = (vocab + 2 * vec - 2) / vec;  // at the worst skew
   const long long slots = (vectors + blocks - 1) / blocks;
-  const long long bytes = slots * (16 + (a.draft != nullptr ? vec * 4 : 0));
+  const long long bytes = slots * (a.draft != nullptr ? vec * 4 : 16);
   if (bytes > kMostBytes) return T4A_ERR_DOMAIN_TOO_LARGE;
   if (batch * blocks > 0x7fffffffll) return T4A_ERR_LAUNCH_LIMIT;
   a.slots = static_cast<int>(slots);

@@ -475,7 +475,7 @@ def check_walk(logits, tokens, parents, uniforms, draft, race, temperature):
 @pytest.mark.parametrize("with_draft", [False, True])
 @pytest.mark.parametrize("temperature", [0.0, 0.7, 1.0])
 @pytest.mark.parametrize("batch,nodes,vocab", [(1, 1, 1), (3, 2, 37), (2, 5, 1000), (4, 9, 8191), (3, 6, 8195),
-                                               (2, 12, 32003), (2, 4, 128256)])
+                                               (2, 12, 32003), (2, 4, 128256), (1, 3, 262144)])
 def test_verify(cuda, dtype, with_draft, temperature, batch, nodes, vocab):
     seed = vocab + nodes
     gen, rng = generator(seed), random.Random(seed)
@@ -537,6 +537,23 @@ def test_verify_of_a_row_with_no_probability(cuda):
                                                    uniforms=torch.zeros(1, 3, device="cuda"), race=ones)
         assert count.tolist() == [0] and path.tolist() == [[-1] * 3] and said.tolist() == [[0, -1, -1]]
         assert logs.tolist() == [[-math.inf, 0.0, 0.0]]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_verify_of_a_residual_with_nothing_left(cuda, dtype):
+    """The draft takes all that the target has: after each child turned down the node's softmax again."""
+    vocab = 20011
+    logits = torch.full((2, 4, vocab), -math.inf, device="cuda").to(dtype)
+    logits[0, :, 17001] = 3.0
+    logits[1, :, 5] = -2.0
+    logits[1, :, 19999] = -2.0
+    draft = torch.full((2, 4, vocab), 1 / 2, device="cuda")
+    draft[0, :, 17001] = 1.0
+    tokens = torch.tensor([[0, 4, 9, 17000], [0, 4, 5, 7]], dtype=torch.int32, device="cuda")
+    parents = torch.tensor([[-1, 0, 0, 0], [-1, 0, 0, 2]], dtype=torch.int32, device="cuda")
+    uniforms = torch.full((2, 4), 0.25, device="cuda")
+    race = torch.ones(2, vocab, device="cuda")
+    assert check_walk(logits, tokens, parents, uniforms, draft, race, 1.0).tolist() == [0, 1]
 
 
 def test_verify_of_strided_tensors(cuda):
