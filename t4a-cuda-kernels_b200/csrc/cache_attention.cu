@@ -98,6 +98,8 @@ __global__ void __launch_bounds__(kJoinThreads) k_join(const AttendArgs a) {
   if (lane == 0) store_lse(a, b, head, row, empty ? -INFINITY : less + log2f(sum));
 }
 
+constexpr int kManyTiles = 4096;
+
 struct Choice {
   int padded, row_tiles, rows;  // row_tiles 0: the tensor-memory kernel
 };
@@ -108,13 +110,20 @@ struct Choice {
 // sequences of up to 4096 tokens, 8 cache heads, dim 128, a call warp-level against one in tensor
 // memory: 16-bit cache, 16 rows 53 against 54 us, 32 rows 73 against 55; int8, 16 rows 49 against 70,
 // 32 rows 69 against 72, 48 rows 114 against 77; E4M3, 32 rows 74 against 85, 48 rows 120 against 90.
-// At 131072 tokens in int8 and 32 rows: 119 against 166.
-Choice choose(int kind, int dim, int rows) {
+// At 131072 tokens in int8 and 32 rows: 119 against 166.  What the warp-level kernel pays for a
+// unit, joining its warps' outputs, is most of a call whose blocks have a few tiles each, so 17 to 32
+// rows of codes go by the tiles of all tables, 8 heads, 32 rows, in E4M3 and in int8: 4 sequences of up
+// to 4096 (2048 tiles) 58 against 44 and 52 against 40, 7 of up to 4099 (3640) 64 against 56 and 58
+// against 50, 16 of 2048 (4096) 73 against 75 and 67 against 65, 16 of 4096 (8192) 97 against 120 and
+// 91 against 104.  (Not at dim 96, which tensor memory pads to 128: 7 of up to 4099 in E4M3 take 52
+// against 58; and 44 against 46 at dim 64.)
+Choice choose(int kind, int dim, int rows, long long tiles) {
   Choice c;
   c.padded = dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : 256;
   c.row_tiles = rows <= 8 ? 1 : rows <= 16 || c.padded == 256 ? 2 : 4;
   c.rows = 8 * c.row_tiles;
-  if (rows > (is_quantised(kind) ? 32 : 16) && c.padded <= 128) {
+  const bool warps = is_quantised(kind) && (c.padded < 128 || tiles >= kManyTiles);
+  if (rows > (warps ? 32 : 16) && c.padded <= 128) {
     c.padded = dim <= 64 ? 64 : 128;
     c.row_tiles = 0;
     c.rows = kTcTileRows;
@@ -163,14 +172,14 @@ int plan_attention(int dtype, const t4a_kv_cache* cache, const t4a_cuda_layout* 
   a->places = a->cache.pages == 0 ? 0 : static_cast<int>(places);
   a->tile_pages = kTile / a->cache.page_size;
   a->tile_places = kTile % a->cache.page_size;
-  *choice = choose(cache->kind, a->cache.dim, a->rows);
-  a->tile_rows = choice->rows;
-  a->row_tiles = (a->rows + choice->rows - 1) / choice->rows;
   // The line of tiles is counted in 32 bits.
   long long tiles = (places + kTile - 1) / kTile;
   for (long long by : {batch, static_cast<long long>(a->cache.heads)})
     if (plan::mul_overflows(tiles, by, &tiles)) return T4A_ERR_OVERFLOW;
   if (tiles > INT_MAX || batch * a->cache.heads * a->rows > INT_MAX) return T4A_ERR_DOMAIN_TOO_LARGE;
+  *choice = choose(cache->kind, a->cache.dim, a->rows, tiles);
+  a->tile_rows = choice->rows;
+  a->row_tiles = (a->rows + choice->rows - 1) / choice->rows;
   int blocks;
   T4A_TRY(dispatch(cache->kind, *a, *choice, nullptr, &blocks));
   a->groups = a->row_tiles < blocks ? blocks / a->row_tiles : 1;

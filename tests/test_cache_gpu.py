@@ -210,6 +210,25 @@ def test_blocks_that_take_several_tiles_and_units(cuda, kind, dtype, batch, node
     check_attention(c)
 
 
+@pytest.mark.parametrize("kind,dtype", [(I8, BF16), (I8, F16), (E4M3, BF16), (E4M3, F16)])
+@pytest.mark.parametrize("batch,nodes,kv,group,dim,page,contexts", [
+    (2, 3, 1, 8, 128, 16, [0, 40]),
+    (3, 5, 2, 6, 112, 24, [300, 0, 65]),
+    (24, 8, 8, 4, 128, 16, [600, 1200, 3, 128]),
+    (16, 7, 6, 3, 112, 32, [700, 64]),
+    (2, 4, 2, 8, 128, 64, [9000, 1]),
+])
+def test_attention_through_a_long_table(cuda, kind, dtype, batch, nodes, kv, group, dim, page, contexts):
+    """A table with room for some 200000 places, most of it beyond the sequences."""
+    c = attention_case(batch + 7, batch, nodes, kv, group, dim, page, contexts, kind, dtype)
+    poison_unused(c)
+    wide = torch.full((batch, 200000 // page + 1), -1, dtype=torch.int32, device="cuda")
+    if wide.shape[1] > c["table"].shape[1]:
+        wide[:, :c["table"].shape[1]] = c["table"]
+        c["table"] = wide
+    check_attention(c)
+
+
 @pytest.mark.parametrize("kind,dtype", KINDS)
 def test_attention_without_a_mask_is_a_chain(cuda, kind, dtype):
     check_attention(attention_case(3, 2, 6, 2, 4, 128, 16, [50, 300], kind, dtype, tree=False), mask=None)
