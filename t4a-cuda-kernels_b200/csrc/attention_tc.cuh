@@ -8,17 +8,19 @@
 //   O += P V    [128 x dim], P from tensor memory, V from shared memory as it lies (d fastest)
 // so a row's maximum and sum need no exchange between threads, and P never leaves the SM's tensor
 // memory.  Roles: four warps of softmax and results, four warps for 16-bit cache rows (eight for
-// codes), and one thread that issues the products.  S of the next tile is issued before P V of this
-// one, and two blocks share an SM (256 columns of tensor memory and some 105 KB of shared memory
-// each), so products run while exponentials are taken: an SM needs 512 cycles for a tile's products
-// and 512 for its 8192 exponentials.
-// A tile takes a block some 2100 cycles (16-bit) and its softmax bounds it, not a unit's rate:
-// TMEM loads and stores, the maximum, the exponentials and the barriers follow one another.  Two
-// threads to a row were slower (189 us for 168 below: they have to meet at every tile), and so
-// were packed F32 operations, whole tiles in registers, and K and V by the same warps (228).
-// 4 sequences of up to 16384 tokens, 512 rows a cache head, BF16, 99 GFLOP: 159 us, 625 TFLOP/s,
-// 0.38 of a library product's rate; tensor pipe 0.31, DRAM reads 203 MB, each cache row once.
-// 7 trees of 13 nodes over 4099 tokens, E4M3, 39 rows: 36 us, of which a block's five tiles are half;
+// codes), and a warp that issues the products from one elected thread.  S of the tile after the next
+// is issued behind P V of this one, and two blocks share an SM (256 columns of tensor memory and some
+// 105 KB of shared memory each), so products run while exponentials are taken: an SM needs 512 cycles
+// for a tile's products and 512 for its 8192 exponentials.
+// A tile takes a block some 2700 cycles (16-bit) and its softmax bounds it, not a unit's rate: the
+// barrier, the load, the maximum, the exponentials and the store follow one another, and a look at a
+// barrier takes 450 cycles even when it is through.  Hence the look ahead at the next scores.  With
+// the issuing thread by itself (`lane == 0`), each product and wait was serialised over the warp and
+// bound the tile: 170 us for the 155 of a call below; and halves of 32 tokens at a time took 159.
+// Packed F32 operations, and K and V by the same warps (228 for 168 then), were slower.
+// 4 sequences of up to 16384 tokens, 512 rows a cache head, BF16, 99 GFLOP: 146 us, 680 TFLOP/s,
+// 0.41 of a library product's rate; DRAM reads 203 MB, each cache row once.
+// 7 trees of 13 nodes over 4099 tokens, E4M3, 39 rows: 34 us, of which a block's five tiles are half;
 // there unpacking bounds a tile (some 4500 cycles).
 //
 // Shared rows of Q, K and V are 128-byte lines of 64 values, their 16-byte units XORed with the
@@ -84,7 +86,7 @@ struct TcRoles {
   static constexpr int loaders = Quantised ? 256 : 128;  // half of them K's rows, half V's
   static constexpr int threads = kTcSoftmax + loaders + 128;
   static constexpr int at_launch = Quantised ? 64 : 80;
-  static constexpr int softmax = Quantised ? 96 : 120, loader = Quantised ? 64 : 72, issue = Quantised ? 32 : 48;
+  static constexpr int softmax = Quantised ? 112 : 128, loader = Quantised ? 56 : 64, issue = Quantised ? 32 : 48;
   static_assert(kTcSoftmax * softmax + loaders * loader + 128 * issue == threads * at_launch,
                 "a larger sum would wait for good");
   static constexpr int side_warps = loaders / 64;         // of K, and of V
@@ -141,6 +143,24 @@ __device__ __forceinline__ bool barrier_wait(unsigned long long* b, unsigned par
   }
   *failed = 1;
   return false;
+}
+
+__device__ __forceinline__ bool barrier_test(unsigned long long* b, unsigned parity) {
+  unsigned ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(shared_at(b)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// One lane of a whole warp, always the same: the compiler then knows that a single thread issues what
+// follows, where after a test of the lane it serialises each product over the warp.
+__device__ __forceinline__ bool elected() {
+  unsigned one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
 }
 
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -572,42 +592,56 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
   } else if (warp >= kIssueWarp) {
     // ---- products ----
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Roles::issue));
-    if (warp == kIssueWarp && lane == 0) {
+    if (warp == kIssueWarp) {
       const unsigned form_s = tc_form<kBf16>(kTile, false), form_o = tc_form<kBf16>(Dim, true);
       const unsigned q_at = shared_at(q_lines);
+      // All lanes wait together (a lane by itself takes longer), one issues.
+      auto ready = [&](unsigned long long* b, unsigned parity) {
+        const bool all = __all_sync(0xffffffffu, barrier_wait(b, parity, failed));
+        __syncwarp();
+        fence_async();  // the rows were written by ordinary stores and copies
+        tc_after();
+        return all;
+      };
+      auto scores = [&](int t) {
+        const int stage = t % kTcStages;
+        const unsigned k_at = shared_at(k_lines(stage));
+#pragma unroll
+        for (int k = 0; k < Dim / 16; ++k)
+          tc_mma(tmem + (t & 1) * 64, operand(q_at + (k >> 2) * kTcRows * 128 + (k & 3) * 32, 16, 1024),
+                 operand(k_at + (k >> 2) * kTile * 128 + (k & 3) * 32, 16, 1024), form_s, k > 0);
+        tc_commit(&bar->k_empty[stage]);
+        tc_commit(&bar->s_full[t % kTcSlots]);
+      };
+      auto outputs = [&](int t) {
+        const int stage = t % kTcStages;
+        const unsigned v_at = shared_at(v_lines(stage));
+#pragma unroll
+        for (int k = 0; k < kTile / 16; ++k)
+          tc_mma_from(tmem_o, tmem + (t & 1) * 64 + k * 8, operand(v_at + k * 2048, kTile * 128, 1024), form_o);
+        tc_commit(&bar->v_empty[stage]);
+        tc_commit(&bar->o_done[t & 1]);
+      };
+      auto k_barrier = [&](int t) { return &bar->k_full[t % kTcStages]; };
+      auto stage_parity = [&](int t) { return static_cast<unsigned>((t / kTcStages) & 1); };
       bool good = true;
       unsigned unit = 0;
       while (at.left > 0 && good) {
-        const int n = min(at.left, at.tiles - at.tile);
-        good = barrier_wait(&bar->q_full, unit & 1, failed);
-        for (int i = 0; i <= n && good; ++i) {
-          if (i < n) {
-            const int t = tiles_done + i, stage = t % kTcStages;
-            good = barrier_wait(&bar->k_full[stage], (t / kTcStages) & 1, failed);
-            if (!good) break;
-            fence_async();  // the rows were written by ordinary stores and copies
-            tc_after();
-            const unsigned k_at = shared_at(k_lines(stage));
-#pragma unroll
-            for (int k = 0; k < Dim / 16; ++k)
-              tc_mma(tmem + (t & 1) * 64, operand(q_at + (k >> 2) * kTcRows * 128 + (k & 3) * 32, 16, 1024),
-                     operand(k_at + (k >> 2) * kTile * 128 + (k & 3) * 32, 16, 1024), form_s, k > 0);
-            tc_commit(&bar->k_empty[stage]);
-            tc_commit(&bar->s_full[t % kTcSlots]);
-          }
-          if (i > 0) {
-            const int t = tiles_done + i - 1, stage = t % kTcStages;
-            good = barrier_wait(&bar->v_full[stage], (t / kTcStages) & 1, failed) &&
-                   barrier_wait(&bar->p_full[t & 1], (t >> 1) & 1, failed);
-            if (!good) break;
-            fence_async();
-            tc_after();
-            const unsigned v_at = shared_at(v_lines(stage));
-#pragma unroll
-            for (int k = 0; k < kTile / 16; ++k)
-              tc_mma_from(tmem_o, tmem + (t & 1) * 64 + k * 8, operand(v_at + k * 2048, kTile * 128, 1024), form_o);
-            tc_commit(&bar->v_empty[stage]);
-            tc_commit(&bar->o_done[t & 1]);
+        const int n = min(at.left, at.tiles - at.tile), t0 = tiles_done;
+        good = ready(&bar->q_full, unit & 1) && ready(k_barrier(t0), stage_parity(t0));
+        if (good && elected()) scores(t0);
+        if (good && n > 1) {
+          good = ready(k_barrier(t0 + 1), stage_parity(t0 + 1));
+          if (good && elected()) scores(t0 + 1);
+        }
+        // P V of a tile, and the scores of the one after the next into the buffer that P leaves.
+        for (int i = 0; i < n && good; ++i) {
+          const int t = t0 + i;
+          good = ready(&bar->v_full[t % kTcStages], stage_parity(t)) && ready(&bar->p_full[t & 1], (t >> 1) & 1);
+          if (good && elected()) outputs(t);
+          if (good && i + 2 < n) {
+            good = ready(k_barrier(t + 2), stage_parity(t + 2));
+            if (good && elected()) scores(t + 2);
           }
         }
         tiles_done += n;
@@ -712,10 +746,12 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
       }
       float m = -INFINITY, less = -1e30f, mz = -INFINITY, lz = 0.0f;
       float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      bool ahead = false;  // the next tile's scores are known to be there
       for (int i = 0; i < n && good; ++i) {
         const int t = tiles_done + i;
         // Warps without a live row only keep step.
-        good = any_here ? barrier_wait(&bar->s_full[t % kTcSlots], (t / kTcSlots) & 1, failed)
+        good = any_here ? __all_sync(0xffffffffu, ahead) ||
+                              barrier_wait(&bar->s_full[t % kTcSlots], (t / kTcSlots) & 1, failed)
                         : barrier_wait<true>(&bar->s_full[t % kTcSlots], (t / kTcSlots) & 1, failed);
         if (!good) break;
         tc_after();
@@ -785,15 +821,18 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
             odd_lo = odd[0];
             odd_hi = odd[1];
           }
-          // By halves of 32 tokens, so that a thread needs few registers; P's first half overwrites
+          // Codes by halves of 32 tokens, since their loaders leave a thread few registers; P overwrites
           // scores that have been read.
+          constexpr int kSides = kQuantised ? 1 : 2;  // of 32 tokens at a time
 #pragma unroll 1
-          for (int half = 0; half < 2; ++half) {
-            uint32_t s[32];
-            tc_load(s, s_at + 32 * half);
+          for (int half = 0; half < 2; half += kSides) {
+            uint32_t s[kSides][32];
+#pragma unroll
+            for (int q = 0; q < kSides; ++q) tc_load(s[q], s_at + 32 * (half + q));
             tc_loaded();
-            if constexpr (kQuantised) scale_scores(s, ks + 32 * half, lv + 32 * half);
-            float top = highest(s);
+            if constexpr (kQuantised) scale_scores(s[0], ks + 32 * half, lv + 32 * half);
+            float top = highest(s[0]);
+            if constexpr (kSides == 2) top = fmaxf(top, highest(s[1]));
             if constexpr (!kQuantised) top *= now_factor;  // factors are not negative
             const bool rises = here && top > less + (kSlack + kLift);
             if (__any_sync(0xffffffffu, rises)) {
@@ -804,7 +843,7 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
                 less = top - kLift;
                 l4[0] *= shrink, l4[1] *= shrink, l4[2] *= shrink, l4[3] *= shrink;
               }
-              if (half == 1) {
+              if (kSides == 1 && half == 1) {
                 // The first half's weights go by the old reference.
                 uint32_t p[16];
                 tc_load16(p, s_at);
@@ -828,18 +867,18 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
                 tc_stored();
               }
             }
-            if (Kind != T4A_I8 && (half ? odd_hi : odd_lo) != 0 && good) {
+            if (Kind != T4A_I8 && (kSides == 2 ? odd_lo | odd_hi : half ? odd_hi : odd_lo) != 0 && good) {
               if (i > 0) good = barrier_wait(&bar->o_done[(t - 1) & 1], ((t - 1) >> 1) & 1, failed);
               tc_after();
 #pragma unroll 1
-              for (int j = 0; j < 32; ++j) {
-                if (!(((half ? odd_hi : odd_lo) >> j) & 1)) continue;
+              for (int j = 32 * half; j < 32 * (half + kSides); ++j) {
+                if (!(((j < 32 ? odd_lo : odd_hi) >> (j & 31)) & 1)) continue;
                 uint32_t score;
-                tc_load1(&score, s_at + 32 * half + j);
+                tc_load1(&score, s_at + j);
                 tc_loaded();
-                const bool sees = here && (((half ? see_hi : see_lo) >> j) & 1);
+                const bool sees = here && (((j < 32 ? see_lo : see_hi) >> (j & 31)) & 1);
                 const float w = exp2_fast(__uint_as_float(score) - less);
-                const int at_pos = pos0 + 32 * half + j;
+                const int at_pos = pos0 + j;
                 const int page = a.table[b * a.table_batch + (at_pos / a.cache.page_size) * a.table_page];
                 const unsigned char* const v_row = a.cache.v.base + at.head * a.cache.v.head + page * a.cache.v.page +
                                                    (at_pos % a.cache.page_size) * a.cache.v.place;
@@ -859,9 +898,16 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
                 tc_stored();
               }
             }
-            uint32_t p[16];
-            weights<kQuantised, kBf16>(s, p, kQuantised ? 1.0f : now_factor, less, slot.rv + 32 * half, l4);
-            tc_store16(s_at + 16 * half, p);
+            // A look at the next tile's scores, which are there by now as a rule: its answer takes a while.
+            // (Over codes they come later than that.)
+            if (!kQuantised)
+              ahead = i + 1 < n && barrier_test(&bar->s_full[(t + 1) % kTcSlots], ((t + 1) / kTcSlots) & 1);
+#pragma unroll
+            for (int q = 0; q < kSides; ++q) {
+              uint32_t p[16];
+              weights<kQuantised, kBf16>(s[q], p, kQuantised ? 1.0f : now_factor, less, slot.rv + 32 * (half + q), l4);
+              tc_store16(s_at + 16 * (half + q), p);
+            }
             tc_stored();
           }
           tc_before();
