@@ -9,6 +9,14 @@ namespace cache {
 
 constexpr int kSms = 148;
 
+// The most tiles of 8 query rows that the warp-level kernel takes at once; the rule's reasons are
+// where the kernel is chosen.
+constexpr int most_row_tiles(bool quantised, int padded) {
+  if (padded == 256) return 2;
+  if (quantised) return 4;
+  return padded == 128 ? 1 : 2;
+}
+
 // With `blocks`, only says how many blocks to launch: as many as the SMs hold at once.
 template <int Kind, int Dim, int kRowTiles>
 int launch_one(const AttendArgs& a, cudaStream_t stream, int* blocks) {
@@ -25,13 +33,13 @@ int launch_one(const AttendArgs& a, cudaStream_t stream, int* blocks) {
 
 template <int Kind, int Dim>
 int launch_rows_of(const AttendArgs& a, int row_tiles, cudaStream_t stream, int* blocks) {
-  switch (row_tiles) {
-    case 1: return launch_one<Kind, Dim, 1>(a, stream, blocks);
-    case 2: return launch_one<Kind, Dim, 2>(a, stream, blocks);
-    default:
-      if constexpr (Dim <= 128) return launch_one<Kind, Dim, 4>(a, stream, blocks);
-      else return T4A_ERR_UNSUPPORTED_OP;
-  }
+  constexpr int kMost = most_row_tiles(KindOf<Kind>::quantised, Dim);
+  if (row_tiles == 1) return launch_one<Kind, Dim, 1>(a, stream, blocks);
+  if constexpr (kMost >= 2)
+    if (row_tiles == 2) return launch_one<Kind, Dim, 2>(a, stream, blocks);
+  if constexpr (kMost >= 4)
+    if (row_tiles == 4) return launch_one<Kind, Dim, 4>(a, stream, blocks);
+  return T4A_ERR_UNSUPPORTED_OP;
 }
 
 template <int Kind>

@@ -108,8 +108,10 @@ struct Choice {
 // hold them (2 at most for a dim over 128, whose outputs would not fit the registers), or 128 rows
 // in tensor memory, where a dim over 128 does not fit beside a second block.  Measured at 16 ragged
 // sequences of up to 4096 tokens, 8 cache heads, dim 128, a call warp-level against one in tensor
-// memory: 16-bit cache, 16 rows 53 against 54 us, 32 rows 73 against 55; int8, 16 rows 49 against 70,
-// 32 rows 69 against 72, 48 rows 114 against 77; E4M3, 32 rows 74 against 85, 48 rows 120 against 90.
+// memory: 16-bit cache, 8 rows 44 against 50 us, 12 rows 51 against 50, 16 rows 53 against 50; dim 96, 16
+// rows 45 against 50, 24 rows 56 against 51; dim 64, 16 rows 34 against 39, 24 rows 43 against 40.  int8,
+// 16 rows 49 against 70, 32 rows 69 against 72, 48 rows 114 against 77; E4M3, 32 rows 74 against 85, 48
+// rows 120 against 87.
 // At 131072 tokens in int8 and 32 rows: 119 against 166.  What the warp-level kernel pays for a
 // unit, joining its warps' outputs, is most of a call whose blocks have a few tiles each, so 17 to 32
 // rows of codes go by the tiles of all tables, 8 heads, 32 rows, in E4M3 and in int8: 4 sequences of up
@@ -122,8 +124,9 @@ Choice choose(int kind, int dim, int rows, long long tiles) {
   c.padded = dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : 256;
   c.row_tiles = rows <= 8 ? 1 : rows <= 16 || c.padded == 256 ? 2 : 4;
   c.rows = 8 * c.row_tiles;
-  const bool warps = is_quantised(kind) && (c.padded < 128 || tiles >= kManyTiles);
-  if (rows > (warps ? 32 : 16) && c.padded <= 128) {
+  int most = 8 * most_row_tiles(is_quantised(kind), c.padded);
+  if (is_quantised(kind) && c.padded == 128 && tiles < kManyTiles) most = 16;
+  if (rows > most && c.padded <= 128) {
     c.padded = dim <= 64 ? 64 : 128;
     c.row_tiles = 0;
     c.rows = kTcTileRows;
