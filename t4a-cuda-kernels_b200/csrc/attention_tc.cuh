@@ -19,7 +19,8 @@
 // bound the tile: 170 us for the 155 of a call below; and halves of 32 tokens at a time took 159.
 // Packed F32 operations, and K and V by the same warps (228 for 168 then), were slower.
 // 4 sequences of up to 16384 tokens, 512 rows a cache head, BF16, 99 GFLOP: 146 us, 680 TFLOP/s,
-// 0.41 of a library product's rate; DRAM reads 203 MB, each cache row once.
+// 0.41 of a library product's rate; tensor pipe 0.34, DRAM reads 202 MB,
+// each cache row once.
 // 7 trees of 13 nodes over 4099 tokens, E4M3, 39 rows: 34 us, of which a block's five tiles are half;
 // there unpacking bounds a tile (some 4500 cycles).
 //
