@@ -321,6 +321,11 @@ __device__ __forceinline__ uint32_t scaled_pair(uint32_t pair, float x) {
   }
 }
 
+// Whether tile `tile` of a unit reaches past the context, so that some node may not see all of its
+// tokens.  The loader of V and the softmax both go by this: the one takes infinities and NaNs out of
+// such a tile's rows and writes the slot's `odd`, the other reads it.
+__device__ __forceinline__ bool holds_drafts(int tile, int context) { return (tile + 1) * kTile > context; }
+
 template <int Kind, int Dim>
 __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcShape<Dim>::per_sm) k_attend_tc(const AttendArgs a) {
   using Shape = TcShape<Dim>;
@@ -508,7 +513,7 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
       if constexpr (kQuantised) fetch();
       for (int i = 0; i < n; ++i) {
         const int t = tiles_done + i, stage = t % kTcStages;
-        const bool partly = (at.tile + i + 1) * kTile > context;
+        const bool drafts = holds_drafts(at.tile + i, context);
         good = barrier_wait<true>(&empty[stage], ((t / kTcStages) & 1) ^ 1, failed);
         if (!good) break;
         unsigned char* const to = lines(stage);
@@ -520,7 +525,7 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
 #pragma unroll
           for (int u = 0; u < kRounds; ++u) {
             uint32_t x[4] = {code[u].x, code[u].y, code[u].z, code[u].w}, h[8];
-            if (Kind == T4A_E4M3 && is_v && partly) {
+            if (Kind == T4A_E4M3 && is_v && drafts) {
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const uint32_t nan = __vcmpeq4(x[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
@@ -553,7 +558,7 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
               if (chunk < used) copy16(round_unit(to_shared, u), base + from + chunk * 16, (bits >> in) & 1);
             }
           }
-          if (is_v && partly) {
+          if (is_v && drafts) {
             asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll 1
             for (int u = 0; u < kRounds; ++u) {
@@ -570,12 +575,12 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
             }
           }
         }
-        if (Kind != T4A_I8 && is_v && partly) {
+        if (Kind != T4A_I8 && is_v && drafts) {
           odd = __reduce_or_sync(0xffffffffu, odd);
           if (lane == 0) slots[t % kTcSlots].odd[first_token / kTokens] = static_cast<Flags>(odd);
           __syncwarp();
         }
-        if (kQuantised || (is_v && partly)) {
+        if (kQuantised || (is_v && drafts)) {
           fence_async();
           barrier_arrive(&full[stage]);
         } else {
@@ -761,7 +766,8 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
           const int pos0 = (at.tile + i) * kTile;
           const unsigned s_at = tmem + (t & 1) * 64 + lanes;
           const unsigned there_lo = flags_of(slot.there)[0], there_hi = flags_of(slot.there)[1];
-          const bool partly = (there_lo & there_hi) != 0xffffffffu || pos0 + kTile > context;
+          const bool drafts = holds_drafts(at.tile + i, context);
+          const bool partly = (there_lo & there_hi) != 0xffffffffu || drafts;
           const unsigned zero_lo = kQuantised ? flags_of(slot.zero)[0] : 0u,
                          zero_hi = kQuantised ? flags_of(slot.zero)[1] : 0u;
           const bool rare = partly || (zero_lo | zero_hi) != 0 || (kQuantised && shifted);
@@ -815,12 +821,13 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
             ks = ones;
             lv = zeros;
           }
-          if (Kind != T4A_I8 && partly) {
-            // Whether something was cleaned out of V, for the rows that see it.
+          if (Kind != T4A_I8 && drafts) {
+            // Whether something was cleaned out of V, for the rows that see it: never of tokens that are
+            // not there, whose place in the table leads nowhere.
             good = barrier_wait(&bar->v_full[t % kTcStages], (t / kTcStages) & 1, failed);
             const volatile unsigned* const odd = flags_of(slot.odd);
-            odd_lo = odd[0];
-            odd_hi = odd[1];
+            odd_lo = good ? odd[0] & there_lo : 0;
+            odd_hi = good ? odd[1] & there_hi : 0;
           }
           // Codes by halves of 32 tokens, since their loaders leave a thread few registers; P overwrites
           // scores that have been read.
@@ -890,8 +897,8 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
                   tc_loaded();
 #pragma unroll
                   for (int e = 0; e < 16; ++e) {
-                    const float v = row_value<Kind>(v_row, d + e);
-                    if (sees && !(fabsf(v) < INFINITY)) o[e] = __float_as_uint(__uint_as_float(o[e]) + w * v);
+                    const float v = sees ? row_value<Kind>(v_row, d + e) : 0.0f;
+                    if (!(fabsf(v) < INFINITY)) o[e] = __float_as_uint(__uint_as_float(o[e]) + w * v);
                   }
                   __syncwarp();
                   tc_store16(tmem_o + lanes + d, o);

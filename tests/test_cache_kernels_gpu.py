@@ -1,0 +1,52 @@
+"""tree_attention at row counts that reach each of its kernels, in forms where they differ.
+
+With 2 cache heads: 6 query rows a cache head take the warp-level kernel for every cache, 24 the warp-level
+one or tensor memory by the cache's kind and dim, 40 and 136 tensor memory (one tile of rows, and two).  Bounds
+are those of check_attention.
+"""
+import math
+
+import pytest
+import torch
+
+from test_cache_gpu import BF16, E4M3, F16, I8, KINDS, attention_case, check_attention, poison_unused
+
+pytestmark = pytest.mark.gpu
+
+ROWS = [(3, 2), (12, 2), (20, 2), (34, 4)]  # nodes, query heads to a cache head
+
+
+def poison_pages(c, pages):
+    """Rows of these pages hold the worst that they could."""
+    for name in ("k", "v"):
+        if c[name].dtype in (F16, BF16):
+            c[name][pages] = math.nan
+        else:
+            c[name + "s"][pages] = math.nan
+            if c[name].dtype == E4M3:
+                c[name].view(torch.uint8)[pages] = 0x7f
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
+@pytest.mark.parametrize("nodes,group", ROWS)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_pages_outside_the_cache(cuda, kind, dtype, nodes, group, dim):
+    """Whole tiles of 64 places and parts of tiles, in the context, among the drafted rows and first of all."""
+    c = attention_case(nodes + dim, 3, nodes, 2, group, dim, 16, [700, 333, 90], kind, dtype)
+    poison_unused(c)
+    outside = {0: [4, 5, 6, 7, 9, 20, 41], 1: [0, 15, 16, 333 // 16], 2: [90 // 16]}
+    for b, pages in outside.items():
+        poison_pages(c, c["table"][b, pages].long())
+        for i, page in enumerate(pages):
+            c["table"][b, page] = [-1, c["k"].shape[0], 1 << 30, -(1 << 31)][i % 4]
+    check_attention(c)
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
+@pytest.mark.parametrize("nodes,group", ROWS)
+def test_a_cache_that_no_table_reaches(cuda, kind, dtype, nodes, group):
+    c = attention_case(nodes, 2, nodes, 2, group, 64, 16, [300, 17], kind, dtype)
+    poison_pages(c, slice(None))
+    c["table"][:] = -1
+    out, lse = check_attention(c)
+    assert (out == 0).all() and (lse == -math.inf).all()
