@@ -20,9 +20,10 @@
 // meets the codes then is relative to the largest weight * scale of its row, whatever the scales
 // are; l adds weight / scale.  Rows with a scale of 0 (or below 2^-107, which the writer does not
 // make) count in the softmax alone: they have a maximum and a sum of their own, joined at the end.
-// Q is F16 too, times one power of two for the block's rows that brings their largest magnitude into
-// [2^14, 2^15): 29 binades below it are exact, and what is lost further down is 2^-38 of the
-// largest row's scores.
+// Q is F16 too.  BF16 rows become it exactly from 2^-17 up and within 2^-25 below, so a row whose
+// largest magnitude is outside [1/4, 2^15) is first brought to [2^14, 2^15) by a power of two of its own,
+// which its scores are multiplied by again: a row keeps 23 bits of its largest, whatever the block's
+// other rows hold.  Rows without a live node are zeros.
 // 32 sequences of up to 8192 tokens in I8, 4 rows a cache head, 353 MB: 71 us, 5.0 TB/s, 0.77 of a
 // copy's rate; the issue slots are 0.59 taken, DRAM reads 364 MB.  8 nodes over 131072 tokens in
 // I8, 32 rows, 277 MB: 115 us; there the unpacking and 64 products to 16 tokens with two blocks an
@@ -63,7 +64,7 @@ struct MmaShape {
   // and three took 80; 16-bit rows keep more bytes on their way in two blocks of three.
   static constexpr int stages = bytes == 1 ? 2 : 3;
   static constexpr int q_pitch = Dim * 2 + 16;
-  static constexpr int q_bytes = rows * q_pitch + 16;
+  static constexpr int q_bytes = rows * q_pitch + rows * 4;  // and a power of two for each
   static constexpr int out_pitch = Dim + 4;  // floats: the lanes of a store meet 32 banks
   static constexpr int merge = 4 * rows * (out_pitch * 4 + 16);
   static constexpr int ring = stages * stage > merge ? stages * stage : merge;
@@ -225,15 +226,16 @@ __device__ __forceinline__ float load_q(const AttendArgs& a, long long at) {
                   : __half2float(static_cast<const __half*>(a.q)[at]);
 }
 
-// The unit's query rows into shared memory [rows][Dim], 16 bits, in the order of K's fragments;
-// returns what turns a product into a base-2 score.  A warp takes every fourth row.
+// The unit's live query rows into shared memory [rows][Dim], 16 bits, in the order of K's fragments, and
+// over codes what each row's scores are to be multiplied by; returns whether some row of the warp's
+// has another such factor than 1.  A warp takes every fourth row.
 template <int Kind, int Dim, int kRowTiles>
-__device__ __forceinline__ float stage_q(const AttendArgs& a, int b, int head, int first_row, unsigned char* q_rows,
-                                         float* most_of) {
+__device__ __forceinline__ bool stage_q(const AttendArgs& a, int b, int head, int first_row, int live,
+                                        unsigned char* q_rows, float* row_factor) {
   using Shape = MmaShape<Kind, Dim, kRowTiles>;
   constexpr int kEach = Dim / 32, kMine = Shape::rows / 4;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float x[kMine][kEach], most = 0.0f;
+  float x[kMine][kEach];
 #pragma unroll
   for (int i = 0; i < kMine; ++i) {
     const int row = first_row + warp + 4 * i, node = row / a.group;
@@ -242,23 +244,26 @@ __device__ __forceinline__ float stage_q(const AttendArgs& a, int b, int head, i
 #pragma unroll
     for (int k = 0; k < kEach; ++k) {
       const int d = lane + 32 * k;
-      x[i][k] = row < a.rows && d < a.cache.dim ? load_q(a, base + d) : 0.0f;
-      if (fabsf(x[i][k]) < INFINITY) most = fmaxf(most, fabsf(x[i][k]));
+      x[i][k] = row < a.rows && node < live && d < a.cache.dim ? load_q(a, base + d) : 0.0f;
     }
   }
-  float down = 1.0f, factor = a.scale_log2;
-  if constexpr (KindOf<Kind>::quantised) {
-    most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
-    if (lane == 0) most_of[warp] = most;
-    __syncthreads();
-    most = fmaxf(fmaxf(most_of[0], most_of[1]), fmaxf(most_of[2], most_of[3]));
-    int e = static_cast<int>(__float_as_uint(most) >> 23);  // biased exponent
-    e = most == 0.0f ? 127 : max(e, 16);
-    down = __uint_as_float(static_cast<unsigned>(min(127 + 14 + 127 - e, 253)) << 23);  // 2^(14 - (e - 127))
-    factor /= down;
-  }
+  bool shifted = false;
 #pragma unroll
-  for (int i = 0; i < kMine; ++i)
+  for (int i = 0; i < kMine; ++i) {
+    float down = 1.0f;
+    if (KindOf<Kind>::quantised && a.q_bf16) {
+      float most = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kEach; ++k)
+        if (fabsf(x[i][k]) < INFINITY) most = fmaxf(most, fabsf(x[i][k]));
+      most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+      if (most != 0.0f && (most < 0.25f || most >= 32768.0f)) {
+        const int e = max(static_cast<int>(__float_as_uint(most) >> 23), 16);  // biased exponent
+        down = __uint_as_float(static_cast<unsigned>(min(127 + 14 + 127 - e, 253)) << 23);  // 2^(14 - (e - 127))
+        shifted = true;
+      }
+    }
+    if (KindOf<Kind>::quantised && lane == 0) row_factor[warp + 4 * i] = 1.0f / down;
 #pragma unroll
     for (int k = 0; k < kEach; ++k) {
       const int d = lane + 32 * k, in = d & 15;
@@ -267,7 +272,8 @@ __device__ __forceinline__ float stage_q(const AttendArgs& a, int b, int head, i
       if constexpr (KindOf<Kind>::bf16) reinterpret_cast<__nv_bfloat16*>(q_row)[slot] = __float2bfloat16_rn(x[i][k]);
       else reinterpret_cast<__half*>(q_row)[slot] = __float2half_rn(x[i][k] * down);
     }
-  return factor;
+  }
+  return shifted;
 }
 
 template <int Kind, int Dim, int kRowTiles>
@@ -280,7 +286,7 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
   const int g = lane >> 2, c = lane & 3;
   const int dim = a.cache.dim, used = dim * Shape::bytes / 16;
   unsigned char* const q_rows = smem + Shape::ring;
-  float* const most_of = reinterpret_cast<float*>(q_rows + kRows * Shape::q_pitch);
+  float* const row_factor = reinterpret_cast<float*>(q_rows + kRows * Shape::q_pitch);
 
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -380,8 +386,9 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) issue(i < n);
 
-    const float factor = stage_q<Kind, Dim, kRowTiles>(a, b, at.head, first_row, q_rows, most_of);
-    __syncthreads();
+    const float factor = a.scale_log2;
+    const bool shifted =
+        __syncthreads_or(stage_q<Kind, Dim, kRowTiles>(a, b, at.head, first_row, live, q_rows, row_factor));
     // Q's fragments: [n = row g][k = 2c, 2c+1] and [k = 2c+8, 2c+9] of each step.
     uint32_t q[Shape::hold_q ? kSteps : 1][kRowTiles][2];
     const unsigned q_at = shared_at(q_rows) + (lane & 7) * Shape::q_pitch + (lane >> 3) * 16;
@@ -495,10 +502,19 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
           // A NaN has made the score a NaN where the row is seen, and must not touch l elsewhere.
           per_scale[h] = zero ? -1.0f : vs == vs ? exp2_fast(-lv) : 1.0f;
           nothing = nothing || zero;
+          if (shifted) {
 #pragma unroll
-          for (int j = 0; j < kRowTiles; ++j)
+            for (int j = 0; j < kRowTiles; ++j) {
+              const float2 f = *reinterpret_cast<const float2*>(row_factor + 8 * j + 2 * c);
+              s[j][2 * h] = fmaf(s[j][2 * h], ks * f.x, lv);
+              s[j][2 * h + 1] = fmaf(s[j][2 * h + 1], ks * f.y, lv);
+            }
+          } else {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) s[j][2 * h + e] = fmaf(s[j][2 * h + e], ks, lv);
+            for (int j = 0; j < kRowTiles; ++j)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) s[j][2 * h + e] = fmaf(s[j][2 * h + e], ks, lv);
+          }
         }
         nothing = __any_sync(0xffffffffu, nothing);
       } else {

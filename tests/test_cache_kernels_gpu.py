@@ -50,3 +50,30 @@ def test_a_cache_that_no_table_reaches(cuda, kind, dtype, nodes, group):
     c["table"][:] = -1
     out, lse = check_attention(c)
     assert (out == 0).all() and (lse == -math.inf).all()
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
+@pytest.mark.parametrize("nodes,group", [(2, 3), (4, 4), *ROWS])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("worst", [math.nan, math.inf, 1e20, 3e38])
+def test_queries_of_dead_nodes_may_hold_anything(cuda, kind, dtype, nodes, group, dim, worst):
+    c = attention_case(nodes * 7 + dim, 3, nodes, 2, group, dim, 16, [70, 33, 200], kind, dtype,
+                       live=[nodes - 1, 1, (nodes + 1) // 2])
+    for b in range(3):
+        c["q"][b, int(c["live"][b]):] = min(worst, torch.finfo(dtype).max) if math.isfinite(worst) else worst
+    out, lse = check_attention(c)
+    for b in range(3):
+        assert (out[b, int(c["live"][b]):] == 0).all() and (lse[b, int(c["live"][b]):] == -math.inf).all()
+
+
+@pytest.mark.parametrize("kind", [I8, E4M3])
+@pytest.mark.parametrize("nodes,group", [(2, 3), (4, 4), *ROWS])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_query_rows_of_very_different_sizes(cuda, kind, nodes, group, dim):
+    """Every row has the precision of its own magnitude, whatever the rows beside it hold."""
+    c = attention_case(nodes * 5 + dim, 2, nodes, 2, group, dim, 16, [90, 33], kind, BF16)
+    heads = torch.arange(2 * group, device="cuda")
+    for i in range(nodes):
+        size = torch.tensor([1.0, 1e-30, 1e12, 1e-3, 3e4, 1e20, 1.0], device="cuda")[(heads + i) % 7]
+        c["q"][:, i] = (c["q"][:, i].float() * size[:, None]).to(BF16)
+    check_attention(c)
