@@ -795,9 +795,9 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
               float high = -INFINITY;
 #pragma unroll
               for (int j = 0; j < 32; ++j) {
-                float x = __uint_as_float(s[j]) * factor;
+                // The factors first: a product of codes times the row's alone may pass F32's range.
+                float x = __uint_as_float(s[j]) * (kQuantised ? factor * slot.ks[32 * half + j] : factor);
                 if constexpr (kQuantised) {
-                  x *= slot.ks[32 * half + j];
                   if ((zero & see) >> j & 1) high = fmaxf(high, x);
                   else x += slot.lv[32 * half + j];
                 }

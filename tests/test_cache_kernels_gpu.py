@@ -77,3 +77,12 @@ def test_query_rows_of_very_different_sizes(cuda, kind, nodes, group, dim):
         size = torch.tensor([1.0, 1e-30, 1e12, 1e-3, 3e4, 1e20, 1.0], device="cuda")[(heads + i) % 7]
         c["q"][:, i] = (c["q"][:, i].float() * size[:, None]).to(BF16)
     check_attention(c)
+
+
+@pytest.mark.parametrize("kind", [I8, E4M3])
+@pytest.mark.parametrize("nodes,group", ROWS)
+def test_queries_near_the_largest_float(cuda, kind, nodes, group):
+    """Scores of some 1e36 are finite, and so is what leads to them."""
+    c = attention_case(nodes * 3, 2, nodes, 2, group, 128, 16, [90, 33], kind, BF16)
+    c["q"] = (c["q"].float() * 1e36).to(BF16)
+    check_attention(c)
