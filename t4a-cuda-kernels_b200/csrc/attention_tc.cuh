@@ -48,6 +48,7 @@ constexpr int kTcSoftmax = 128;  // threads; the issuing warp has a warpgroup of
 constexpr int kTcStages = 2;
 constexpr int kTcSlots = 4;  // of tiles' scales and flags: they outlive a stage by two tiles
 constexpr unsigned kTcColumns = 256;
+constexpr float kLargeScore = 4194304.0f;  // 2^22: products below it are rounded by less than 2^-2
 
 // What a tile's rows carry beside their values.
 template <typename Flags>
@@ -906,6 +907,15 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
                 tc_stored();
               }
             }
+            // The weights' fused product keeps what the maximum's rounded one lost: up to half a unit of its
+            // last place, which for large scores is a weight beyond F16.  Those are rounded first.
+            if (!kQuantised && fabsf(less) >= kLargeScore) {
+#pragma unroll
+              for (int q = 0; q < kSides; ++q)
+#pragma unroll
+                for (int j = 0; j < 32; ++j) s[q][j] = __float_as_uint(__uint_as_float(s[q][j]) * now_factor);
+              now_factor = 1.0f;
+            }
             // A look at the next tile's scores, which are there by now as a rule: its answer takes a while.
             // (Over codes they come later than that.)
             if (!kQuantised)
@@ -913,7 +923,7 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
 #pragma unroll
             for (int q = 0; q < kSides; ++q) {
               uint32_t p[16];
-              weights<kQuantised, kBf16>(s[q], p, kQuantised ? 1.0f : now_factor, less, slot.rv + 32 * (half + q), l4);
+              weights<kQuantised, kBf16>(s[q], p, now_factor, less, slot.rv + 32 * (half + q), l4);
               tc_store16(s_at + 16 * (half + q), p);
             }
             tc_stored();

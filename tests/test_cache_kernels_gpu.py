@@ -86,3 +86,12 @@ def test_queries_near_the_largest_float(cuda, kind, nodes, group):
     c = attention_case(nodes * 3, 2, nodes, 2, group, 128, 16, [90, 33], kind, BF16)
     c["q"] = (c["q"].float() * 1e36).to(BF16)
     check_attention(c)
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
+@pytest.mark.parametrize("nodes,group", ROWS)
+@pytest.mark.parametrize("scale", [3e5, -1e8, 1e10, 1e22])
+def test_large_scores(cuda, kind, dtype, nodes, group, scale):
+    """Scores whose last place is larger than the exponentials' range."""
+    c = attention_case(nodes * 3, 2, nodes, 2, group, 64, 16, [90, 333], kind, dtype)
+    check_attention(c, scale=scale)
