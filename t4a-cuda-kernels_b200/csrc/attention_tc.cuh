@@ -751,7 +751,7 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
         fence_async();
         barrier_arrive(&bar->q_full);
       }
-      float m = -INFINITY, less = -1e30f, mz = -INFINITY, lz = 0.0f;
+      float m = -INFINITY, less = 0.0f, mz = -INFINITY, lz = 0.0f;  // less: m - kLift once m is finite
       float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       bool ahead = false;  // the next tile's scores are known to be there
       for (int i = 0; i < n && good; ++i) {
@@ -843,7 +843,7 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
             float top = highest(s[0]);
             if constexpr (kSides == 2) top = fmaxf(top, highest(s[1]));
             if constexpr (!kQuantised) top *= now_factor;  // factors are not negative
-            const bool rises = here && top > less + (kSlack + kLift);
+            const bool rises = here && top > m + kSlack;
             if (__any_sync(0xffffffffu, rises)) {
               float shrink = 1.0f;
               if (rises) {

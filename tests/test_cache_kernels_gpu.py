@@ -95,3 +95,14 @@ def test_large_scores(cuda, kind, dtype, nodes, group, scale):
     """Scores whose last place is larger than the exponentials' range."""
     c = attention_case(nodes * 3, 2, nodes, 2, group, 64, 16, [90, 333], kind, dtype)
     check_attention(c, scale=scale)
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
+@pytest.mark.parametrize("nodes,group", ROWS)
+def test_scores_far_below_zero(cuda, kind, dtype, nodes, group):
+    """All of a row's scores below -1e30: the row sees its tokens all the same."""
+    c = attention_case(nodes * 3, 2, nodes, 2, group, 64, 16, [90, 333], kind, dtype)
+    c["q"] = c["q"].abs()
+    c["k"] = -c["k"].abs() if kind != E4M3 else (-c["k"].float().abs()).to(kind)
+    out, lse = check_attention(c, scale=1e32)
+    assert float(lse.max()) < -1e30
