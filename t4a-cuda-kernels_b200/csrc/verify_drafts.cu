@@ -288,7 +288,8 @@ class Walk {
           if (kMode == kGreedy) {
             // Indices rise along a thread's walk, so the first of equals is its lowest.
             const int i = (first + j) * kVec - skew + e;
-            if (i >= 0 && i < a.vocab && (v > mine.m || mine.key == 0)) mine.key = make_key(ordered(v), i);
+            // (-0 equals 0, so it has 0's key.)
+            if (i >= 0 && i < a.vocab && (v > mine.m || mine.key == 0)) mine.key = make_key(ordered(v + 0.0f), i);
           }
           mine.m = fmaxf(mine.m, v);
         }
