@@ -18,7 +18,7 @@
 // Quantised rows stay codes in shared memory and become F16 in registers, exactly.  K's scale
 // multiplies the score.  V's scale is an addend of the exponent, S + log2(scale): the weight that
 // meets the codes then is relative to the largest weight * scale of its row, whatever the scales
-// are; l adds weight / scale.  Rows with a scale of 0 (or below 2^-107, which the writer does not
+// are; l adds weight / scale.  Rows with a scale of 0 (or below 2^-110, which the writer does not
 // make) count in the softmax alone: they have a maximum and a sum of their own, joined at the end.
 // Q is F16 too.  BF16 rows become it exactly from 2^-17 up and within 2^-25 below, so a row whose
 // largest magnitude is outside [1/4, 2^15) is first brought to [2^14, 2^15) by a power of two of its own,
@@ -44,7 +44,7 @@ namespace cache {
 constexpr int kMmaThreads = 128;
 constexpr float kSlack = 8.0f;  // log2 by which a maximum may exceed the one in use
 constexpr float kLift = 7.0f;   // log2 of what all weights carry
-constexpr float kLeastScale = 6.1629758e-33f;  // 2^-107
+constexpr float kLeastScale = 7.7037198e-34f;  // 2^-110: the writer's least is 2^-100 / 448
 
 template <int Kind>
 struct KindOf {

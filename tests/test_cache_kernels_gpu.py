@@ -9,7 +9,10 @@ import math
 import pytest
 import torch
 
-from test_cache_gpu import BF16, E4M3, F16, I8, KINDS, attention_case, check_attention, poison_unused
+import cache_reference as ref
+import t4a_b200 as t4
+from test_cache_gpu import (BF16, E4M3, F16, I8, KINDS, UNIT, attention_case, check_attention, generator,
+                            poison_unused)
 
 pytestmark = pytest.mark.gpu
 
@@ -106,3 +109,31 @@ def test_scores_far_below_zero(cuda, kind, dtype, nodes, group):
     c["k"] = -c["k"].abs() if kind != E4M3 else (-c["k"].float().abs()).to(kind)
     out, lse = check_attention(c, scale=1e32)
     assert float(lse.max()) < -1e30
+
+
+def check_relative(c):
+    """As check_attention, for outputs far from 1: errors go by the outputs' own magnitudes alone."""
+    scale = c["q"].shape[3] ** -0.5
+    out, lse = t4.tree_attention(c["q"], c["k"], c["v"], c["table"], c["context"], mask=c["sees"], k_scale=c["ks"],
+                                 v_scale=c["vs"])
+    want, want_lse, spread, size = ref.attention(c["q"], c["k"], c["v"], c["ks"], c["vs"], c["table"], c["context"],
+                                                 c["sees"], c["live"], scale)
+    u = (UNIT[BF16] if c["k"].dtype == BF16 else UNIT[F16]) + UNIT[c["q"].dtype] + 2.0 ** -13
+    assert float(((out.double() - want).abs() / spread).max()) <= u
+    assert float(((lse.double() - want_lse).abs() / (size + want_lse.abs() + 1)).max()) <= 2.0 ** -18
+
+
+@pytest.mark.parametrize("kind", [I8, E4M3])
+@pytest.mark.parametrize("nodes,group", ROWS)
+@pytest.mark.parametrize("least", [2.0 ** -100, 1.5 * 2.0 ** -99])
+def test_the_smallest_rows_that_are_kept(cuda, kind, nodes, group, least):
+    """V rows whose largest magnitude is the least that the writer does not store as zeros."""
+    c = attention_case(nodes, 2, nodes, 2, group, 64, 16, [90, 33], kind, BF16)
+    rows = c["v"].shape[0] * 16
+    gen = generator(nodes)
+    value = torch.rand(rows, 2, 64, generator=gen, device="cuda") * 2 - 1
+    value = (value / value.abs().amax(dim=2, keepdim=True)).clamp(-1, 1) * least
+    key = torch.randn(rows, 2, 64, generator=gen, device="cuda")
+    t4.cache_write(key, value, c["k"], c["v"], torch.arange(rows, device="cuda"), k_scale=c["ks"], v_scale=c["vs"])
+    assert (c["vs"] > 0).all()
+    check_relative(c)
