@@ -10,7 +10,8 @@
  * strides (layout axes 0..3: dim, heads, page_size, pages).  dim is a multiple of 16, at
  * most 256, with unit stride, and every row starts on a 16-byte boundary.  A slot is
  * page * page_size + place.  A quantised kind holds one F32 scale per row (layout axes
- * 0..2: heads, page_size, pages): a row's values are code * scale.
+ * 0..2: heads, page_size, pages): a row's values are code * scale.  A scale is not below
+ * zero; attention gives NaN to whatever sees a V row that has such a one.
  */
 #ifndef T4A_B200_CACHE_H_
 #define T4A_B200_CACHE_H_

@@ -497,10 +497,11 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const float ks = scales[8 * h] * factor, vs = scales[kTile + 8 * h];
-          const bool zero = vs < kLeastScale;
+          const bool zero = fabsf(vs) < kLeastScale;
           const float lv = zero ? 0.0f : __log2f(vs);
-          // A NaN has made the score a NaN where the row is seen, and must not touch l elsewhere.
-          per_scale[h] = zero ? -1.0f : vs == vs ? exp2_fast(-lv) : 1.0f;
+          // A NaN, also of a scale below zero, has made the score a NaN where the row is seen, and must
+          // not touch l elsewhere.
+          per_scale[h] = zero ? -1.0f : lv == lv ? exp2_fast(-lv) : 1.0f;
           nothing = nothing || zero;
           if (shifted) {
 #pragma unroll

@@ -495,15 +495,16 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
         TcSlot<Flags>& slot = slots[t % kTcSlots];
         if (lane == 0) slot.there[first_token / kTokens] = static_cast<Flags>(bits);
         if constexpr (kQuantised) {
-          const bool zero = vs < kLeastScale;
+          const bool zero = fabsf(vs) < kLeastScale;
           const unsigned zeros_of = __ballot_sync(0xffffffffu, zero) & kAllThere;
           if (lane == 0) slot.zero[first_token / kTokens] = static_cast<Flags>(zeros_of);
           const float lv = zero ? -INFINITY : __log2f(vs);
           if (lane < kTokens) {
             slot.ks[first_token + lane] = ks * fabsf(a.scale_log2);
             slot.lv[first_token + lane] = lv;
-            // A NaN has made the score a NaN where the row is seen, and must not touch l elsewhere.
-            slot.rv[first_token + lane] = zero ? 0.0f : vs == vs ? exp2_fast(-lv) : 1.0f;
+            // A NaN, also of a scale below zero, has made the score a NaN where the row is seen, and must
+            // not touch l elsewhere.
+            slot.rv[first_token + lane] = zero ? 0.0f : lv == lv ? exp2_fast(-lv) : 1.0f;
           }
         }
         __syncwarp();

@@ -137,3 +137,19 @@ def test_the_smallest_rows_that_are_kept(cuda, kind, nodes, group, least):
     t4.cache_write(key, value, c["k"], c["v"], torch.arange(rows, device="cuda"), k_scale=c["ks"], v_scale=c["vs"])
     assert (c["vs"] > 0).all()
     check_relative(c)
+
+
+@pytest.mark.parametrize("kind", [I8, E4M3])
+@pytest.mark.parametrize("nodes,group", ROWS)
+def test_scales_below_zero_show(cuda, kind, nodes, group):
+    """No writer makes a V scale below zero: who sees its row gets NaN, who does not its usual result."""
+    c = attention_case(nodes, 2, nodes, 2, group, 64, 16, [40, 117], kind, BF16)
+    want, want_lse = check_attention(c)
+    for b, place in ((0, 40 + 1), (1, 117 + 1)):
+        c["vs"][int(c["table"][b, place // 16]), place % 16] = -0.01
+    out, lse = t4.tree_attention(c["q"], c["k"], c["v"], c["table"], c["context"], mask=c["sees"], k_scale=c["ks"],
+                                 v_scale=c["vs"])
+    reached = c["sees"][:, :, 1][:, :, None].expand(lse.shape)
+    assert reached.any() and not reached.all()
+    assert torch.isnan(lse[reached]).all() and torch.isnan(out[reached]).all()
+    assert torch.equal(out[~reached], want[~reached]) and torch.equal(lse[~reached], want_lse[~reached])
