@@ -86,7 +86,9 @@ int t4a_cache_read(void* stream, int dtype, int index_dtype, const t4a_kv_cache*
  *     of the softmax's sum.  A node that sees nothing gets zeros and -infinity.
  * Rows that a node does not see do not enter its result, whatever they hold.  Sums and the
  * softmax are in F32; a weight is rounded to the cache's 16-bit type (F16 for the quantised
- * kinds) before its product with V. */
+ * kinds) before its product with V.  Over a quantised cache the scales of the V rows that a node
+ * sees, but those of 0, lie within a factor of 2^90 of one another: a row far below that may be
+ * missing from the softmax. */
 int t4a_tree_attention_workspace_bytes(int dtype, const t4a_kv_cache* cache, const t4a_cuda_layout* q_layout,
                                        const t4a_cuda_layout* table_layout, size_t* bytes);
 int t4a_tree_attention(void* stream, int dtype, const t4a_kv_cache* cache, void* out,

@@ -17,8 +17,9 @@
 //
 // Quantised rows stay codes in shared memory and become F16 in registers, exactly.  K's scale
 // multiplies the score.  V's scale is an addend of the exponent, S + log2(scale): the weight that
-// meets the codes then is relative to the largest weight * scale of its row, whatever the scales
-// are; l adds weight / scale.  Rows with a scale of 0 (or below 2^-110, which the writer does not
+// meets the codes then is relative to the largest weight * scale of its row; l adds weight / scale.
+// The weight becomes 0 from 2^-133 of the largest down, so while the scales of the seen rows lie within
+// 2^90 of one another, what l loses is 2^-43 of its largest term.  Rows with a scale of 0 (or below 2^-110, which the writer does not
 // make) count in the softmax alone: they have a maximum and a sum of their own, joined at the end.
 // Q is F16 too.  BF16 rows become it exactly from 2^-17 up and within 2^-25 below, so a row whose
 // largest magnitude is outside [1/4, 2^15) is first brought to [2^14, 2^15) by a power of two of its own,

@@ -153,3 +153,14 @@ def test_scales_below_zero_show(cuda, kind, nodes, group):
     assert reached.any() and not reached.all()
     assert torch.isnan(lse[reached]).all() and torch.isnan(out[reached]).all()
     assert torch.equal(out[~reached], want[~reached]) and torch.equal(lse[~reached], want_lse[~reached])
+
+
+@pytest.mark.parametrize("kind", [I8, E4M3])
+@pytest.mark.parametrize("nodes,group", ROWS)
+def test_value_scales_as_far_apart_as_they_may_be(cuda, kind, nodes, group):
+    """Scales of V from 2^-45 to 2^45: rows that hardly matter to the output count in the softmax all the same."""
+    c = attention_case(nodes, 2, nodes, 2, group, 64, 16, [150, 700], kind, BF16)
+    gen = generator(nodes)
+    ends = torch.where(torch.rand(c["vs"].shape, generator=gen, device="cuda") < 0.1, 45.0, -45.0)
+    c["vs"] = torch.exp2(ends)
+    check_relative(c)
