@@ -311,7 +311,7 @@ __device__ __forceinline__ void weights(const uint32_t (&s)[32], uint32_t* p, fl
   }
 }
 
-// A pair of weights, times x.
+// A pair of weights, times x, a power of two: rounded only where a weight leaves F16's normal range.
 template <bool Bf16>
 __device__ __forceinline__ uint32_t scaled_pair(uint32_t pair, float x) {
   if constexpr (Bf16) {
@@ -848,9 +848,11 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
             if (__any_sync(0xffffffffu, rises)) {
               float shrink = 1.0f;
               if (rises) {
-                shrink = exp2_fast(m - top);
-                m = top;
-                less = top - kLift;
+                // References are whole numbers, so that weights and outputs shrink by powers of two: exactly.
+                const float to = ceilf(top), by = m - to;
+                shrink = by < -126.0f ? 0.0f : __uint_as_float(static_cast<unsigned>(static_cast<int>(by) + 127) << 23);
+                m = to;
+                less = to - kLift;
                 l4[0] *= shrink, l4[1] *= shrink, l4[2] *= shrink, l4[3] *= shrink;
               }
               if (kSides == 1 && half == 1) {

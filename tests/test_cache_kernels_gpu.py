@@ -164,3 +164,28 @@ def test_value_scales_as_far_apart_as_they_may_be(cuda, kind, nodes, group):
     ends = torch.where(torch.rand(c["vs"].shape, generator=gen, device="cuda") < 0.1, 45.0, -45.0)
     c["vs"] = torch.exp2(ends)
     check_relative(c)
+
+
+@pytest.mark.parametrize("kind", [I8, E4M3])
+@pytest.mark.parametrize("nodes,group", ROWS)
+def test_a_weight_is_rounded_once(cuda, kind, nodes, group):
+    """A maximum that rises within a tile by a factor that would round the weights before it once more, in the
+    same direction for all of them, as the output's own rounding."""
+    c = attention_case(nodes, 1, nodes, 2, group, 64, 16, [64], kind, F16)
+    near = 1 + 0.98 * 2.0 ** -11  # F16 rounds it down to 1
+    score = torch.full((64,), -200.0, dtype=torch.float64)  # in powers of two
+    score[0], score[1:32], score[32] = 0.0, math.log2(near) - 1, 9 - math.log2(near)
+    weight = torch.exp2(score)
+    value = torch.where((score < 0) & (score > -2), 96.0, 0.0)
+    c["q"][:] = 0
+    c["q"][..., 0] = 1
+    c["sees"][:] = False
+    slot = (c["table"][0].long()[:, None] * 16 + torch.arange(16, device="cuda")).flatten()[:64]
+    out = float((weight * value).sum() / weight.sum())
+    three = near / (1 - 2 * 0.98 * 2.0 ** -11)  # what is left after two roundings down is `near` again
+    size = three * 2.0 ** math.floor(math.log2(out)) / out
+    for name, codes in (("k", torch.eye(1, 64).expand(64, 64)), ("v", value[:, None].expand(64, 64))):
+        c[name].view(-1, 2, 64)[slot] = codes.to("cuda")[:, None].expand(64, 2, 64).to(kind)
+    c["ks"].view(-1, 2)[slot] = (score / math.log2(math.e)).float().to("cuda")[:, None]
+    c["vs"][:] = size
+    check_attention(c, scale=1.0)
