@@ -189,3 +189,100 @@ def test_a_weight_is_rounded_once(cuda, kind, nodes, group):
     c["ks"].view(-1, 2)[slot] = (score / math.log2(math.e)).float().to("cuda")[:, None]
     c["vs"][:] = size
     check_attention(c, scale=1.0)
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
+@pytest.mark.parametrize("nodes,group", ROWS)
+def test_contexts_past_the_table_and_below_zero(cuda, kind, dtype, nodes, group):
+    c = attention_case(nodes + 1, 4, nodes, 2, group, 64, 16, [200] * 4, kind, dtype)
+    places = c["table"].shape[1] * 16
+    c["context"] = torch.tensor([places - nodes // 2, places + 5, 1 << 30, -7], dtype=torch.int32, device="cuda")
+    check_attention(c)
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
+@pytest.mark.parametrize("nodes,group", ROWS)
+@pytest.mark.parametrize("scale", [0.0, -0.0, -0.3, 1.7])
+def test_score_scales(cuda, kind, dtype, nodes, group, scale):
+    check_attention(attention_case(nodes + 2, 2, nodes, 2, group, 64, 16, [170, 5], kind, dtype), scale=scale)
+
+
+@pytest.mark.parametrize("kind", [I8, E4M3])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("nodes,group", ROWS)
+@pytest.mark.parametrize("size", [0.0, 1e-30, 1e-6, 1e6])
+def test_value_rows_of_zero_and_of_very_different_sizes(cuda, kind, dtype, nodes, group, size):
+    """Zero rows of V in the context, among the drafted rows, as a whole tile and as all that a node sees."""
+    c = attention_case(nodes + 3, 3, nodes, 2, group, 128, 16, [400, 90, 0], kind, dtype)
+    c["vs"][::2] *= size if dtype == BF16 or size < 1 else 1e2
+    c["vs"][1] = 0
+    c["vs"][c["table"][0, 8:12].long()] = 0
+    c["vs"][c["table"][2].long()] = 0
+    c["k"].view(torch.int8)[2] = 0
+    check_attention(c)
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
+@pytest.mark.parametrize("nodes,group", ROWS)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_maxima_that_rise_late_and_early(cuda, kind, dtype, nodes, group, dim):
+    """One sequence over many blocks, and short ones in one; rows whose best token comes first, last and between,
+    in either half of a tile, each some hundreds of powers of two above the rest."""
+    c = attention_case(nodes + 4, 3, nodes, 2, group, dim, 16, [9000, 300, 64], kind, dtype)
+    for b, length in enumerate((9000, 300, 64)):
+        for i in range(nodes):
+            place = [0, length - 1, length // 2, 31, 33, 63, length - 33][i % 7]
+            row = c["k"][int(c["table"][b, place // 16]), place % 16].float()
+            c["q"][b, i] = (row.sign() * 3).repeat_interleave(group, dim=0).to(dtype)
+    check_attention(c)
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
+@pytest.mark.parametrize("nodes,group", ROWS)
+@pytest.mark.parametrize("gap", [1, 2, 4])
+def test_rows_off_16_bytes(cuda, kind, dtype, nodes, group, gap):
+    """Queries and outputs at 2-, 4- and 8-byte boundaries, heads and batch in other orders, caches by heads."""
+    c = attention_case(nodes + 5, 3, nodes, 2, group, 80, 8, [130, 9, 700], kind, dtype)
+    for name in ("k", "v"):
+        c[name] = c[name].transpose(1, 2).contiguous().transpose(1, 2)
+        if c[name + "s"] is not None:
+            c[name + "s"] = c[name + "s"].permute(2, 0, 1).contiguous().permute(1, 2, 0)
+    wide = torch.zeros(3, nodes, 2 * group * 80 + gap, dtype=dtype, device="cuda")
+    q = wide[:, :, gap:].unflatten(2, (2 * group, 80))
+    q.copy_(c["q"])
+    c["q"] = q
+    out = torch.zeros(2 * group, 3, nodes, 80 + gap, dtype=dtype, device="cuda").permute(1, 2, 0, 3)[..., gap:]
+    check_attention(c, out=out)
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
+@pytest.mark.parametrize("nodes,group", ROWS)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_values_that_are_no_numbers(cuda, kind, dtype, nodes, group, dim):
+    """NaN and infinite V values in several drafted rows reach the nodes that see them, also where a page of the
+    context lies outside the cache, and in the tile that context and drafts share."""
+    c = attention_case(nodes + 6, 3, nodes, 2, group, dim, 16, [700, 333, 90], kind, dtype)
+    clean = {k: t.clone() if torch.is_tensor(t) else t for k, t in c.items()}
+    reached = torch.zeros(3, nodes, dtype=torch.bool, device="cuda")
+    for b in range(3):
+        for x in (c, clean):
+            x["table"][b, [1, 3]] = torch.tensor([-1, 1 << 30], dtype=torch.int32, device="cuda")
+        for bad in (nodes - 1, nodes // 2):
+            place = int(c["context"][b]) + bad
+            at = (int(c["table"][b, place // 16]), place % 16)
+            if kind == I8:
+                c["vs"][at] = math.nan
+            elif kind == E4M3:
+                c["v"].view(torch.uint8)[at] = 0x7f
+            else:
+                c["v"][at] = math.nan if b else math.inf
+            reached[b] |= c["sees"][b, :, bad]
+    out, lse = t4.tree_attention(c["q"], c["k"], c["v"], c["table"], c["context"], mask=c["sees"], k_scale=c["ks"],
+                                 v_scale=c["vs"])
+    want, want_lse, spread, size = ref.attention(clean["q"], clean["k"], clean["v"], clean["ks"], clean["vs"],
+                                                 clean["table"], clean["context"], clean["sees"], clean["live"],
+                                                 dim ** -0.5)
+    assert reached.any() and not torch.isfinite(out[reached]).any() and torch.isfinite(out[~reached]).all()
+    u = (UNIT[BF16] if kind == BF16 else UNIT[F16]) + UNIT[dtype] + 2.0 ** -13
+    assert float(((out.double() - want).abs() - u * spread - 2.0 ** -24)[~reached].max()) <= 0
+    assert float(((lse.double() - want_lse).abs() / (size + want_lse.abs() + 1))[~reached].max()) <= 2.0 ** -18
