@@ -92,7 +92,7 @@ def tree(depth):
 
 def generate(target, prompt, count, depth=3, temperature=0.0, seed=1):
     """At least `count` tokens after each prompt [batch, n], and the steps that they took; depth 0 drafts
-    nothing: a token a step."""
+    nothing: a token a step.  A sequence that has its tokens waits for the others: its step is repeated."""
     gen = torch.Generator(device="cuda").manual_seed(seed)
     batch, n = prompt.shape
     parents, sees = tree(depth)
@@ -129,12 +129,12 @@ def generate(target, prompt, count, depth=3, temperature=0.0, seed=1):
             old = torch.where(kept >= 0, kept, new)
             cache.move(context[:, None].long() + old, context[:, None].long() + new)
         steps += 1
+        goes_on = torch.tensor([len(o) < count for o in out], device="cuda")
         for o, row, k in zip(out, said.tolist(), taken.tolist()):
-            o.extend(row[:k + 1])
-        context += taken + 1
-        tokens[:, 0] = said.gather(1, taken[:, None].long())[:, 0]
-        if int(context.max()) + nodes > cache.table.shape[1] * cache.page:
-            break
+            if len(o) < count:
+                o.extend(row[:k + 1])
+        context += torch.where(goes_on, taken + 1, 0)
+        tokens[:, 0] = torch.where(goes_on, said.gather(1, taken[:, None].long())[:, 0], tokens[:, 0])
     return out, steps
 
 
