@@ -7,8 +7,9 @@ dim] (float16, bfloat16, int8 or float8_e4m3fn; any strides but 1 along dim), it
 [pages, page_size, heads] float32.  The library checks layouts and refuses with a
 T4AError; a wrong dtype is a TypeError, a tensor on another device or of another rank a
 ValueError.  Calls run on the current stream, or on `stream`, whose allocations results
-and workspace then are.  The functions are native (binding/cache_torch.cpp): a small call
-is a few microseconds on the host.
+and workspace then are; inputs may be freed while that stream still reads them, but what
+wrote them has to be waited for (stream.wait_stream).  The functions are native
+(binding/cache_torch.cpp): a small call is a few microseconds on the host.
 """
 import ctypes
 import importlib.machinery
@@ -60,7 +61,11 @@ def _call(name, stream, *args):
     function = getattr(native(), name)
     import torch
     with torch.cuda.stream(stream):
-        return function(*args)
+        got = function(*args)
+    for t in args:  # their memory is not given out again before the stream is through with it
+        if torch.is_tensor(t):
+            t.record_stream(stream)
+    return got
 
 
 def cache_write(key, value, k_cache, v_cache, slots, k_scale=None, v_scale=None, stream=None):
