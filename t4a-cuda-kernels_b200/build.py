@@ -115,14 +115,30 @@ def build_waitzero(force=False):
     return lib
 
 
+def torch_place():
+    """(directory, identity) of the installed torch, without importing it; None where there is none."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None or spec.origin is None:
+        return None
+    directory = os.path.dirname(spec.origin)
+    version = os.path.join(directory, "version.py")
+    return directory, directory + "\n" + (open(version).read() if os.path.exists(version) else "")
+
+
 def build_binding(lib, force=False):
-    """lib/_cache_torch.so: the Python functions of binding/cache_torch.cpp over torch tensors."""
+    """lib/_cache_torch.so: the Python functions of binding/cache_torch.cpp over torch tensors.  Built against the
+    torch that is installed, and anew when that is another one; without torch the library is all there is."""
     import sysconfig
-    spec = importlib.util.find_spec("torch")  # its headers and libraries, without importing it
-    torch_dir = os.path.dirname(spec.origin)
     src = os.path.join(HERE, "binding", "cache_torch.cpp")
     out = os.path.join(LIBDIR, "_cache_torch.so")
-    if force or stale(out, [src] + headers(src)):
+    place = torch_place()
+    if place is None:
+        print("torch is not installed: the paged-cache operators' Python binding is left out", file=sys.stderr)
+        return None
+    torch_dir, identity = place
+    built_for = os.path.join(BUILD, "cache_torch.torch")
+    same = os.path.exists(built_for) and open(built_for).read() == identity
+    if force or not same or stale(out, [src] + headers(src)):
         cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
         includes = [os.path.join(torch_dir, "include"), os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
                     os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
@@ -130,6 +146,8 @@ def build_binding(lib, force=False):
         run(["g++", "-std=c++17", "-O2", "-fPIC", "-shared"] + [f for i in includes for f in ("-isystem", i)] +
             [src, "-o", out, "-L", LIBDIR, "-lt4a_b200", "-L", torch_libs, "-ltorch_python", "-ltorch_cpu", "-lc10",
              "-lc10_cuda", "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + torch_libs])
+        with open(built_for, "w") as f:
+            f.write(identity)
     return out
 
 
