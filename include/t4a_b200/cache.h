@@ -104,7 +104,9 @@ int t4a_tree_attention(void* stream, int dtype, const t4a_kv_cache* cache, void*
  *     the target after each node.  tokens, parents: I32 [batch][nodes], compact; a parent's
  *     index is below its child's, and node 0's entries are not read.
  *   draft: F32, layout axes vocab, nodes, batch, or NULL: the distribution that a node's
- *     children were drawn from.  uniforms: F32 [batch][nodes], compact, in [0, 1).
+ *     children were drawn from, each independently, so that siblings may be alike.  Children
+ *     drawn without replacement, or picked as the likeliest, need draft NULL: the tokens said then
+ *     follow the target wherever the children came from; with a draft they would not.  uniforms: F32 [batch][nodes], compact, in [0, 1).
  *   race: F32, layout axes vocab, batch: reciprocals of standard exponential variates.
  * At a node r = softmax(logits / temperature).  Its children are tried in order: child c with
  * token x is taken when uniforms[c] * draft[x] < r[x] (draft[x] = 1 without draft).  Else r

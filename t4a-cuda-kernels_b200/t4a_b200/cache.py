@@ -113,6 +113,9 @@ def verify_drafts(logits, tokens, parents, uniforms=None, draft=None, race=None,
     children).  Child x of a node is taken when uniforms[b, child] * draft[b, node, x] < r[x] (draft
     None: deterministic drafts, 1), r being softmax(logits / temperature) less what the children
     turned down before it took; the last token is argmax r * race.  temperature 0: argmaxes.
+    With `draft` a node's children are independent draws from it, so siblings may be alike; children
+    drawn without replacement, or picked as the likeliest, need draft=None for what is said to follow
+    the target.
     Returns (count [batch], path [batch, nodes], said [batch, nodes], logs [batch, nodes]): nodes
     taken, which, the tokens with the last one behind them (-1 elsewhere), their log-probabilities."""
     return _call("verify", stream, logits, tokens, parents, uniforms, draft, race, temperature)
