@@ -9,7 +9,8 @@ T4AError; a wrong dtype is a TypeError, a tensor on another device or of another
 ValueError.  Calls run on the current stream, or on `stream`, whose allocations results
 and workspace then are; inputs may be freed while that stream still reads them, but what
 wrote them has to be waited for (stream.wait_stream).  The functions are native
-(binding/cache_torch.cpp): a small call is a few microseconds on the host.
+(binding/cache_torch.cpp): a small call is a few microseconds on the host.  They serve
+decoding and have no backward pass: results never require a gradient, whatever the inputs do.
 """
 import ctypes
 import importlib.machinery

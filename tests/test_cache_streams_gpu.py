@@ -1,4 +1,4 @@
-"""Inputs that are freed right after a call on another stream."""
+"""How the paged-cache operators treat tensors that torch does more with: other streams, gradients."""
 import pytest
 import torch
 
@@ -52,3 +52,15 @@ def test_inputs_outlive_a_call_on_another_stream(cuda, operator):
     side.synchronize()
     torch.cuda.synchronize()
     assert others and all(torch.equal(a, b) for a, b in zip([*got, k, v], want))
+
+
+def test_results_never_require_a_gradient(cuda):
+    """Inputs that require one are taken, as the docstring says, and nothing is recorded."""
+    k, v = (torch.zeros(4, 16, 2, 64, dtype=torch.float16, device="cuda") for _ in range(2))
+    key = torch.randn(20, 2, 64, device="cuda", requires_grad=True)
+    slots = torch.arange(20, device="cuda")
+    t4.cache_write(key, key, k, v, slots)
+    q = torch.randn(1, 2, 4, 64, device="cuda").half().requires_grad_()
+    out, lse = t4.tree_attention(q, k, v, torch.arange(4, dtype=torch.int32, device="cuda")[None],
+                                 torch.full((1,), 18, dtype=torch.int32, device="cuda"))
+    assert not any(t.requires_grad for t in (k, v, out, lse, *t4.cache_read(k, v, slots, torch.float32)))
