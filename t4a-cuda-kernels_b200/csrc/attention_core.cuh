@@ -149,22 +149,23 @@ __device__ __forceinline__ bool node_sees(const AttendArgs& a, int b, int i, int
   return a.mask[b * a.mask_batch + i * a.mask_node + j * a.mask_seen] != 0;
 }
 
-__device__ __forceinline__ void store_out(const AttendArgs& a, long long at, float x, float y, bool two) {
+// Two neighbouring values of out, the first at an even column.
+__device__ __forceinline__ void store_out(const AttendArgs& a, long long at, float x, float y) {
   if (a.q_bf16) {
     __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.out) + at;
-    if (a.pairs && two) {
+    if (a.pairs) {
       *reinterpret_cast<__nv_bfloat162*>(o) = __floats2bfloat162_rn(x, y);
     } else {
       o[0] = __float2bfloat16_rn(x);
-      if (two) o[1] = __float2bfloat16_rn(y);
+      o[1] = __float2bfloat16_rn(y);
     }
   } else {
     __half* o = static_cast<__half*>(a.out) + at;
-    if (a.pairs && two) {
+    if (a.pairs) {
       *reinterpret_cast<__half2*>(o) = __floats2half2_rn(x, y);
     } else {
       o[0] = __float2half_rn(x);
-      if (two) o[1] = __float2half_rn(y);
+      o[1] = __float2half_rn(y);
     }
   }
 }

@@ -734,7 +734,7 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
       x = dead ? 0.0f : x * over;
       y = dead ? 0.0f : y * over;
       if (whole) {
-        store_out(a, out_row(a, b, at.head, row) + d, x, y, true);
+        store_out(a, out_row(a, b, at.head, row) + d, x, y);
         if (d == 0) store_lse(a, b, at.head, row, lse2);
       } else {
         *reinterpret_cast<float2*>(a.part_out + (part + r) * dim + d) = make_float2(x, y);

@@ -408,7 +408,6 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
     unsigned long long* const full = is_v ? bar->v_full : bar->k_full;
     unsigned long long* const empty = is_v ? bar->v_empty : bar->k_empty;
     auto lines = [&](int stage) { return is_v ? v_lines(stage) : k_lines(stage); };
-    // The row and chunk of a lane in round u.
     // The row and chunk of a lane in round u: round u's rows are kStep further on than round 0's.
     // Codes become two units each: 8 lanes then take 4 chunks of two rows, whose units the swizzle
     // keeps apart, rather than 8 of one.

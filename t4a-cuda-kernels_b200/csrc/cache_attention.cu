@@ -31,7 +31,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_join(const AttendArgs a) {
   if (!any) return;
   const long long to = out_row(a, b, head, row);
   if (tiles == 0) {
-    for (int d = 2 * (warp * 32 + lane); d < dim; d += 64 * kWarps) store_out(a, to + d, 0.0f, 0.0f, true);
+    for (int d = 2 * (warp * 32 + lane); d < dim; d += 64 * kWarps) store_out(a, to + d, 0.0f, 0.0f);
     if (warp == 0 && lane == 0) store_lse(a, b, head, row, -INFINITY);
     return;
   }
@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_join(const AttendArgs a) {
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int d = 2 * lane + 64 * k;
-    if (d < dim) store_out(a, to + d, x[2 * k] * over, x[2 * k + 1] * over, true);
+    if (d < dim) store_out(a, to + d, x[2 * k] * over, x[2 * k + 1] * over);
   }
   if (lane == 0) store_lse(a, b, head, row, empty ? -INFINITY : less + log2f(sum));
 }
