@@ -495,27 +495,29 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
       bool nothing = false;  // a scale of 0 among the thread's tokens
       if constexpr (kQuantised) {
         const float* const scales = reinterpret_cast<const float*>(stage + kScales) + 16 * warp + g;
+        float ks[2], lv[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float ks = scales[8 * h] * factor, vs = scales[kTile + 8 * h];
+          const float vs = scales[kTile + 8 * h];
           const bool zero = fabsf(vs) < kLeastScale;
-          const float lv = zero ? 0.0f : __log2f(vs);
+          ks[h] = scales[8 * h] * factor;
+          lv[h] = zero ? 0.0f : __log2f(vs);
           // A NaN, also of a scale below zero, has made the score a NaN where the row is seen, and must
           // not touch l elsewhere.
-          per_scale[h] = zero ? -1.0f : lv == lv ? exp2_fast(-lv) : 1.0f;
+          per_scale[h] = zero ? -1.0f : lv[h] == lv[h] ? exp2_fast(-lv[h]) : 1.0f;
           nothing = nothing || zero;
-          if (shifted) {
+        }
+        if (!shifted) {
 #pragma unroll
-            for (int j = 0; j < kRowTiles; ++j) {
-              const float2 f = *reinterpret_cast<const float2*>(row_factor + 8 * j + 2 * c);
-              s[j][2 * h] = fmaf(s[j][2 * h], ks * f.x, lv);
-              s[j][2 * h + 1] = fmaf(s[j][2 * h + 1], ks * f.y, lv);
-            }
-          } else {
+          for (int j = 0; j < kRowTiles; ++j)
 #pragma unroll
-            for (int j = 0; j < kRowTiles; ++j)
+            for (int e = 0; e < 4; ++e) s[j][e] = fmaf(s[j][e], ks[e >> 1], lv[e >> 1]);
+        } else {
 #pragma unroll
-              for (int e = 0; e < 2; ++e) s[j][2 * h + e] = fmaf(s[j][2 * h + e], ks, lv);
+          for (int j = 0; j < kRowTiles; ++j) {
+            const float2 f = *reinterpret_cast<const float2*>(row_factor + 8 * j + 2 * c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[j][e] = fmaf(s[j][e], ks[e >> 1] * (e & 1 ? f.y : f.x), lv[e >> 1]);
           }
         }
         nothing = __any_sync(0xffffffffu, nothing);
