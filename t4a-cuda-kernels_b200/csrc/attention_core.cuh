@@ -9,6 +9,13 @@
 // several groups share leaves parts (its output over the part's own softmax sum, and the base-2 log of
 // that sum); k_join weighs them by 2^(lse - max) in a fixed order.  No atomics: the same inputs
 // give the same bits.
+//
+// A product's sums are truncated, not rounded, so that they fall behind by up to half a unit of the last
+// place with every addition: 2048 tiles in a row lost 2.0e-4 of an output in the warp-level kernel and
+// 8.4e-4, four additions a tile, in the one on tensor memory.  A block therefore makes a pass of at most
+// kMmaMostTiles or kTcMostTiles (6e-5 either), and adds up a unit's passes, rounded, in the place of its part.
+// A pass more is a prologue and an epilogue more: 32 sequences of 64-node trees over 16384 tokens, some 570
+// tiles a block in tensor memory, take 1040 us for the 1004 of one pass a unit.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -21,6 +28,7 @@ namespace t4a {
 namespace cache {
 
 constexpr int kTile = 64;
+constexpr int kMmaMostTiles = 512, kTcMostTiles = 128;  // of a pass
 
 struct AttendArgs {
   View cache;
@@ -40,6 +48,8 @@ struct AttendArgs {
   int batch, nodes, group, rows;  // rows = nodes * group
   int row_tiles, tile_rows;
   int places;       // table pages * page_size, or the most that 32 bits allow
+  int most_tiles;   // of a pass
+  int passes;       // whether the tables are long enough for a block to have more than one over a unit
   int tile_pages, tile_places;  // kTile / page_size and kTile % page_size
   int q_bf16;      // q and out are BF16, else F16
   int plain_copies;  // K and V have the same strides, rows fill the padded dim, and offsets fit 32 bits
@@ -69,6 +79,7 @@ __device__ __forceinline__ int sequence_tiles(const AttendArgs& a, int b) {
 struct Cursor {
   int b, head, row_tile;
   int tile, tiles;  // within the unit
+  int from;         // where the block's part of the unit begins
   int left;         // of the block's stretch
 };
 
@@ -125,7 +136,7 @@ __device__ __forceinline__ Cursor find_start(const AttendArgs& a, int block) {
       c.tiles = __shfl_sync(0xffffffffu, mine, at) / units;
       const int in = start - before - __shfl_sync(0xffffffffu, sum - mine, at), unit = in / c.tiles;
       c.b = b0 + at;
-      c.tile = in - unit * c.tiles;
+      c.tile = c.from = in - unit * c.tiles;
       c.head = unit;
       return c;
     }
@@ -135,9 +146,17 @@ __device__ __forceinline__ Cursor find_start(const AttendArgs& a, int block) {
   return c;
 }
 
-// The next unit with tiles; called with left > 0, so there is one.
-__device__ __forceinline__ void next_unit(const AttendArgs& a, Cursor* c) {
-  c->tile = 0;
+// Tiles of the pass that begins at the cursor.
+__device__ __forceinline__ int pass_tiles(const AttendArgs& a, const Cursor& c) {
+  return min(min(c.left, c.tiles - c.tile), a.most_tiles);
+}
+
+// Past a pass of n tiles: the unit's next one, or the next unit with tiles, if any are left.
+__device__ __forceinline__ void next_pass(const AttendArgs& a, Cursor* c, int n) {
+  c->left -= n;
+  c->tile += n;
+  if (c->left <= 0 || c->tile < c->tiles) return;
+  c->tile = c->from = 0;
   if (++c->head < a.cache.heads) return;
   c->head = 0;
   do ++c->b;
@@ -168,6 +187,18 @@ __device__ __forceinline__ void store_out(const AttendArgs& a, long long at, flo
       o[1] = __float2half_rn(y);
     }
   }
+}
+
+// How a pass's results join those of the passes before it, whose sum's logarithm is `before`: both
+// times a weight.  *lse: the pass's, then that of all.
+__device__ __forceinline__ void join_passes(float before, float* lse, float* keep, float* add) {
+  const float most = fmaxf(before, *lse), less = most == -INFINITY ? 0.0f : most;
+  *keep = exp2f(before - less);
+  *add = exp2f(*lse - less);
+  const float sum = *keep + *add, over = sum == 0.0f ? 0.0f : 1.0f / sum;
+  *keep *= over;
+  *add *= over;
+  *lse = sum == 0.0f ? -INFINITY : less + log2f(sum);
 }
 
 constexpr float kLn2 = 0.6931471805599453f;

@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
     int context, live, length;
     sequence_tokens(a, b, &context, &live, &length);
     const int first_row = at.row_tile * kRows;
-    const int tile0 = at.tile, n = min(at.left, at.tiles - at.tile);
+    const int tile0 = at.tile, n = pass_tiles(a, at);
 
     // This lane's token of a tile: K's row for the lower half of the warp, V's for the upper.
     const Pages& side = lane < 16 ? a.cache.k : a.cache.v;
@@ -703,12 +703,14 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
         }
       }
     __syncthreads();
-    const bool begun = tile0 == 0, whole = begun && n == at.tiles;
+    // Whether the block has the unit's first tile, and all; whether passes came before this one.
+    const bool begun = at.from == 0, whole = begun && tile0 + n == at.tiles, again = tile0 != at.from;
     const long long part = (static_cast<long long>(blockIdx.x) * 2 + (begun ? 1 : 0)) * kRows;
-    // A thread takes two columns of a row.
-    for (int k = threadIdx.x; k < kRows * (Dim / 2); k += kMmaThreads) {
-      const int r = k / (Dim / 2), d = 2 * (k - r * (Dim / 2));
-      if (first_row + r >= a.rows || d >= dim) continue;
+    // What the warps' outputs of row r are relative to, their common factor, and the log of the sum.
+    struct RowSum {
+      float less, over, lse2;
+    };
+    auto sum_of = [&](int r) {
       float mo = -INFINITY, ml = -INFINITY;  // references of the output and of the sum
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
@@ -717,38 +719,65 @@ __global__ void __launch_bounds__(kMmaThreads, MmaShape<Kind, Dim, kRowTiles>::p
         ml = fmaxf(ml, kQuantised ? fmaxf(st.x, st.z) : st.x);
       }
       const float less_o = mo == -INFINITY ? 0.0f : mo, less_l = ml == -INFINITY ? 0.0f : ml;
-      float ll = 0.0f, x = 0.0f, y = 0.0f;
+      float ll = 0.0f;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const float4 st = stats[w * kRows + r];
         if (kQuantised && st.w != 0.0f) ll += st.w * exp2_fast(st.z - less_l);
         if (st.x == -INFINITY && st.y == 0.0f) continue;
-        const float weight = exp2_fast(st.x - less_o);
-        const float2 v = *reinterpret_cast<const float2*>(merged + (w * kRows + r) * Shape::out_pitch + d);
         ll += st.y * exp2_fast(st.x - less_l);
-        x += v.x * weight;
-        y += v.y * weight;
       }
-      const int row = first_row + r;
-      const bool dead = row / a.group >= live || ll == 0.0f;
-      const float over = dead ? 0.0f : (mo == ml ? 1.0f : exp2_fast(less_o - less_l)) / ll;
-      const float lse2 = dead ? -INFINITY : less_l + log2f(ll);
-      x = dead ? 0.0f : x * over;
-      y = dead ? 0.0f : y * over;
-      if (whole) {
-        store_out(a, out_row(a, b, at.head, row) + d, x, y);
-        if (d == 0) store_lse(a, b, at.head, row, lse2);
-      } else {
-        *reinterpret_cast<float2*>(a.part_out + (part + r) * dim + d) = make_float2(x, y);
-        if (d == 0) a.part_lse[part + r] = lse2;
+      const bool dead = (first_row + r) / a.group >= live || ll == 0.0f;
+      return RowSum{less_o, dead ? 0.0f : (mo == ml ? 1.0f : exp2_fast(less_o - less_l)) / ll,
+                    dead ? -INFINITY : less_l + log2f(ll)};
+    };
+    auto store_sum = [&](int r, float lse2) {
+      if (whole) store_lse(a, b, at.head, first_row + r, lse2);
+      else a.part_lse[part + r] = lse2;
+    };
+    // A thread takes two columns of a row.
+    for (int k = threadIdx.x; k < kRows * (Dim / 2); k += kMmaThreads) {
+      const int r = k / (Dim / 2), d = 2 * (k - r * (Dim / 2));
+      if (first_row + r >= a.rows || d >= dim) continue;
+      RowSum sum = sum_of(r);
+      float x = 0.0f, y = 0.0f;
+      if (sum.over != 0.0f) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float4 st = stats[w * kRows + r];
+          if (st.x == -INFINITY && st.y == 0.0f) continue;
+          const float weight = exp2_fast(st.x - sum.less);
+          const float2 v = *reinterpret_cast<const float2*>(merged + (w * kRows + r) * Shape::out_pitch + d);
+          x += v.x * weight;
+          y += v.y * weight;
+        }
+        x *= sum.over;
+        y *= sum.over;
       }
+      float2* const kept = reinterpret_cast<float2*>(a.part_out + (part + r) * dim + d);
+      if (again) {
+        float keep, add;
+        join_passes(a.part_lse[part + r], &sum.lse2, &keep, &add);
+        const float2 before = *kept;
+        x = before.x * keep + x * add;
+        y = before.y * keep + y * add;
+      }
+      if (whole) store_out(a, out_row(a, b, at.head, first_row + r) + d, x, y);
+      else *kept = make_float2(x, y);
+      if (d == 0 && !again) store_sum(r, sum.lse2);
     }
     __syncthreads();
-    at.left -= n;
-    if (at.left > 0) {
-      next_unit(a, &at);
-      clear_pads();
+    if (again) {  // the sums before have been read
+      if (threadIdx.x < kRows && first_row + threadIdx.x < a.rows) {
+        RowSum sum = sum_of(threadIdx.x);
+        float keep, add;
+        join_passes(a.part_lse[part + threadIdx.x], &sum.lse2, &keep, &add);
+        store_sum(threadIdx.x, sum.lse2);
+      }
+      __syncthreads();
     }
+    next_pass(a, &at, n);
+    if (at.left > 0) clear_pads();
   }
 }
 

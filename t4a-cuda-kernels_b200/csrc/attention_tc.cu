@@ -6,17 +6,18 @@ namespace t4a {
 namespace cache {
 namespace {
 
-template <int Kind, int Dim>
+template <int Kind, int Dim, bool kPasses>
 int launch_one_tc(const AttendArgs& a, cudaStream_t stream) {
   static std::atomic<unsigned long long> allowed{0};
-  T4A_TRY(runtime::allow_shared(k_attend_tc<Kind, Dim>, TcShape<Dim>::shared, &allowed));
-  return runtime::launch_early<AttendArgs>(k_attend_tc<Kind, Dim>, a.groups * a.row_tiles,
+  T4A_TRY(runtime::allow_shared(k_attend_tc<Kind, Dim, kPasses>, TcShape<Dim>::shared, &allowed));
+  return runtime::launch_early<AttendArgs>(k_attend_tc<Kind, Dim, kPasses>, a.groups * a.row_tiles,
                                            TcRoles<KindOf<Kind>::quantised>::threads, TcShape<Dim>::shared, stream, a);
 }
 
 template <int Kind>
 int launch_kind_tc(const AttendArgs& a, int padded, cudaStream_t stream) {
-  return padded == 64 ? launch_one_tc<Kind, 64>(a, stream) : launch_one_tc<Kind, 128>(a, stream);
+  if (padded == 64) return a.passes ? launch_one_tc<Kind, 64, true>(a, stream) : launch_one_tc<Kind, 64, false>(a, stream);
+  return a.passes ? launch_one_tc<Kind, 128, true>(a, stream) : launch_one_tc<Kind, 128, false>(a, stream);
 }
 
 }  // namespace

@@ -73,6 +73,7 @@ __device__ __forceinline__ const unsigned* flags_of(const Flags* f) {
 // Scales that change nothing, for scores that have had theirs.
 struct alignas(16) TcNeutral {
   float ones[kTile], zeros[kTile];
+  float keep[kTcRows];        // the weight of a row's passes before this one
   long long row_at[kTcRows];  // and where the unit's rows of q lie, -1 for none
 };
 
@@ -327,7 +328,8 @@ __device__ __forceinline__ uint32_t scaled_pair(uint32_t pair, float x) {
 // such a tile's rows and writes the slot's `odd`, the other reads it.
 __device__ __forceinline__ bool holds_drafts(int tile, int context) { return (tile + 1) * kTile > context; }
 
-template <int Kind, int Dim>
+// `kPasses`: whether a block may have more than one pass over a unit, which costs the others 2%.
+template <int Kind, int Dim, bool kPasses>
 __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcShape<Dim>::per_sm) k_attend_tc(const AttendArgs a) {
   using Shape = TcShape<Dim>;
   constexpr bool kQuantised = KindOf<Kind>::quantised, kBf16 = KindOf<Kind>::bf16;
@@ -343,6 +345,7 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
   TcSlot<Flags>* const slots = reinterpret_cast<TcSlot<Flags>*>(smem + Shape::slots_at);
   float* const ones = reinterpret_cast<TcNeutral*>(smem + Shape::neutral_at)->ones;
   float* const zeros = reinterpret_cast<TcNeutral*>(smem + Shape::neutral_at)->zeros;
+  float* const keeps = reinterpret_cast<TcNeutral*>(smem + Shape::neutral_at)->keep;
   long long* const row_at = reinterpret_cast<TcNeutral*>(smem + Shape::neutral_at)->row_at;
   TcBarriers* const bar = reinterpret_cast<TcBarriers*>(smem + Shape::barriers_at);
   unsigned* const tmem_at = reinterpret_cast<unsigned*>(bar + 1);
@@ -431,7 +434,7 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
       const int b = at.b;
       int context, live, length;
       sequence_tokens(a, b, &context, &live, &length);
-      const int n = min(at.left, at.tiles - at.tile);
+      const int n = kPasses ? pass_tiles(a, at) : min(at.left, at.tiles - at.tile);
       const unsigned char* const base = mine.base + at.head * mine.head;
       const int* const my_table = a.table + b * a.table_batch;
       int pos = at.tile * kTile + first_token + lane % kTokens;  // the lane's token of the next tile to look up
@@ -592,8 +595,7 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
         if (kQuantised && i + 1 < n) fetch();
       }
       tiles_done += n;
-      at.left -= n;
-      if (at.left > 0) next_unit(a, &at);
+      next_pass(a, &at, n);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp >= kIssueWarp) {
@@ -634,7 +636,7 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
       bool good = true;
       unsigned unit = 0;
       while (at.left > 0 && good) {
-        const int n = min(at.left, at.tiles - at.tile), t0 = tiles_done;
+        const int n = kPasses ? pass_tiles(a, at) : min(at.left, at.tiles - at.tile), t0 = tiles_done;
         good = ready(&bar->q_full, unit & 1) && ready(k_barrier(t0), stage_parity(t0));
         if (good && elected()) scores(t0);
         if (good && n > 1) {
@@ -653,8 +655,7 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
         }
         tiles_done += n;
         ++unit;
-        at.left -= n;
-        if (at.left > 0) next_unit(a, &at);
+        next_pass(a, &at, n);
       }
     }
     __syncwarp();
@@ -668,7 +669,7 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
       const int b = at.b;
       int context, live, length;
       sequence_tokens(a, b, &context, &live, &length);
-      const int n = min(at.left, at.tiles - at.tile);
+      const int n = kPasses ? pass_tiles(a, at) : min(at.left, at.tiles - at.tile);
       const int row = at.row_tile * kTcRows + r, node = row / a.group;
       const bool here = row < a.rows && node < live, any_here = __any_sync(0xffffffffu, here);
       // A negative scale is Q's sign, so that the largest product is the largest score.
@@ -938,7 +939,8 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
       tiles_done += n;
       if (good) good = barrier_wait(&bar->o_done[(tiles_done - 1) & 1], ((tiles_done - 1) >> 1) & 1, failed);
       tc_after();
-      const bool begun = at.tile == 0, whole = begun && n == at.tiles;
+      // Whether the block has the unit's first tile, and all; whether passes came before this one.
+      const bool begun = at.from == 0, whole = begun && at.tile + n == at.tiles, again = kPasses && at.tile != at.from;
       // Sums relative to the larger reference; O stays relative to its own.
       const float mo = m == -INFINITY ? 0.0f : less;
       const float ml = kQuantised ? fmaxf(m == -INFINITY ? -INFINITY : less, mz) : (m == -INFINITY ? -INFINITY : less);
@@ -950,14 +952,21 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
       float lse2 = dead ? -INFINITY : less_l + log2f(ll);
       if (!good) over = lse2 = __uint_as_float(0x7fc00000u);
       const long long part = (static_cast<long long>(blockIdx.x) * 2 + (begun ? 1 : 0)) * kTcRows;
+      if (again && row < a.rows) {
+        float keep, add;
+        join_passes(a.part_lse[part + r], &lse2, &keep, &add);
+        over *= add;
+        keeps[r] = keep;
+      }
       if (row < a.rows) {
         if (whole) store_lse(a, b, at.head, row, lse2);
         else a.part_lse[part + r] = lse2;
       }
       // Results through Q's lines, which no product reads any more, so that a warp writes whole rows:
-      // 16-bit results all at once, parts in F32 by halves of a row's line block.
+      // 16-bit results all at once; parts, and what joins passes before it, in F32 by halves of a row's
+      // line block.
       row_at[r] = row < a.rows ? (whole ? out_row(a, b, at.head, row) : (part + r) * dim) : -1;
-      if (whole) {
+      if (whole && !again) {
 #pragma unroll 1
         for (int d = 0; d < Dim; d += 16) {
           uint32_t o[16], h[8];
@@ -1015,7 +1024,26 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
           }
           asm volatile("bar.sync 1, 128;" ::: "memory");
           const int unit = r % 16;  // of 4 values
-          if (half + 4 * unit < dim) {
+          if (again && half + 4 * unit < dim) {
+            // What the passes before have left, by the same thread, and this one's.
+#pragma unroll 1
+            for (int of = r / 16; of < kTcRows; of += 8) {
+              const long long to = row_at[of];
+              if (to < 0) continue;
+              float4* const kept = reinterpret_cast<float4*>(a.part_out + (part + of) * dim + half + 4 * unit);
+              const float4 before = *kept;
+              float4 x = *reinterpret_cast<const float4*>(part_lines + of * 256 + ((unit ^ (of & 7)) << 4));
+              const float keep = keeps[of];
+              x = make_float4(fmaf(before.x, keep, x.x), fmaf(before.y, keep, x.y), fmaf(before.z, keep, x.z),
+                              fmaf(before.w, keep, x.w));
+              if (whole) {
+                store_out(a, to + half + 4 * unit, x.x, x.y);
+                store_out(a, to + half + 4 * unit + 2, x.z, x.w);
+              } else {
+                *kept = x;
+              }
+            }
+          } else if (half + 4 * unit < dim) {
 #pragma unroll 4
             for (int u = 0; u < 16; ++u) {
               const int of = u * 8 + r / 16;
@@ -1029,8 +1057,7 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
         }
       }
       tc_before();
-      at.left -= n;
-      if (at.left > 0) next_unit(a, &at);
+      next_pass(a, &at, n);
     }
   }
   __syncthreads();

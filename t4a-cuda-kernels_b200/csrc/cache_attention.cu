@@ -182,16 +182,18 @@ int plan_attention(int dtype, const t4a_kv_cache* cache, const t4a_cuda_layout* 
   if (tiles > INT_MAX || batch * a->cache.heads * a->rows > INT_MAX) return T4A_ERR_DOMAIN_TOO_LARGE;
   *choice = choose(cache->kind, a->cache.dim, a->rows, tiles);
   a->tile_rows = choice->rows;
+  a->most_tiles = choice->row_tiles == 0 ? kTcMostTiles : kMmaMostTiles;
   a->row_tiles = (a->rows + choice->rows - 1) / choice->rows;
   int blocks;
   T4A_TRY(dispatch(cache->kind, *a, *choice, nullptr, &blocks));
   a->groups = a->row_tiles < blocks ? blocks / a->row_tiles : 1;
+  a->passes = tiles > static_cast<long long>(a->groups) * a->most_tiles;
   return T4A_OK;
 }
 
-// Parts, where there is more than one group to share a unit.
+// Parts, where there is more than one group to share a unit or more than one pass over it.
 size_t part_rows(const AttendArgs& a) {
-  return a.groups > 1 ? static_cast<size_t>(a.groups) * a.row_tiles * 2 * a.tile_rows : 4;
+  return a.groups > 1 || a.passes ? static_cast<size_t>(a.groups) * a.row_tiles * 2 * a.tile_rows : 4;
 }
 
 size_t workspace_of(const AttendArgs& a) { return part_rows(a) * (a.cache.dim + 1) * sizeof(float); }
