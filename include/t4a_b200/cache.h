@@ -76,7 +76,7 @@ int t4a_cache_read(void* stream, int dtype, int index_dtype, const t4a_kv_cache*
  *     cache heads).
  *   table: I32, layout axes pages of a sequence, batch.  A page outside the cache is not seen.
  *   context: I32 [batch], committed tokens; node j's row is at place context + j.  Places
- *     past the table are not seen; a negative context counts as 0.
+ *     past the table, and from 2^31 - 257 on, are not seen; a negative context counts as 0.
  *   nodes: I32 [batch], live nodes of each sequence, or NULL for all; the others see nothing
  *     and are not seen.
  *   mask: BOOL, layout axes seen node j, node i, batch (any strides, 0 among them): whether

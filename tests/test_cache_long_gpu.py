@@ -63,3 +63,21 @@ def test_units_of_several_passes(cuda, kind, dtype, nodes, group, dim):
     assert torch.equal(lse == -torch.inf, empty)
     off = (lse.double() - want_lse[some]).abs() / (2.0 ** -18 * (size + want_lse.abs() + 1))[some]
     assert float(off[~empty].max()) <= 1
+
+
+@pytest.mark.parametrize("nodes,group", [(1, 4), (20, 2)])
+def test_places_near_the_most(cuda, nodes, group):
+    """2047 entries of a table that lead to one page of 2^20 places: sequences whose places almost fill 31 bits."""
+    page, dim = 1 << 20, 64
+    gen = generator(nodes)
+    k, v, ks, vs = ref.random_cache(gen, 1, page, 1, dim, torch.int8)
+    q = torch.randn(1, nodes, group, dim, generator=gen, device="cuda").half()
+    table = torch.zeros(1, 2047, dtype=torch.int32, device="cuda")
+    context = torch.full((1,), 2047 * page - nodes, dtype=torch.int32, device="cuda")
+    sees = torch.ones(1, nodes, nodes, dtype=torch.bool, device="cuda")
+    out, lse = t4.tree_attention(q, k, v, table, context, mask=sees, k_scale=ks, v_scale=vs)
+    want, want_lse, spread, size = ref.attention(q, k, v, ks, vs, table[:, :1], torch.full((1,), page - nodes), sees,
+                                                 torch.full((1,), nodes), dim ** -0.5)
+    assert float(((out.double() - want).abs() / spread).max()) <= 2 * UNIT[F16] + 2.0 ** -13
+    off = (lse.double() - want_lse - math.log(2047)).abs()
+    assert float((off / (size + want_lse.abs() + 1)).max()) <= 2.0 ** -18
