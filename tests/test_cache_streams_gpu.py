@@ -64,3 +64,26 @@ def test_results_never_require_a_gradient(cuda):
     out, lse = t4.tree_attention(q, k, v, torch.arange(4, dtype=torch.int32, device="cuda")[None],
                                  torch.full((1,), 18, dtype=torch.int32, device="cuda"))
     assert not any(t.requires_grad for t in (k, v, out, lse, *t4.cache_read(k, v, slots, torch.float32)))
+
+
+@pytest.mark.parametrize("batch,nodes,group", [(1, 1, 4), (5, 20, 2), (40, 2, 4)])
+def test_lengths_written_right_before_a_call(cuda, batch, nodes, group):
+    """The attention's kernels are set up while the one that writes the contexts still runs."""
+    gen = torch.Generator(device="cuda").manual_seed(batch)
+    k, v = (torch.randn(batch * 40, 16, 2, 64, generator=gen, device="cuda").half() for _ in range(2))
+    table = torch.randperm(batch * 40, generator=gen, device="cuda").view(batch, 40).int()
+    q = torch.randn(batch, nodes, 2 * group, 64, generator=gen, device="cuda").half()
+    steps = torch.randint(0, 600, (50, batch), generator=gen, device="cuda", dtype=torch.int32)
+    live = torch.randint(0, nodes + 1, (50, batch), generator=gen, device="cuda", dtype=torch.int32)
+    want = []
+    for i in range(50):
+        torch.cuda.synchronize()
+        want.append(t4.tree_attention(q, k, v, table, steps[i], nodes=live[i]))
+        torch.cuda.synchronize()
+    context, now = torch.zeros(batch, dtype=torch.int32, device="cuda"), torch.zeros_like(live[0])
+    got = []
+    for i in range(50):
+        context.copy_(steps[i])
+        now.copy_(live[i])
+        got.append(t4.tree_attention(q, k, v, table, context, nodes=now))
+    assert all(torch.equal(a, b) for x, y in zip(got, want) for a, b in zip(x, y))
