@@ -9,7 +9,9 @@
 // for each row;  O = O * 2^(m_old - m) + 2^(S - m) V.  m moves only where a new maximum exceeds it
 // by 2^8, so the multiplications of O are rare, and weights carry a further 2^7: they reach from
 // 2^15 down, so that F16 keeps all bits of those that are 2^-21 of the largest.  O / l depends on
-// neither.
+// neither.  Weights take V's 16-bit type, F16 over codes, since both operands of a product have one: an
+// output is off by its unit roundoff of sum w|v| at most.  l adds them as they were, in F32, so that the
+// log-sum-exp has no part in that.
 //
 // Each of a block's 4 warps takes 16 of a tile's 64 tokens, and copies just these (cp.async, 16
 // bytes a lane) into its part of a ring of stages; no warp waits for another within a unit.  The

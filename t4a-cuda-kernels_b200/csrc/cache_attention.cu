@@ -13,7 +13,8 @@ constexpr int kJoinThreads = 128, kJoinWarps = kJoinThreads / 32;
 // unit; zeros where the sequence has nothing to see; else its parts weighed by 2^(lse - max), in a
 // fixed order.  kWarps warps take a row's parts in turn: one where units have a few parts, four
 // where a long sequence has dozens, which then come in a few rounds of loads.  Launched beside the
-// attention, it finds its place on the line of tiles while that runs.
+// attention, it finds its place on the line of tiles while that runs: the attention lets it start only
+// behind its own wait for the kernels before, which may have written the lengths.
 template <int kWarps>
 __global__ void __launch_bounds__(kJoinThreads) k_join(const AttendArgs a) {
   __shared__ float sums[kWarps == 1 ? 1 : kWarps][kMaxDim], weights[kWarps], tops[kWarps];
@@ -114,7 +115,8 @@ struct Choice {
 // rows 120 against 87.
 // At 131072 tokens in int8 and 32 rows: 119 against 166.  What the warp-level kernel pays for a
 // unit, joining its warps' outputs, is most of a call whose blocks have a few tiles each, so 17 to 32
-// rows of codes go by the tiles of all tables, 8 heads, 32 rows, in E4M3 and in int8: 4 sequences of up
+// rows of codes go by the tiles that all tables hold (lengths are on the device: a table much wider than
+// its sequences goes to the warp-level kernel, however short they are); 8 heads, 32 rows, in E4M3 and in int8: 4 sequences of up
 // to 4096 (2048 tiles) 58 against 44 and 52 against 40, 7 of up to 4099 (3640) 64 against 56 and 58
 // against 50, 16 of 2048 (4096) 73 against 75 and 67 against 65, 16 of 4096 (8192) 97 against 120 and
 // 91 against 104.  (Not at dim 96, which tensor memory pads to 128: 7 of up to 4099 in E4M3 take 52

@@ -42,7 +42,7 @@ int allow_shared(Kernel kernel, int bytes, std::atomic<unsigned long long>* done
 }
 
 // Launches a kernel that may be set up while the stream's previous one ends; it waits for that one
-// (griddepcontrol.wait) before it touches memory.
+// (griddepcontrol.wait) before it writes memory or reads what that one writes.
 template <typename Args>
 int launch_early(void (*kernel)(Args), unsigned grid, unsigned block, size_t shared, cudaStream_t stream,
                  const Args& args) {
