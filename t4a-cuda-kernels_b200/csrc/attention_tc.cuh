@@ -848,11 +848,17 @@ __global__ void __launch_bounds__(TcRoles<KindOf<Kind>::quantised>::threads, TcS
             if (__any_sync(0xffffffffu, rises)) {
               float shrink = 1.0f;
               if (rises) {
-                // References are whole numbers, so that weights and outputs shrink by powers of two: exactly.
-                const float to = ceilf(top), by = m - to;
-                shrink = by < -126.0f ? 0.0f : __uint_as_float(static_cast<unsigned>(static_cast<int>(by) + 127) << 23);
-                m = to;
-                less = to - kLift;
+                // The reference is the maximum, whose weight is exact then; but where the tile's first
+                // weights are 16 bits already it moves by whole numbers, so that they shrink exactly.
+                const float steps = ceilf(top - m);
+                if (kSides == 1 && half == 1 && steps <= 126.0f) {
+                  shrink = __uint_as_float(static_cast<unsigned>(127 - static_cast<int>(steps)) << 23);
+                  m += steps;
+                } else {
+                  shrink = exp2_fast(m - top);
+                  m = top;
+                }
+                less = m - kLift;
                 l4[0] *= shrink, l4[1] *= shrink, l4[2] *= shrink, l4[3] *= shrink;
               }
               if (kSides == 1 && half == 1) {
