@@ -27,10 +27,10 @@
 // largest magnitude is outside [1/4, 2^15) is first brought to [2^14, 2^15) by a power of two of its own,
 // which its scores are multiplied by again: a row keeps 23 bits of its largest, whatever the block's
 // other rows hold.  Rows without a live node are zeros.
-// 32 sequences of up to 8192 tokens in I8, 4 rows a cache head, 353 MB: 71 us, 5.0 TB/s, 0.77 of a
-// copy's rate; the issue slots are 0.59 taken, DRAM reads 364 MB.  8 nodes over 131072 tokens in
-// I8, 32 rows, 277 MB: 115 us; there the unpacking and 64 products to 16 tokens with two blocks an
-// SM bound it (issue 0.42, most stalls on fixed latencies).  One token over 1000, BF16: 7 us.
+// 32 sequences of up to 8192 tokens in I8, 4 rows a cache head, 353 MB: 70 us, 5.0 TB/s, 0.77 of a
+// copy's rate; the issue slots are 0.60 taken, DRAM reads 364 MB.  8 nodes over 131072 tokens in
+// I8, 32 rows, 277 MB: 120 us; there the unpacking and 64 products to 16 tokens with two blocks an
+// SM bound it (issue 0.43, most stalls on fixed latencies).  One token over 1000, BF16: 8.6 us.
 // ldmatrix moves pairs of codes, so a thread's codes are not where 16-bit values would be:
 //   K: a thread's 4 neighbouring codes serve as k = 2c, 2c+1, 2c+8, 2c+9, and Q has the same order;
 //   V (transposed): a register holds codes d, d+1 of tokens t, t+1; byte permutes make the pairs

@@ -18,10 +18,10 @@
 // the issuing thread by itself (`lane == 0`), each product and wait was serialised over the warp and
 // bound the tile: 170 us for the 155 of a call below; and halves of 32 tokens at a time took 159.
 // Packed F32 operations, and K and V by the same warps (228 for 168 then), were slower.
-// 4 sequences of up to 16384 tokens, 512 rows a cache head, BF16, 99 GFLOP: 146 us, 680 TFLOP/s,
-// 0.41 of a library product's rate; tensor pipe 0.34, DRAM reads 202 MB,
+// 4 sequences of up to 16384 tokens, 512 rows a cache head, BF16, 99 GFLOP: 148 us, 670 TFLOP/s,
+// 0.41 of a library product's rate; tensor pipe 0.33, DRAM reads 203 MB,
 // each cache row once.
-// 7 trees of 13 nodes over 4099 tokens, E4M3, 39 rows: 34 us, of which a block's five tiles are half;
+// 7 trees of 13 nodes over 4099 tokens, E4M3, 39 rows: 38 us, of which a block's five tiles are half;
 // there unpacking bounds a tile (some 4500 cycles).
 //
 // Shared rows of Q, K and V are 128-byte lines of 64 values, their 16-byte units XORed with the
