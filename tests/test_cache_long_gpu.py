@@ -10,7 +10,7 @@ import torch
 
 import cache_reference as ref
 import t4a_b200 as t4
-from test_cache_gpu import BF16, F16, KINDS, UNIT, attention_case, generator
+from test_cache_gpu import BF16, E4M3, F16, I8, KINDS, UNIT, attention_case, check_attention, generator
 
 pytestmark = pytest.mark.gpu
 
@@ -81,3 +81,10 @@ def test_places_near_the_most(cuda, nodes, group):
     assert float(((out.double() - want).abs() / spread).max()) <= 2 * UNIT[F16] + 2.0 ** -13
     off = (lse.double() - want_lse - math.log(2047)).abs()
     assert float((off / (size + want_lse.abs() + 1)).max()) <= 2.0 ** -18
+
+
+@pytest.mark.parametrize("kind,dtype,nodes,group,dim,context", [(I8, BF16, 300, 128, 64, 9000), (F16, F16, 300, 128, 64, 9000),
+                                                                (E4M3, F16, 40, 120, 256, 33000), (BF16, BF16, 40, 120, 256, 33000)])
+def test_several_passes_of_more_row_tiles_than_blocks(cuda, kind, dtype, nodes, group, dim, context):
+    """Every tile of query rows has a block of its own, which goes over the whole cache in passes."""
+    check_attention(attention_case(dim, 1, nodes, 1, group, dim, 64, [context], kind, dtype))
